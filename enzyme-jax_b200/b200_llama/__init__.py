@@ -38,7 +38,9 @@ EXPORTS = (
     "b200_token_vjp_workspace_bytes", "b200_token_vjp", "b200_comm_init_rank_ex", "b200_comm_setup_peer_memory",
     "b200_comm_attach_memory", "b200_tp_exchange_buffers", "b200_tp_reduce_norm", "b200_token_forward",
     "b200_static_sizes", "b200_jvp_workspace_bytes", "b200_forward_jvp", "b200_token_jvp_workspace_bytes",
-    "b200_token_jvp", "b200_plan_set_option", "b200_plan_get_option",
+    "b200_token_jvp", "b200_plan_set_option", "b200_plan_get_option", "b200_attention_packed",
+    "b200_attention_packed_backward", "b200_kv4_append", "b200_kv4_read", "b200_attention_decode_kv4_scratch_bytes",
+    "b200_attention_decode_kv4", "b200_copy_pages",
 )
 
 
@@ -131,6 +133,14 @@ def lib() -> ctypes.CDLL:
                                           c_void_p]
         l.b200_comm_destroy.argtypes = [c_void_p]
         l.b200_comm_peer_memory.argtypes = [c_void_p, POINTER(c_int32)]
+        l.b200_attention_packed.argtypes = [c_void_p] * 6 + [c_int32] * 11 + [c_void_p]
+        l.b200_attention_packed_backward.argtypes = [c_void_p] * 11 + [c_int32] * 15 + [c_void_p]
+        l.b200_kv4_append.argtypes = [c_void_p] * 7 + [c_int32] * 10 + [c_void_p]
+        l.b200_kv4_read.argtypes = [c_void_p] * 7 + [c_int32] * 10 + [c_void_p]
+        l.b200_attention_decode_kv4_scratch_bytes.argtypes = [c_int32] * 4 + [POINTER(c_size_t)]
+        l.b200_attention_decode_kv4.argtypes = [c_void_p] * 7 + [c_size_t] + [c_int32] * 11 + [c_void_p]
+        l.b200_copy_pages.argtypes = [c_void_p] + [c_int32] * 5 + [c_void_p] * 3 + [c_int32, c_void_p, ctypes.c_int64,
+                                                                                  c_void_p, c_void_p]
         _lib = l
     return _lib
 
@@ -282,6 +292,334 @@ def attention_decode_static(q: torch.Tensor, kv_layer: torch.Tensor, page_table:
 
 
 # --------------------------------------------------------------------------
+# packed prompts, the 4-bit cache, page copies
+# --------------------------------------------------------------------------
+
+def _device_of(what: str, **tensors):
+    """The one CUDA device all given tensors are on."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise B200Error(1, f"{what}: {name} must be a CUDA tensor")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise B200Error(1, f"{what}: {name} is on {t.device}, the others on {dev}")
+    return dev
+
+
+class _On:
+    """Makes ``device`` current for a call, so that the stream and the launches are that device's."""
+
+    def __init__(self, device):
+        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+        return _stream()
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+        return False
+
+
+def _rows(what: str, name: str, t: torch.Tensor, cols: int, rows: Optional[int] = None,
+          dtype: Optional[torch.dtype] = None) -> int:
+    """Row pitch of a [rows, cols] tensor with unit column stride."""
+    if t.dim() != 2 or t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
+        raise B200Error(2, f"{what}: {name} has shape {tuple(t.shape)}, expected [{'rows' if rows is None else rows}, {cols}]")
+    if dtype is not None and t.dtype != dtype:
+        raise B200Error(3, f"{what}: {name} is {t.dtype}, expected {dtype}")
+    if t.shape[0] <= 1:
+        if cols > 1 and t.shape[0] == 1 and t.stride(1) != 1:
+            raise B200Error(2, f"{what}: {name} needs unit column stride")
+        return max(cols, 1)
+    if t.stride(1) != 1 or t.stride(0) < cols:
+        raise B200Error(2, f"{what}: {name} needs unit column stride and rows that do not overlap")
+    return t.stride(0)
+
+
+def _index(what: str, name: str, t: torch.Tensor, dim: int = 1) -> None:
+    if t.dtype != torch.int32 or t.dim() != dim or not t.is_contiguous():
+        raise B200Error(3, f"{what}: {name} must be a contiguous int32 tensor of {dim} dimension(s)")
+
+
+def _heads(what: str, q: torch.Tensor, n_heads: int, n_kv_heads: int) -> int:
+    if n_heads <= 0 or n_kv_heads <= 0 or n_heads % n_kv_heads or q.dim() != 2 or q.shape[1] % n_heads:
+        raise B200Error(2, f"{what}: {n_heads} query heads over {n_kv_heads} key heads do not fit q {tuple(q.shape)}")
+    return q.shape[1] // n_heads
+
+
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, n_heads: int,
+                     n_kv_heads: Optional[int] = None, *, impl: int = 0, out: Optional[torch.Tensor] = None,
+                     lse: Optional[torch.Tensor] = None):
+    """Causal attention over packed sequences of different lengths, with grouped heads.
+
+    ``q`` [rows, n_heads*hs], ``k`` and ``v`` [rows, n_kv_heads*hs] (strided row views are fine); ``cu_seqlens`` int32
+    [n_seqs + 1] on the device: sequence s owns rows cu_seqlens[s] .. cu_seqlens[s+1]-1.  Returns ``(o, lse)`` with lse
+    fp32 [n_heads, rows].  Rows of no sequence are not written: give ``out`` / ``lse`` to choose what stands there."""
+    what = "attention_packed"
+    n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
+    dev = _device_of(what, q=q, k=k, v=v, cu_seqlens=cu_seqlens, out=out, lse=lse)
+    hs = _heads(what, q, n_heads, n_kv_heads)
+    rows, dt = q.shape[0], q.dtype
+    ldq = _rows(what, "q", q, n_heads * hs)
+    ldk = _rows(what, "k", k, n_kv_heads * hs, rows, dt)
+    ldv = _rows(what, "v", v, n_kv_heads * hs, rows, dt)
+    _index(what, "cu_seqlens", cu_seqlens)
+    if cu_seqlens.numel() < 1:
+        raise B200Error(2, f"{what}: cu_seqlens holds n_seqs + 1 entries, at least one")
+    if out is None:
+        out = torch.empty(rows, n_heads * hs, dtype=dt, device=dev)
+    ldo = _rows(what, "out", out, n_heads * hs, rows, dt)
+    if lse is None:
+        lse = torch.empty(n_heads, rows, dtype=torch.float32, device=dev)
+    elif lse.dtype != torch.float32 or tuple(lse.shape) != (n_heads, rows) or not lse.is_contiguous():
+        raise B200Error(2, f"{what}: lse must be a contiguous fp32 [{n_heads}, {rows}]")
+    with _On(dev) as stream:
+        check(lib().b200_attention_packed(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                                          cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, rows, n_heads, n_kv_heads, hs,
+                                          ldq, ldk, ldv, ldo, _dt(dt), impl, stream))
+    return out, lse
+
+
+def attention_packed_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
+                              d_o: torch.Tensor, cu_seqlens: torch.Tensor, n_heads: int,
+                              n_kv_heads: Optional[int] = None, *, impl: int = 0, dq: Optional[torch.Tensor] = None,
+                              dk: Optional[torch.Tensor] = None, dv: Optional[torch.Tensor] = None):
+    """Reverse mode of :func:`attention_packed`: returns ``(dq, dk, dv)`` of the layouts and dtype of q, k, v; dk and dv
+    are summed over the query heads of a group.  Rows of no sequence are not written."""
+    what = "attention_packed_backward"
+    n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
+    dev = _device_of(what, q=q, k=k, v=v, o=o, lse=lse, d_o=d_o, cu_seqlens=cu_seqlens, dq=dq, dk=dk, dv=dv)
+    hs = _heads(what, q, n_heads, n_kv_heads)
+    rows, dt = q.shape[0], q.dtype
+    wq, wk = n_heads * hs, n_kv_heads * hs
+    ldq = _rows(what, "q", q, wq)
+    ldk = _rows(what, "k", k, wk, rows, dt)
+    ldv = _rows(what, "v", v, wk, rows, dt)
+    ldo = _rows(what, "o", o, wq, rows, dt)
+    lddo = _rows(what, "d_o", d_o, wq, rows, dt)
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (n_heads, rows) or not lse.is_contiguous():
+        raise B200Error(2, f"{what}: lse must be a contiguous fp32 [{n_heads}, {rows}]")
+    _index(what, "cu_seqlens", cu_seqlens)
+    if cu_seqlens.numel() < 1:
+        raise B200Error(2, f"{what}: cu_seqlens holds n_seqs + 1 entries, at least one")
+    dq = torch.empty(rows, wq, dtype=dt, device=dev) if dq is None else dq
+    dk = torch.empty(rows, wk, dtype=dt, device=dev) if dk is None else dk
+    dv = torch.empty(rows, wk, dtype=dt, device=dev) if dv is None else dv
+    lddq = _rows(what, "dq", dq, wq, rows, dt)
+    lddk = _rows(what, "dk", dk, wk, rows, dt)
+    lddv = _rows(what, "dv", dv, wk, rows, dt)
+    delta = torch.empty(n_heads * rows, dtype=torch.float32, device=dev)
+    with _On(dev) as stream:
+        check(lib().b200_attention_packed_backward(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), d_o.data_ptr(), dq.data_ptr(),
+            dk.data_ptr(), dv.data_ptr(), delta.data_ptr(), cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, rows, n_heads,
+            n_kv_heads, hs, ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv, _dt(dt), impl, stream))
+    return dq, dk, dv
+
+
+def new_kv4_pages(n_layers: int, n_pages: int, n_kv_heads: int, page_size: int, head_size: int, device="cuda"):
+    """Pools of a 4-bit key/value cache: ``codes`` uint8 [n_layers, 2, n_pages, n_kv_heads, page_size, head_size/2] and
+    ``params`` bf16 [n_layers, 2, n_pages, n_kv_heads, page_size, 2] (scale, minimum).  A row stands for
+    minimum + scale * code.  ``codes[l], params[l]`` is one layer, what the kv4 functions take."""
+    if head_size % 2:
+        raise B200Error(2, f"head size {head_size} is odd")
+    codes = torch.zeros(n_layers, 2, n_pages, n_kv_heads, page_size, head_size // 2, dtype=torch.uint8, device=device)
+    params = torch.zeros(n_layers, 2, n_pages, n_kv_heads, page_size, 2, dtype=torch.bfloat16, device=device)
+    return codes, params
+
+
+def _kv4_layer(what: str, codes: torch.Tensor, params: torch.Tensor):
+    if codes.dim() != 5 or codes.shape[0] != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous():
+        raise B200Error(2, f"{what}: codes must be a contiguous uint8 [2, n_pages, n_kv_heads, page_size, hs/2]")
+    if params.dtype != torch.bfloat16 or tuple(params.shape) != tuple(codes.shape[:4]) + (2,) or not params.is_contiguous():
+        raise B200Error(2, f"{what}: params must be a contiguous bf16 {tuple(codes.shape[:4]) + (2,)}")
+    _, n_pages, n_kv_heads, page_size, half = codes.shape
+    return n_pages, n_kv_heads, page_size, 2 * half
+
+
+def _kv4_rows(what: str, page_table: torch.Tensor, cu_seqlens: torch.Tensor, ctx_before: Optional[torch.Tensor]) -> int:
+    _index(what, "page_table", page_table, 2)
+    _index(what, "cu_seqlens", cu_seqlens)
+    n_seqs = page_table.shape[0]
+    if cu_seqlens.numel() != n_seqs + 1:
+        raise B200Error(2, f"{what}: cu_seqlens has {cu_seqlens.numel()} entries for {n_seqs} page-table rows")
+    if ctx_before is not None:
+        _index(what, "ctx_before", ctx_before)
+        if ctx_before.numel() != n_seqs:
+            raise B200Error(2, f"{what}: ctx_before has {ctx_before.numel()} entries for {n_seqs} sequences")
+    return n_seqs
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, page_table: torch.Tensor,
+               cu_seqlens: torch.Tensor, ctx_before: Optional[torch.Tensor] = None) -> None:
+    """Quantises the packed rows k, v [rows, n_kv_heads*hs] into one layer of a 4-bit cache.  Row t of sequence s becomes
+    its cached row ``ctx_before[s] + t - cu_seqlens[s]`` (``ctx_before`` None: the sequences start empty).  Rows without
+    a place (behind the page table, or a page id outside the pool) are skipped and make :func:`device_status` raise."""
+    what = "kv4_append"
+    dev = _device_of(what, k=k, v=v, codes=codes, params=params, page_table=page_table, cu_seqlens=cu_seqlens,
+                     ctx_before=ctx_before)
+    n_pages, n_kv_heads, page_size, hs = _kv4_layer(what, codes, params)
+    n_seqs = _kv4_rows(what, page_table, cu_seqlens, ctx_before)
+    ldk = _rows(what, "k", k, n_kv_heads * hs)
+    ldv = _rows(what, "v", v, n_kv_heads * hs, k.shape[0], k.dtype)
+    with _On(dev) as stream:
+        check(lib().b200_kv4_append(k.data_ptr(), v.data_ptr(), codes.data_ptr(), params.data_ptr(),
+                                    page_table.data_ptr(), cu_seqlens.data_ptr(), _ptr(ctx_before), n_seqs, k.shape[0],
+                                    n_kv_heads, hs, ldk, ldv, n_pages, page_size, page_table.shape[1], _dt(k.dtype),
+                                    stream))
+
+
+def kv4_read(codes: torch.Tensor, params: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
+             ctx_before: Optional[torch.Tensor], rows: int, *, dtype: torch.dtype = torch.bfloat16,
+             k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None):
+    """Reads cached rows back as packed k, v [rows, n_kv_heads*hs]: the way back of :func:`kv4_append` with the same
+    ``cu_seqlens`` and ``ctx_before``, e.g. the keys of a shared prefix for :func:`attention_packed`.  Rows without a
+    place are not written."""
+    what = "kv4_read"
+    dev = _device_of(what, codes=codes, params=params, page_table=page_table, cu_seqlens=cu_seqlens,
+                     ctx_before=ctx_before, k=k, v=v)
+    n_pages, n_kv_heads, page_size, hs = _kv4_layer(what, codes, params)
+    n_seqs = _kv4_rows(what, page_table, cu_seqlens, ctx_before)
+    k = torch.empty(rows, n_kv_heads * hs, dtype=dtype, device=dev) if k is None else k
+    v = torch.empty(rows, n_kv_heads * hs, dtype=dtype, device=dev) if v is None else v
+    ldk = _rows(what, "k", k, n_kv_heads * hs, rows, dtype)
+    ldv = _rows(what, "v", v, n_kv_heads * hs, rows, dtype)
+    with _On(dev) as stream:
+        check(lib().b200_kv4_read(k.data_ptr(), v.data_ptr(), codes.data_ptr(), params.data_ptr(),
+                                  page_table.data_ptr(), cu_seqlens.data_ptr(), _ptr(ctx_before), n_seqs, rows,
+                                  n_kv_heads, hs, ldk, ldv, n_pages, page_size, page_table.shape[1], _dt(dtype), stream))
+    return k, v
+
+
+def attention_decode_kv4(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, page_table: torch.Tensor,
+                         ctx_lens: torch.Tensor, n_heads: int, *, impl: int = 0, out: Optional[torch.Tensor] = None,
+                         scratch: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Decode attention of q [batch, n_heads*hs] over one layer of a 4-bit cache.  Sequence b attends to its first
+    ``ctx_lens[b]`` (int32 [batch] on the device) cached rows; zero rows give a zero output.  Query head h reads key head
+    h / (n_heads / n_kv_heads)."""
+    what = "attention_decode_kv4"
+    dev = _device_of(what, q=q, codes=codes, params=params, page_table=page_table, ctx_lens=ctx_lens, out=out,
+                     scratch=scratch)
+    n_pages, n_kv_heads, page_size, hs = _kv4_layer(what, codes, params)
+    if n_heads <= 0 or n_heads % n_kv_heads:
+        raise B200Error(2, f"{what}: {n_heads} query heads over {n_kv_heads} key heads")
+    ldq = _rows(what, "q", q, n_heads * hs)
+    batch = q.shape[0]
+    _index(what, "page_table", page_table, 2)
+    _index(what, "ctx_lens", ctx_lens)
+    if page_table.shape[0] != batch or ctx_lens.numel() != batch:
+        raise B200Error(2, f"{what}: page_table {tuple(page_table.shape)} and ctx_lens {tuple(ctx_lens.shape)} for a batch of {batch}")
+    if out is None:
+        out = torch.empty(batch, n_heads * hs, dtype=q.dtype, device=dev)
+    ldo = _rows(what, "out", out, n_heads * hs, batch, q.dtype)
+    with _On(dev) as stream:
+        if scratch is None:
+            n = c_size_t(0)
+            check(lib().b200_attention_decode_kv4_scratch_bytes(batch, n_heads, n_kv_heads, hs, byref(n)))
+            scratch = torch.empty(n.value, dtype=torch.uint8, device=dev)
+        check(lib().b200_attention_decode_kv4(q.data_ptr(), codes.data_ptr(), params.data_ptr(), page_table.data_ptr(),
+                                              ctx_lens.data_ptr(), out.data_ptr(), scratch.data_ptr(),
+                                              scratch.numel() * scratch.element_size(), batch, n_heads, n_kv_heads, hs,
+                                              ldq, ldo, n_pages, page_size, page_table.shape[1], _dt(q.dtype), impl,
+                                              stream))
+    return out
+
+
+def _check_copies(what: str, n_pages: int, src, dst) -> None:
+    if len(src) != len(dst):
+        raise B200Error(2, f"{what}: {len(src)} sources for {len(dst)} destinations")
+    for p in list(src) + list(dst):
+        if not 0 <= int(p) < n_pages:
+            raise B200Error(1, f"{what}: page {p} is not a page of this pool of {n_pages}")
+    if len(set(dst)) != len(dst):
+        raise B200Error(1, f"{what}: a destination page is named twice")
+    sources = {}
+    for s, d in zip(src, dst):
+        sources.setdefault(s, set()).add(d)
+    for d in dst:
+        if sources.get(d, set()) - {d}:
+            raise B200Error(1, f"{what}: destination page {d} is the source of another copy")
+
+
+def _page_list(what: str, name: str, x, dev) -> torch.Tensor:
+    if isinstance(x, torch.Tensor):
+        if not x.is_cuda:
+            raise B200Error(1, f"{what}: {name} must be a CUDA tensor or a list of page numbers")
+        _index(what, name, x)
+        return x
+    return torch.tensor([int(i) for i in x], dtype=torch.int32, device=dev)
+
+
+def _copy_pages(what, pool, src, dst, rows, page_table, page_map) -> None:
+    if pool.dim() < 4 or not pool.is_contiguous():
+        raise B200Error(2, f"{what}: the pool must be contiguous [..., n_pages, n_heads, page_size, row]")
+    n_pages, n_heads, page_size, row = pool.shape[-4:]
+    planes = 1
+    for d in pool.shape[:-4]:
+        planes *= d
+    if src.numel() != dst.numel() or (rows is not None and rows.numel() != src.numel()):
+        raise B200Error(2, f"{what}: src, dst and rows must have one entry per copy")
+    if page_map is not None and page_map.numel() != n_pages:
+        raise B200Error(2, f"{what}: page_map has {page_map.numel()} entries for {n_pages} pages")
+    dev = _device_of(what, pool=pool, src=src, dst=dst, rows=rows, page_table=page_table, page_map=page_map)
+    if pool.numel() == 0:
+        return
+    with _On(dev) as stream:
+        check(lib().b200_copy_pages(pool.data_ptr(), planes, n_pages, n_heads, page_size, row * pool.element_size(),
+                                    src.data_ptr(), dst.data_ptr(), _ptr(rows), src.numel(), _ptr(page_table),
+                                    0 if page_table is None else page_table.numel(), _ptr(page_map), stream))
+
+
+def copy_pages(pool: torch.Tensor, src, dst, rows=None) -> None:
+    """Copies page ``src[i]`` to page ``dst[i]`` in every plane of a pool [..., n_pages, n_heads, page_size, row] (the
+    pools of ``Plan.new_kv_pages`` and both pools of :func:`new_kv4_pages`), the first ``rows[i]`` rows of each head when
+    ``rows`` is given.  Lists of page numbers are checked on the host; int32 CUDA tensors are taken as they are, and
+    their destinations must be distinct and no copy's source."""
+    what = "copy_pages"
+    _device_of(what, pool=pool)
+    lists = [not isinstance(x, torch.Tensor) for x in (src, dst)]
+    if all(lists):
+        src, dst = [int(p) for p in src], [int(p) for p in dst]
+        _check_copies(what, pool.shape[-4] if pool.dim() >= 4 else 0, src, dst)
+    elif any(lists):
+        raise B200Error(1, f"{what}: give src and dst both as lists or both as CUDA tensors")
+    rows = None if rows is None else _page_list(what, "rows", rows, pool.device)
+    _copy_pages(what, pool, _page_list(what, "src", src, pool.device), _page_list(what, "dst", dst, pool.device), rows,
+                None, None)
+
+
+def compact_pages(pools, src, dst, page_table: torch.Tensor, page_map) -> None:
+    """Moves pages ``src[i]`` to ``dst[i]`` in one pool, or in every pool of a list that shares the page table (codes and
+    params of a 4-bit cache), and rewrites the int32 ``page_table`` in place: entry p becomes ``page_map[p]``.
+    ``PageAllocator.compact`` returns the three lists."""
+    what = "compact_pages"
+    pools = list(pools) if isinstance(pools, (list, tuple)) else [pools]
+    if not pools:
+        raise B200Error(1, f"{what}: no pool")
+    _device_of(what, page_table=page_table, **{f"pools[{i}]": p for i, p in enumerate(pools)})
+    if page_table.dtype != torch.int32 or not page_table.is_contiguous():
+        raise B200Error(3, f"{what}: page_table must be a contiguous int32 tensor")
+    dev = page_table.device
+    if len({p.shape[-4] if p.dim() >= 4 else 0 for p in pools}) != 1:
+        raise B200Error(2, f"{what}: the pools differ in their number of pages")
+    if not isinstance(src, torch.Tensor) and not isinstance(dst, torch.Tensor):
+        src, dst = [int(p) for p in src], [int(p) for p in dst]
+        _check_copies(what, pools[0].shape[-4] if pools[0].dim() >= 4 else 0, src, dst)
+    src, dst = _page_list(what, "src", src, dev), _page_list(what, "dst", dst, dev)
+    page_map = _page_list(what, "page_map", page_map, dev)
+    for i, pool in enumerate(pools):  # the table follows in the last pool's launch
+        last = i == len(pools) - 1
+        _copy_pages(what, pool, src, dst, None, page_table if last else None, page_map if last else None)
+
+
+# --------------------------------------------------------------------------
 # communicator
 # --------------------------------------------------------------------------
 
@@ -298,26 +636,88 @@ def argmax(logits: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Te
 
 class PageAllocator:
     """Free list over the pages of one KV pool (host side).  Sequences take whole pages; a page table row lists a
-    sequence's pages in position order, as ``b200_decode_step`` reads it."""
+    sequence's pages in position order, as ``b200_decode_step`` reads it.  A page may be shared by several sequences
+    (:meth:`share`, :meth:`fork`); it is free again when the last of them gave it back."""
 
     def __init__(self, n_pages: int):
         self.n_pages = int(n_pages)
         self._free = list(range(self.n_pages - 1, -1, -1))
+        self._refs: Dict[int, int] = {}
 
     @property
     def free_pages(self) -> int:
         return len(self._free)
 
+    def refs(self, page: int) -> int:
+        """Number of holders of a page (0: free)."""
+        return self._refs.get(page, 0)
+
     def alloc(self, n: int):
         if n > len(self._free):
             raise B200Error(5, f"KV pool exhausted: {n} pages wanted, {len(self._free)} free")
-        return [self._free.pop() for _ in range(n)]
+        pages = [self._free.pop() for _ in range(n)]
+        for p in pages:
+            self._refs[p] = 1
+        return pages
+
+    def _held(self, pages) -> None:
+        counts: Dict[int, int] = {}
+        for p in pages:
+            counts[p] = counts.get(p, 0) + 1
+        for p, n in counts.items():
+            if self._refs.get(p, 0) < n:
+                raise B200Error(1, f"page {p} is not an allocated page of this pool")
 
     def free(self, pages) -> None:
+        """Gives pages back, once per entry; all of them or, when one is not held, none."""
+        pages = list(pages)
+        self._held(pages)
+        gone = []
         for p in pages:
-            if not 0 <= p < self.n_pages or p in self._free:
+            self._refs[p] -= 1
+            if self._refs[p] == 0:
+                del self._refs[p]
+                gone.append(p)
+        self._free.extend(reversed(gone))
+
+    def share(self, pages) -> None:
+        """Adds one holder to each of the pages."""
+        pages = list(pages)
+        for p in pages:
+            if p not in self._refs:
                 raise B200Error(1, f"page {p} is not an allocated page of this pool")
-        self._free.extend(reversed(list(pages)))
+        for p in pages:
+            self._refs[p] += 1
+
+    def fork(self, pages, length: int, page_size: int):
+        """Pages of a second sequence that begins with the first ``length`` rows of the sequence on ``pages``: full pages
+        are shared, a partly filled last one gets a page of its own.  Returns ``(new_pages, copies)``; ``copies`` is a
+        list of at most one ``(src, dst, rows)`` for :func:`copy_pages`."""
+        pages = list(pages)
+        if length < 0 or page_size <= 0 or length > len(pages) * page_size:
+            raise B200Error(2, f"{length} rows do not fit {len(pages)} pages of {page_size}")
+        full, rest = divmod(length, page_size)
+        for p in pages[:full + (1 if rest else 0)]:
+            if p not in self._refs:
+                raise B200Error(1, f"page {p} is not an allocated page of this pool")
+        own = self.alloc(1) if rest else []
+        self.share(pages[:full])
+        return pages[:full] + own, [(pages[full], own[0], rest)] if rest else []
+
+    def compact(self):
+        """Moves the pages in use to the lowest numbers.  Returns ``(src, dst, page_map)`` for :func:`compact_pages`:
+        page src[i] moves to dst[i], and page_map[p] is where page p is found afterwards (itself unless it moves).  Page
+        numbers the caller keeps elsewhere have to be sent through ``page_map`` too."""
+        live = len(self._refs)
+        src = sorted(p for p in self._refs if p >= live)
+        dst = sorted(p for p in range(live) if p not in self._refs)
+        page_map = list(range(self.n_pages))
+        for s, d in zip(src, dst):
+            page_map[s] = d
+            self._refs[d] = self._refs.pop(s)
+        if src:
+            self._free = list(range(self.n_pages - 1, live - 1, -1))
+        return src, dst, page_map
 
 
 def _new_unique_id() -> bytes:

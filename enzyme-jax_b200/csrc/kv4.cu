@@ -1,0 +1,510 @@
+// The 4-bit key/value cache: append (quantise into pages), read back, and decode attention.
+//
+// Append.  A row x of one head becomes
+//   minimum = bf16 rounded down of min x,   scale = bf16 rounded up of (max x - minimum) / 15,
+//   code    = round-half-even((x - minimum) / scale) in 0..15.
+// With those directions of rounding every x lies between the values of code 0 and code 15, so the error is at most half
+// a scale.  A row that holds an infinity or NaN (or whose spread overflows) gets NaN parameters and reads back as NaN:
+// one bad value must not come back as a plausible one.  hs/8 lanes share a row: 8 elements and one 32-bit word of codes
+// each; the row's minimum and maximum are 4 shuffles.  HBM-bound (bytes of the inputs plus hs/2 + 4 per row and half).
+#include "kv4.cuh"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace b200 {
+
+namespace {
+
+__host__ __device__ constexpr int lanes_of(int hs) { return hs <= 16 ? 2 : hs <= 32 ? 4 : hs <= 64 ? 8 : 16; }
+
+__device__ __forceinline__ float bf16_down(float x) {
+  const uint32_t b = __float_as_uint(x), cut = b & 0xffff0000u;
+  return __uint_as_float((b >> 31) && cut != b ? cut + 0x10000u : cut);
+}
+__device__ __forceinline__ float bf16_up_nonneg(float x) {
+  const uint32_t b = __float_as_uint(x), cut = b & 0xffff0000u;
+  return __uint_as_float(cut != b ? cut + 0x10000u : cut);
+}
+
+struct Kv4RowsArgs {
+  Kv4Pool pool;
+  const int32_t* cu = nullptr;      // [n_seqs + 1]
+  const int32_t* before = nullptr;  // [n_seqs] rows each sequence held already, or null
+  int n_seqs = 0, rows = 0;
+  uint32_t* status = nullptr;
+};
+
+// Cache row (inside the key half) of packed row t for head hk; false when the row belongs to no sequence or the page
+// table has no valid page for it.
+__device__ __forceinline__ bool place_of(const Kv4RowsArgs& a, int t, int hk, size_t* row) {
+  // the sequence of row t: largest s with cu[s] <= t
+  int lo = -1, hi = a.n_seqs;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (__ldg(a.cu + mid) <= t) lo = mid;
+    else hi = mid - 1;
+  }
+  if (lo < 0 || lo >= a.n_seqs) return false;
+  const long long pos = (long long)(t - __ldg(a.cu + lo)) + (a.before ? __ldg(a.before + lo) : 0);
+  const long long slot = pos / a.pool.page_size;
+  if (pos < 0 || slot >= a.pool.max_pages) {
+    atomicOr(a.status, ST_BAD_PAGE);
+    return false;
+  }
+  const int page = __ldg(a.pool.table + (size_t)lo * a.pool.max_pages + slot);
+  if ((unsigned)page >= (unsigned)a.pool.n_pages) {
+    atomicOr(a.status, ST_BAD_PAGE);
+    return false;
+  }
+  *row = ((size_t)page * a.pool.n_kv_heads + hk) * a.pool.page_size + (size_t)(pos - slot * a.pool.page_size);
+  return true;
+}
+
+constexpr int AT = 256;  // threads of the append and read kernels
+
+// Threads: LPR lanes per (row, head, half); consecutive groups take consecutive heads of one row.
+template <typename T, int HS>
+__global__ void __launch_bounds__(AT) kv4_append_kernel(Kv4RowsArgs a, const T* __restrict__ k, const T* __restrict__ v,
+                                                        int ldk, int ldv, bool vec) {
+  constexpr int LPR = lanes_of(HS), GPB = AT / LPR;
+  const int li = threadIdx.x % LPR;
+  const long long item = (long long)blockIdx.x * GPB + threadIdx.x / LPR;
+  const int nk = a.pool.n_kv_heads;
+  const long long items = (long long)a.rows * nk * 2;
+  const bool real = item < items;
+  const int t = real ? (int)(item / (2 * nk)) : 0, rest = real ? (int)(item % (2 * nk)) : 0;
+  const int half = rest / nk, hk = rest % nk;
+  size_t row = 0;
+  const bool ok = real && place_of(a, t, hk, &row);
+  const bool active = ok && li * 8 < HS;
+  const T* src = (half ? v + (size_t)t * ldv : k + (size_t)t * ldk) + hk * HS + li * 8;
+  float x[8];
+  if (active) {
+    if (vec) {
+      load8(src, x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = to_f32(src[i]);
+    }
+  }
+  float lo = INFINITY, hi = -INFINITY;
+  bool bad = false;
+  if (active) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      lo = fminf(lo, x[i]);
+      hi = fmaxf(hi, x[i]);
+      bad |= !(fabsf(x[i]) < INFINITY);
+    }
+  }
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
+  }
+  if (!ok) return;
+  const float mn = bf16_down(lo);
+  const float spread = hi - mn;
+  bad |= !(spread < INFINITY) || !(mn > -INFINITY);
+  const float scale = bf16_up_nonneg(__fdiv_rn(spread, 15.f));
+  if (half) row += kv4_half(a.pool);
+  if (active) {
+    uint32_t w = 0u;
+    if (!bad && scale > 0.f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float c = fminf(rintf(__fdiv_rn(x[i] - mn, scale)), 15.f);
+        w |= (uint32_t)c << (4 * i);
+      }
+    }
+    reinterpret_cast<uint32_t*>(a.pool.codes)[row * (HS / 8) + li] = w;
+  }
+  if (li == 0) a.pool.params[row] = bad ? 0x7fc07fc0u : (__float_as_uint(scale) >> 16) | (__float_as_uint(mn) & 0xffff0000u);
+}
+
+// Reads packed rows back: minimum + scale * code (the product is exact in fp32), rounded to T.
+template <typename T, int HS>
+__global__ void __launch_bounds__(AT) kv4_read_kernel(Kv4RowsArgs a, T* __restrict__ k, T* __restrict__ v, int ldk, int ldv, bool vec) {
+  constexpr int LPR = lanes_of(HS), GPB = AT / LPR;
+  const int li = threadIdx.x % LPR;
+  const long long item = (long long)blockIdx.x * GPB + threadIdx.x / LPR;
+  const int nk = a.pool.n_kv_heads;
+  if (item >= (long long)a.rows * nk * 2 || li * 8 >= HS) return;
+  const int t = (int)(item / (2 * nk)), rest = (int)(item % (2 * nk));
+  const int half = rest / nk, hk = rest % nk;
+  size_t row = 0;
+  if (!place_of(a, t, hk, &row)) return;
+  if (half) row += kv4_half(a.pool);
+  const uint32_t w = reinterpret_cast<const uint32_t*>(a.pool.codes)[row * (HS / 8) + li];
+  const uint32_t prm = a.pool.params[row];
+  const float scale = __uint_as_float(prm << 16), mn = __uint_as_float(prm & 0xffff0000u);
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((w >> (4 * i)) & 15u), scale, mn);
+  T* dst = (half ? v + (size_t)t * ldv : k + (size_t)t * ldk) + hk * HS + li * 8;
+  if (vec) {
+    store8(dst, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dst[i] = from_f32<T>(x[i]);
+  }
+}
+
+// ---- decode attention on the CUDA cores ----------------------------------------------------------------------------
+// One query head per segment; LPK lanes hold one key (8 dims each), so a warp-wide load brings in 32/LPK rows.  q.k is
+// taken over the codes, scale and minimum enter once per row: s = scale * (q.code) + minimum * sum(q).  fp32 throughout.
+constexpr int SW = 4, SG = 4;  // warps per CTA, keys in flight per lane
+
+template <typename T, int HS>
+__global__ void __launch_bounds__(SW * 32) kv4_decode_simt_kernel(Kv4DecodeArgs a) {
+  constexpr int LPK = lanes_of(HS), KPW = 32 / LPK;
+  extern __shared__ int32_t pre[];
+  __shared__ int32_t warp_sums[SW];
+  __shared__ float s_acc[SW][HS], s_m[SW], s_l[SW];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LPK, li = lane % LPK;
+  const bool lane_on = li * 8 < HS;
+  unit_prefix<SW * 32>(a, pre, warp_sums);
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i <= a.batch; i += blockDim.x) a.prefix[i] = pre[i];
+  const Kv4Pool& p = a.pool;
+  const int nseg = p.n_kv_heads * a.subs;
+  const long long units = (long long)pre[a.batch] * nseg;
+  const int ctas = (int)(units < (long long)gridDim.x ? units : (long long)gridDim.x);
+  if ((int)blockIdx.x >= ctas) return;
+  const long long r0 = range_start(units, ctas, blockIdx.x), r1 = range_start(units, ctas, blockIdx.x + 1);
+  const uint32_t* codes = reinterpret_cast<const uint32_t*>(p.codes);
+  const size_t half = kv4_half(p);
+  int b = 0;
+  for (long long x = r0; x < r1;) {
+    while ((long long)pre[b + 1] * nseg <= x) ++b;
+    const int nb = pre[b + 1] - pre[b];
+    const long long base = (long long)pre[b] * nseg;
+    const int seg = (int)((x - base) / nb);
+    const long long s0 = base + (long long)seg * nb, s1 = s0 + nb;
+    const long long x1 = r1 < s1 ? r1 : s1;
+    const int hk = seg / a.subs, head = hk * a.subs + seg % a.subs;
+    const int len = kv4_len(a, b);
+    const int c0 = (int)(x - s0) * kUnit, c1 = min(len, (int)(x1 - s0) * kUnit);
+    const int32_t* table = p.table + (size_t)b * p.max_pages;
+
+    float qf[8], acc[8], qsum = 0.f, m = -INFINITY, l = 0.f, cmin = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      qf[i] = lane_on ? to_f32(((const T*)a.q)[(size_t)b * a.ldq + head * HS + li * 8 + i]) * a.scale : 0.f;
+      qsum += qf[i];
+      acc[i] = 0.f;
+    }
+#pragma unroll
+    for (int o = LPK / 2; o > 0; o >>= 1) qsum += __shfl_xor_sync(0xffffffffu, qsum, o);
+    for (int u0 = c0 + warp * (SG * KPW); u0 < c1; u0 += SW * SG * KPW) {
+      uint32_t kw[SG], vw[SG], kp[SG], vp[SG];
+      bool live[SG];
+#pragma unroll
+      for (int g = 0; g < SG; ++g) {
+        const int u = u0 + g * KPW + sub;
+        live[g] = u < c1;
+        kw[g] = vw[g] = kp[g] = vp[g] = 0u;
+        if (live[g]) {
+          const int page = __ldg(table + u / p.page_size);
+          live[g] = (unsigned)page < (unsigned)p.n_pages;
+          if (live[g]) {
+            const size_t row = ((size_t)page * p.n_kv_heads + hk) * p.page_size + u % p.page_size;
+            kp[g] = p.params[row];
+            vp[g] = p.params[row + half];
+            if (lane_on) {
+              kw[g] = codes[row * (HS / 8) + li];
+              vw[g] = codes[(row + half) * (HS / 8) + li];
+            }
+          } else {
+            atomicOr(a.status, ST_BAD_PAGE);
+          }
+        }
+      }
+      float s[SG], bm = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < SG; ++g) {
+        float d = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d = fmaf(qf[i], (float)((kw[g] >> (4 * i)) & 15u), d);
+#pragma unroll
+        for (int o = LPK / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        d = fmaf(__uint_as_float(kp[g] << 16), d, __uint_as_float(kp[g] & 0xffff0000u) * qsum);
+        s[g] = live[g] ? d : -INFINITY;
+        bm = fmaxf(bm, s[g]);
+      }
+      const float nm = fmaxf(m, bm);
+      const float corr = m == nm ? 1.f : exp_by_build(m - nm);
+      l *= corr;
+      cmin *= corr;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] *= corr;
+#pragma unroll
+      for (int g = 0; g < SG; ++g) {
+        if (live[g]) {  // a row behind the end may hold anything
+          const float pr = exp_by_build(s[g] - nm);
+          l += pr;
+          const float w = pr * __uint_as_float(vp[g] << 16);
+          cmin = fmaf(pr, __uint_as_float(vp[g] & 0xffff0000u), cmin);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, (float)((vw[g] >> (4 * i)) & 15u), acc[i]);
+        }
+      }
+      m = nm;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] += cmin;
+    // key groups of the warp, then the warps of the CTA
+#pragma unroll
+    for (int o = LPK; o < 32; o <<= 1) {
+      const float mo = __shfl_xor_sync(0xffffffffu, m, o), lo = __shfl_xor_sync(0xffffffffu, l, o);
+      const float nm = fmaxf(m, mo);
+      const float f0 = m == nm ? 1.f : exp_by_build(m - nm), f1 = mo == nm ? 1.f : exp_by_build(mo - nm);
+      l = l * f0 + lo * f1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = acc[i] * f0 + __shfl_xor_sync(0xffffffffu, acc[i], o) * f1;
+      m = nm;
+    }
+    if (sub == 0 && lane_on) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s_acc[warp][li * 8 + i] = acc[i];
+    }
+    if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+    __syncthreads();
+    float gm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < SW; ++w) gm = fmaxf(gm, s_m[w]);
+    float f[SW], gl = 0.f;
+#pragma unroll
+    for (int w = 0; w < SW; ++w) {
+      f[w] = s_m[w] == gm ? 1.f : exp_by_build(s_m[w] - gm);
+      gl += s_l[w] * f[w];
+    }
+    const bool whole = x == s0 && x1 == s1;
+    float* part = a.partials + (size_t)(2 * blockIdx.x + (x == r0 ? 0 : 1)) * (HS + 2);
+    for (int e = threadIdx.x; e < HS; e += blockDim.x) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < SW; ++w) v = fmaf(s_acc[w][e], f[w], v);
+      if (whole) ((T*)a.o)[(size_t)b * a.ldo + head * HS + e] = from_f32<T>(gl == 0.f ? 0.f : v / gl);
+      else part[e] = v;
+    }
+    if (!whole && threadIdx.x == 0) { part[HS] = gm; part[HS + 1] = gl; }
+    __syncthreads();  // s_acc is reused by the next segment
+    x = x1;
+  }
+}
+
+// Joins the partial blocks of the segments that several CTAs shared, and writes zeros for sequences without cached rows.
+template <typename T, int HS>
+__global__ void __launch_bounds__(128) kv4_join_kernel(Kv4DecodeArgs a, int grid) {
+  const int nseg = a.pool.n_kv_heads * a.subs;
+  const int b = blockIdx.x / nseg, seg = blockIdx.x % nseg;
+  pdl_wait();
+  const int p0 = a.prefix[b], nb = a.prefix[b + 1] - p0;
+  const long long units = (long long)a.prefix[a.batch] * nseg;
+  const int group = a.n_heads / a.pool.n_kv_heads;
+  const int first = (seg % a.subs) * a.cols, n = min(a.cols, group - first);
+  const int head0 = (seg / a.subs) * group + first;
+  T* o = (T*)a.o + (size_t)b * a.ldo + head0 * HS;
+  if (nb == 0) {
+    for (int e = threadIdx.x; e < n * HS; e += blockDim.x) o[e] = from_f32<T>(0.f);
+    return;
+  }
+  const int ctas = (int)(units < (long long)grid ? units : (long long)grid);
+  const long long s0 = (long long)p0 * nseg + (long long)seg * nb, s1 = s0 + nb;
+  const int ca = range_owner(units, ctas, s0), cb = range_owner(units, ctas, s1 - 1);
+  if (ca == cb) return;  // finished by its CTA
+  const size_t slot = (size_t)a.cols * (HS + 2);
+  const int sa = range_start(units, ctas, ca) == s0 ? 0 : 1;
+  for (int e = threadIdx.x; e < n * HS; e += blockDim.x) {
+    const int c = e / HS, d = e % HS;
+    float m = -INFINITY, l = 0.f, acc = 0.f;
+    for (int i = ca; i <= cb; ++i) {
+      const float* part = a.partials + (2 * (size_t)i + (i == ca ? sa : 0)) * slot + (size_t)c * (HS + 2);
+      const float mo = part[HS], nm = fmaxf(m, mo);
+      const float f0 = m == nm ? 1.f : exp_by_build(m - nm), f1 = mo == nm ? 1.f : exp_by_build(mo - nm);
+      l = l * f0 + part[HS + 1] * f1;
+      acc = acc * f0 + part[d] * f1;
+      m = nm;
+    }
+    o[e] = from_f32<T>(l == 0.f ? 0.f : acc / l);
+  }
+}
+
+template <typename F> int32_t by_type(const char* what, int dtype, int hs, F&& f) {
+  auto go = [&](auto t) -> int32_t {
+    switch (hs) {
+      case 16: return f(t, std::integral_constant<int, 16>());
+      case 32: return f(t, std::integral_constant<int, 32>());
+      case 48: return f(t, std::integral_constant<int, 48>());
+      case 64: return f(t, std::integral_constant<int, 64>());
+      case 128: return f(t, std::integral_constant<int, 128>());
+    }
+    return fail(B200_ERR_BAD_SHAPE, "%s: head size %d is not one of 16/32/48/64/128", what, hs);
+  };
+  if (dtype == B200_F32) return go(float());
+  if (dtype == B200_BF16) return go(bf16());
+  return fail(B200_ERR_BAD_DTYPE, "%s: unsupported dtype %d", what, dtype);
+}
+
+int32_t check_pool(const char* what, const Kv4Pool& p) {
+  if (p.n_pages < 0 || p.n_kv_heads <= 0 || p.page_size <= 0 || p.max_pages < 0 || p.head_size <= 0)
+    return fail(B200_ERR_BAD_SHAPE, "%s: sizes must be positive", what);
+  switch (p.head_size) {
+    case 16: case 32: case 48: case 64: case 128: return B200_OK;
+  }
+  return fail(B200_ERR_BAD_SHAPE, "%s: head size %d is not one of 16/32/48/64/128", what, p.head_size);
+}
+int32_t check_pool_ptrs(const char* what, const Kv4Pool& p) {
+  if (!p.codes || !p.params || !p.table) return fail(B200_ERR_INVALID_ARG, "%s: null operand", what);
+  if (!aligned16(p.codes) || !aligned16(p.params)) return fail(B200_ERR_MISALIGNED, "%s: codes and params must be 16-byte aligned", what);
+  return B200_OK;
+}
+
+// Grid of the decode kernels: two resident CTAs of 4 warps per SM would not cover HBM latency, so up to kCtasPerSm are
+// launched; a range may hold less than a whole segment, so a single long sequence fills the GPU too.
+constexpr int kCtasPerSm = 8;
+
+int decode_grid() { return kCtasPerSm * sm_count(); }
+
+}  // namespace
+
+size_t kv4_partial_floats(int ctas, int cols, int head_size) { return (size_t)2 * ctas * cols * (head_size + 2); }
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" {
+
+int32_t b200_kv4_append(const void* k, const void* v, void* codes, void* params, const int32_t* page_table,
+                        const int32_t* cu_seqlens, const int32_t* ctx_before, int32_t n_seqs, int32_t rows,
+                        int32_t n_kv_heads, int32_t head_size, int32_t ldk, int32_t ldv, int32_t n_pages,
+                        int32_t page_size, int32_t max_pages, int32_t dtype, b200_stream_t stream) {
+  Kv4RowsArgs a;
+  a.pool.codes = (uint8_t*)codes; a.pool.params = (uint32_t*)params; a.pool.table = page_table;
+  a.pool.n_pages = n_pages; a.pool.n_kv_heads = n_kv_heads; a.pool.page_size = page_size;
+  a.pool.head_size = head_size; a.pool.max_pages = max_pages;
+  a.cu = cu_seqlens; a.before = ctx_before; a.n_seqs = n_seqs; a.rows = rows;
+  B200_TRY(check_pool("kv4 append", a.pool));
+  if (n_seqs < 0 || rows < 0) return fail(B200_ERR_BAD_SHAPE, "kv4 append: n_seqs=%d rows=%d", n_seqs, rows);
+  if (ldk < (long long)n_kv_heads * head_size || ldv < (long long)n_kv_heads * head_size)
+    return fail(B200_ERR_BAD_SHAPE, "kv4 append: a row pitch is smaller than the row");
+  if (dtype != B200_F32 && dtype != B200_BF16) return fail(B200_ERR_BAD_DTYPE, "kv4 append: unsupported dtype %d", dtype);
+  if (rows == 0 || n_seqs == 0) return B200_OK;
+  if (!k || !v || !cu_seqlens) return fail(B200_ERR_INVALID_ARG, "kv4 append: null operand");
+  B200_TRY(check_pool_ptrs("kv4 append", a.pool));
+  a.status = device_status_word();
+  if (!a.status) return fail(B200_ERR_CUDA, "no device status word");
+  const bool vec = aligned16(k) && aligned16(v) && ldk % 8 == 0 && ldv % 8 == 0;
+  return by_type("kv4 append", dtype, head_size, [&](auto t, auto hs) -> int32_t {
+    using T = decltype(t);
+    constexpr int HS = decltype(hs)::value;
+    const long long groups = (long long)rows * n_kv_heads * 2, per = AT / lanes_of(HS), blocks = (groups + per - 1) / per;
+    if (blocks > 0x7fffffffLL) return fail(B200_ERR_BAD_SHAPE, "kv4 append: too many rows");
+    kv4_append_kernel<T, HS><<<(unsigned)blocks, AT, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, (const T*)k, (const T*)v, ldk, ldv, vec);
+    B200_LAUNCH_OK("kv4_append_kernel");
+    return B200_OK;
+  });
+}
+
+int32_t b200_kv4_read(void* k, void* v, const void* codes, const void* params, const int32_t* page_table,
+                      const int32_t* cu_seqlens, const int32_t* ctx_before, int32_t n_seqs, int32_t rows,
+                      int32_t n_kv_heads, int32_t head_size, int32_t ldk, int32_t ldv, int32_t n_pages,
+                      int32_t page_size, int32_t max_pages, int32_t dtype, b200_stream_t stream) {
+  Kv4RowsArgs a;
+  a.pool.codes = (uint8_t*)const_cast<void*>(codes); a.pool.params = (uint32_t*)const_cast<void*>(params);
+  a.pool.table = page_table;
+  a.pool.n_pages = n_pages; a.pool.n_kv_heads = n_kv_heads; a.pool.page_size = page_size;
+  a.pool.head_size = head_size; a.pool.max_pages = max_pages;
+  a.cu = cu_seqlens; a.before = ctx_before; a.n_seqs = n_seqs; a.rows = rows;
+  B200_TRY(check_pool("kv4 read", a.pool));
+  if (n_seqs < 0 || rows < 0) return fail(B200_ERR_BAD_SHAPE, "kv4 read: n_seqs=%d rows=%d", n_seqs, rows);
+  if (ldk < (long long)n_kv_heads * head_size || ldv < (long long)n_kv_heads * head_size)
+    return fail(B200_ERR_BAD_SHAPE, "kv4 read: a row pitch is smaller than the row");
+  if (dtype != B200_F32 && dtype != B200_BF16) return fail(B200_ERR_BAD_DTYPE, "kv4 read: unsupported dtype %d", dtype);
+  if (rows == 0 || n_seqs == 0) return B200_OK;
+  if (!k || !v || !cu_seqlens) return fail(B200_ERR_INVALID_ARG, "kv4 read: null operand");
+  B200_TRY(check_pool_ptrs("kv4 read", a.pool));
+  a.status = device_status_word();
+  if (!a.status) return fail(B200_ERR_CUDA, "no device status word");
+  const bool vec = aligned16(k) && aligned16(v) && ldk % 8 == 0 && ldv % 8 == 0;
+  return by_type("kv4 read", dtype, head_size, [&](auto t, auto hs) -> int32_t {
+    using T = decltype(t);
+    constexpr int HS = decltype(hs)::value;
+    const long long groups = (long long)rows * n_kv_heads * 2, per = AT / lanes_of(HS), blocks = (groups + per - 1) / per;
+    if (blocks > 0x7fffffffLL) return fail(B200_ERR_BAD_SHAPE, "kv4 read: too many rows");
+    kv4_read_kernel<T, HS><<<(unsigned)blocks, AT, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, (T*)k, (T*)v, ldk, ldv, vec);
+    B200_LAUNCH_OK("kv4_read_kernel");
+    return B200_OK;
+  });
+}
+
+int32_t b200_attention_decode_kv4_scratch_bytes(int32_t batch, int32_t n_heads, int32_t n_kv_heads, int32_t head_size,
+                                                size_t* bytes) {
+  if (!bytes) return fail(B200_ERR_INVALID_ARG, "bytes is null");
+  if (batch < 0 || n_heads <= 0 || n_kv_heads <= 0 || head_size <= 0 || n_heads % n_kv_heads)
+    return fail(B200_ERR_BAD_SHAPE, "kv4 decode: batch=%d heads=%d kv_heads=%d head_size=%d", batch, n_heads, n_kv_heads, head_size);
+  const int cols = std::min(8, n_heads / n_kv_heads);
+  *bytes = align_up(((size_t)std::min(batch, kMaxSlice) + 1) * 4, 256) + kv4_partial_floats(decode_grid(), cols, head_size) * 4;
+  return B200_OK;
+}
+
+int32_t b200_attention_decode_kv4(const void* q, const void* codes, const void* params, const int32_t* page_table,
+                                  const int32_t* ctx_lens, void* o, void* scratch, size_t scratch_bytes, int32_t batch,
+                                  int32_t n_heads, int32_t n_kv_heads, int32_t head_size, int32_t ldq, int32_t ldo,
+                                  int32_t n_pages, int32_t page_size, int32_t max_pages, int32_t dtype, int32_t impl,
+                                  b200_stream_t stream) {
+  Kv4DecodeArgs a;
+  a.pool.codes = (uint8_t*)const_cast<void*>(codes); a.pool.params = (uint32_t*)const_cast<void*>(params);
+  a.pool.table = page_table;
+  a.pool.n_pages = n_pages; a.pool.n_kv_heads = n_kv_heads; a.pool.page_size = page_size;
+  a.pool.head_size = head_size; a.pool.max_pages = max_pages;
+  B200_TRY(check_pool("kv4 decode", a.pool));
+  if (batch < 0 || n_heads <= 0 || n_heads % n_kv_heads)
+    return fail(B200_ERR_BAD_SHAPE, "kv4 decode: batch=%d, %d query heads over %d key heads", batch, n_heads, n_kv_heads);
+  if (ldq < (long long)n_heads * head_size || ldo < (long long)n_heads * head_size)
+    return fail(B200_ERR_BAD_SHAPE, "kv4 decode: a row pitch is smaller than the row");
+  if (dtype != B200_F32 && dtype != B200_BF16) return fail(B200_ERR_BAD_DTYPE, "kv4 decode: unsupported dtype %d", dtype);
+  if (impl < 0 || impl > 2) return fail(B200_ERR_INVALID_ARG, "impl %d is not 0, 1 or 2", impl);
+  if (batch == 0) return B200_OK;
+  if (!q || !o || !ctx_lens || !scratch) return fail(B200_ERR_INVALID_ARG, "kv4 decode: null operand");
+  B200_TRY(check_pool_ptrs("kv4 decode", a.pool));
+  if (!aligned16(scratch)) return fail(B200_ERR_MISALIGNED, "kv4 decode: scratch must be 16-byte aligned");
+  size_t need = 0;
+  B200_TRY(b200_attention_decode_kv4_scratch_bytes(batch, n_heads, n_kv_heads, head_size, &need));
+  if (scratch_bytes < need) return fail(B200_ERR_WORKSPACE, "kv4 decode: scratch needs %zu bytes, %zu given", need, scratch_bytes);
+  a.status = device_status_word();
+  if (!a.status) return fail(B200_ERR_CUDA, "no device status word");
+  a.n_heads = n_heads; a.ldq = ldq; a.ldo = ldo; a.dtype = dtype;
+  a.scale = 1.f / sqrtf((float)head_size);
+  a.prefix = (int32_t*)scratch;
+  a.partials = (float*)((char*)scratch + align_up(((size_t)std::min(batch, kMaxSlice) + 1) * 4, 256));
+  if (impl == 1) return fail(B200_ERR_UNSUPPORTED, "no tensor-core kernel for this shape");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  a.subs = n_heads / n_kv_heads; a.cols = 1;
+  const size_t es = dtype == B200_BF16 ? 2 : 4;
+  const long long units_per_seq = ((long long)max_pages * page_size + kUnit - 1) / kUnit * n_heads;
+  for (int b0 = 0; b0 < batch; b0 += kMaxSlice) {
+    a.batch = std::min(kMaxSlice, batch - b0);
+    a.q = (const char*)q + (size_t)b0 * ldq * es;
+    a.o = (char*)o + (size_t)b0 * ldo * es;
+    a.ctx = ctx_lens + b0;
+    a.pool.table = page_table + (size_t)b0 * max_pages;
+    const int grid = (int)std::max(1LL, std::min<long long>(decode_grid(), units_per_seq * a.batch));
+    B200_TRY(by_type("kv4 decode", dtype, head_size, [&](auto t, auto hs) -> int32_t {
+      using T = decltype(t);
+      constexpr int HS = decltype(hs)::value;
+      kv4_decode_simt_kernel<T, HS><<<grid, SW * 32, (a.batch + 1) * sizeof(int32_t), s>>>(a);
+      B200_LAUNCH_OK("kv4_decode_simt_kernel");
+      B200_CUDA_OK(launch_pdl(kv4_join_kernel<T, HS>, dim3(a.batch * n_kv_heads * a.subs), dim3(128), 0, s, a, grid));
+      B200_LAUNCH_OK("kv4_join_kernel");
+      return B200_OK;
+    }));
+  }
+  return B200_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,88 @@
+// A key/value cache in 4 bits.  One layer is
+//   codes   uint8 [2, n_pages, n_kv_heads, page_size, hs/2]   element 2i in the low half of byte i; keys, then values
+//   params  bf16  [2, n_pages, n_kv_heads, page_size, 2]      (scale, minimum) of the row
+// and a row stands for minimum + scale * code.  The scale is one number per cached row of a head: it leaves the dot
+// product q.k and enters the weight p of a value row, so neither row is ever expanded in memory.
+#pragma once
+
+#include "common.cuh"
+
+namespace b200 {
+
+// What kernels of the cache OR into the device status word when a page table names a page outside the pool.
+enum : uint32_t { ST_BAD_PAGE = 1u << 16 };
+
+struct Kv4Pool {
+  uint8_t* codes = nullptr;
+  uint32_t* params = nullptr;  // low half: scale, high half: minimum
+  const int32_t* table = nullptr;  // [batch, max_pages]
+  int n_pages = 0, n_kv_heads = 0, page_size = 0, head_size = 0, max_pages = 0;
+};
+
+// Row index of (page, head, row) inside the key half; the value half begins kv4_half() rows later.
+__host__ __device__ __forceinline__ size_t kv4_half(const Kv4Pool& p) {
+  return (size_t)p.n_pages * p.n_kv_heads * p.page_size;
+}
+
+struct Kv4DecodeArgs {
+  Kv4Pool pool;
+  const void* q = nullptr;         // [batch, ldq]
+  void* o = nullptr;               // [batch, ldo]
+  const int32_t* ctx = nullptr;    // [batch] cached rows of each sequence
+  float* partials = nullptr;       // 2 * grid slots of [columns][head_size + 2]
+  int32_t* prefix = nullptr;       // [batch + 1]
+  uint32_t* status = nullptr;
+  int batch = 0, n_heads = 0, ldq = 0, ldo = 0, dtype = B200_BF16;
+  int subs = 1;                    // head subsets per key head: segments of a sequence are (key head, subset)
+  int cols = 1;                    // query heads per subset (the last one may hold fewer)
+  float scale = 1.f;
+};
+
+// ---- sharing the cached rows out ------------------------------------------------------------------------------------
+// The work of a step is the units of kUnit cached rows of every (sequence, key head, subset), in that order.  Each CTA
+// takes one contiguous range of the whole list, so lengths that differ by any factor balance by themselves.  A segment
+// that lies inside one CTA is finished there; the others leave partial (sum, maximum, accumulator) blocks that a second
+// kernel joins.  Partials are addressed by CTA: 2 slots each (the range's first segment, its last one).
+constexpr int kUnit = 128;
+constexpr int kMaxSlice = 4096;  // sequences per launch: their unit prefix is held in shared memory
+
+__device__ __forceinline__ int kv4_len(const Kv4DecodeArgs& a, int b) {
+  const long long cap = (long long)a.pool.max_pages * a.pool.page_size;
+  const int n = __ldg(a.ctx + b);
+  return n <= 0 ? 0 : (n < cap ? n : (int)cap);
+}
+__device__ __forceinline__ long long range_start(long long units, int ctas, int c) { return units * c / ctas; }
+__device__ __forceinline__ int range_owner(long long units, int ctas, long long u) { return (int)(((u + 1) * ctas - 1) / units); }
+
+// Exclusive prefix of the sequences' unit counts into `pre` [batch + 1] (shared memory), by all threads of the block.
+template <int THREADS> __device__ __forceinline__ void unit_prefix(const Kv4DecodeArgs& a, int32_t* pre, int32_t* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int base = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += THREADS) {
+    const int b = b0 + threadIdx.x;
+    const int mine = b < a.batch ? (kv4_len(a, b) + kUnit - 1) / kUnit : 0;
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 31) warp_sums[warp] = inc;
+    __syncthreads();
+    int before = base, total = base;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) before += warp_sums[w];
+      total += warp_sums[w];
+    }
+    if (b < a.batch) pre[b] = before + inc - mine;
+    base = total;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) pre[a.batch] = base;
+  __syncthreads();
+}
+
+size_t kv4_partial_floats(int ctas, int cols, int head_size);
+
+}  // namespace b200

@@ -12,6 +12,7 @@
 #include "attention.cuh"
 #include "elementwise.cuh"
 #include "gemm_epilogue.cuh"
+#include "kv4.cuh"
 #include "plan.cuh"
 
 namespace b200 {
@@ -621,6 +622,7 @@ int32_t b200_device_status(b200_stream_t stream, uint32_t* code) {
     B200_CUDA_OK(cudaStreamSynchronize(s));
   }
   if (code) *code = host;
+  if (host == ST_BAD_PAGE) return fail(B200_ERR_INVALID_ARG, "a page outside the pool or the page table was skipped (status word 0x%x)", host);
   if (host) return fail(B200_ERR_TIMEOUT, "a bounded device-side wait ran out (status word 0x%x)", host);
   return B200_OK;
 }

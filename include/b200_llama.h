@@ -100,7 +100,8 @@ B200_API const char* b200_version(void);
 /* Reads and clears the device-side status word that kernels with bounded
  * waits set when a wait runs out.  Synchronises the stream (the one place that
  * does, like xla_throw_error in xla_ffi/cuda/throw_error.cc:20-31).  Returns
- * B200_OK or B200_ERR_TIMEOUT; *code receives the raw word. */
+ * B200_OK or B200_ERR_TIMEOUT, or B200_ERR_INVALID_ARG when nothing timed out but a
+ * kernel skipped a page outside its pool; *code receives the raw word. */
 B200_API int32_t b200_device_status(b200_stream_t stream, uint32_t* code);
 
 /* Greedy sampling on the device: out_tokens[r] = argmax of the r-th row of fp32 logits [rows, ld] (first `cols`
@@ -370,6 +371,81 @@ B200_API int32_t b200_attention_decode_static(const void* q, const void* kv_page
                                               int32_t head_size, int32_t ldq, int32_t ldo, int32_t n_pages,
                                               int32_t page_size, int32_t max_pages, int32_t dtype,
                                               b200_stream_t stream);
+
+/* ---- packed prompts, the 4-bit cache, page copies -------------------------- */
+
+/* Causal attention over packed sequences of different lengths with grouped heads (test/llama.py:177-209 applied to every
+ * position of every sequence).  Sequence s owns rows cu_seqlens[s] .. cu_seqlens[s+1]-1 of q, k, v and o; query head h
+ * reads key head h / (n_heads / n_kv_heads).
+ *   q, o        [rows, ldq / ldo], n_heads heads side by side; k, v [rows, ldk / ldv], n_kv_heads heads
+ *   lse         fp32 [n_heads, rows] or NULL
+ *   cu_seqlens  int32 [n_seqs + 1] on the device, ascending; sequences may be empty
+ * Rows before the first and behind the last sequence are neither read into any result nor written.  What stands in rows
+ * a query may not see (later positions, other sequences) does not reach it, infinities and NaN included.
+ * head_size 16, 32, 48, 64 or 128.  impl: 0 = pick, 1 = tensor cores (bf16, head size 64 or 128, 16-byte aligned rows),
+ * 2 = CUDA cores. */
+B200_API int32_t b200_attention_packed(const void* q, const void* k, const void* v, void* o, float* lse,
+                                       const int32_t* cu_seqlens, int32_t n_seqs, int32_t rows, int32_t n_heads,
+                                       int32_t n_kv_heads, int32_t head_size, int32_t ldq, int32_t ldk, int32_t ldv,
+                                       int32_t ldo, int32_t dtype, int32_t impl, b200_stream_t stream);
+
+/* Reverse mode of b200_attention_packed: from its inputs, output, lse and the cotangent d_o to dq (like q), dk and dv
+ * (like k and v; summed over the query heads of a group in a fixed order, no atomics).  delta_scratch: n_heads * rows
+ * floats.  Rows of no sequence are not written; one sequence's infinities and NaN do not reach another one. */
+B200_API int32_t b200_attention_packed_backward(const void* q, const void* k, const void* v, const void* o,
+                                                const float* lse, const void* d_o, void* dq, void* dk, void* dv,
+                                                float* delta_scratch, const int32_t* cu_seqlens, int32_t n_seqs,
+                                                int32_t rows, int32_t n_heads, int32_t n_kv_heads, int32_t head_size,
+                                                int32_t ldq, int32_t ldk, int32_t ldv, int32_t ldo, int32_t lddo,
+                                                int32_t lddq, int32_t lddk, int32_t lddv, int32_t dtype, int32_t impl,
+                                                b200_stream_t stream);
+
+/* One layer of a key/value cache held in 4 bits:
+ *   codes   uint8 [2, n_pages, n_kv_heads, page_size, head_size/2]  keys, then values; element 2i in the low half of byte i
+ *   params  bf16  [2, n_pages, n_kv_heads, page_size, 2]            scale and minimum of the row
+ * A row stands for minimum + scale * code, with minimum = bf16 rounded down of the smallest element, scale = bf16 rounded
+ * up of (largest - minimum) / 15 and code = round-half-even((x - minimum) / scale) in 0..15.  A row that holds an infinity
+ * or NaN, or whose spread overflows fp32, reads back as NaN.
+ *
+ * b200_kv4_append quantises packed rows k, v [rows, ldk / ldv] into the pages: row t of sequence s (cu_seqlens as above)
+ * becomes its row ctx_before[s] + t - cu_seqlens[s] (ctx_before NULL: 0).  A decode step is n_seqs = rows with
+ * cu_seqlens = 0, 1, 2, ...  b200_kv4_read is the way back, to k, v of `dtype`.  page_table int32 [n_seqs, max_pages].
+ * Positions behind the page table and page ids outside the pool are skipped; b200_device_status then answers
+ * B200_ERR_INVALID_ARG. */
+B200_API int32_t b200_kv4_append(const void* k, const void* v, void* codes, void* params, const int32_t* page_table,
+                                 const int32_t* cu_seqlens, const int32_t* ctx_before, int32_t n_seqs, int32_t rows,
+                                 int32_t n_kv_heads, int32_t head_size, int32_t ldk, int32_t ldv, int32_t n_pages,
+                                 int32_t page_size, int32_t max_pages, int32_t dtype, b200_stream_t stream);
+B200_API int32_t b200_kv4_read(void* k, void* v, const void* codes, const void* params, const int32_t* page_table,
+                               const int32_t* cu_seqlens, const int32_t* ctx_before, int32_t n_seqs, int32_t rows,
+                               int32_t n_kv_heads, int32_t head_size, int32_t ldk, int32_t ldv, int32_t n_pages,
+                               int32_t page_size, int32_t max_pages, int32_t dtype, b200_stream_t stream);
+
+/* Decode attention over the 4-bit cache: one query row per sequence against its first ctx_lens[b] cached rows (int32
+ * [batch] on the device, cut to max_pages * page_size; a sequence without rows gets zeros), grouped heads as above.
+ * q, o [batch, ldq / ldo] of `dtype`.  scratch: b200_attention_decode_kv4_scratch_bytes() bytes, 16-byte aligned, used by
+ * this call alone while it runs.  Pages outside the pool are skipped and reported as above.  impl: 0 = pick, 1 = tensor
+ * cores (bf16, head size 64 or 128, page_size a multiple of 16), 2 = CUDA cores. */
+B200_API int32_t b200_attention_decode_kv4_scratch_bytes(int32_t batch, int32_t n_heads, int32_t n_kv_heads,
+                                                         int32_t head_size, size_t* bytes);
+B200_API int32_t b200_attention_decode_kv4(const void* q, const void* codes, const void* params,
+                                           const int32_t* page_table, const int32_t* ctx_lens, void* o, void* scratch,
+                                           size_t scratch_bytes, int32_t batch, int32_t n_heads, int32_t n_kv_heads,
+                                           int32_t head_size, int32_t ldq, int32_t ldo, int32_t n_pages,
+                                           int32_t page_size, int32_t max_pages, int32_t dtype, int32_t impl,
+                                           b200_stream_t stream);
+
+/* Copies n pages inside a pool [n_planes, n_pages, n_heads, page_size, row_bytes] (planes: layers x {key, value}; the
+ * bf16, fp32 and 4-bit pools and the 4-bit pool's params all have this form): page src[i] to page dst[i] in every plane;
+ * with `rows` only the first rows[i] rows of every head (the rest of the destination stays).  With a page table
+ * (table_entries int32, any shape) every entry p in 0..n_pages-1 becomes page_map[p] in the same launch (page_map int32
+ * [n_pages] is required then).  src, dst, rows, page_table and page_map are on the device.  The destinations must be
+ * distinct and none of them a source of another copy.  Page ids outside the pool are skipped; b200_device_status then
+ * answers B200_ERR_INVALID_ARG. */
+B200_API int32_t b200_copy_pages(void* pool, int32_t n_planes, int32_t n_pages, int32_t n_heads, int32_t page_size,
+                                 int32_t row_bytes, const int32_t* src, const int32_t* dst, const int32_t* rows,
+                                 int32_t n, int32_t* page_table, int64_t table_entries, const int32_t* page_map,
+                                 b200_stream_t stream);
 
 /* ---- communicator (NCCL over NVLink) -------------------------------------- */
 

@@ -1,0 +1,123 @@
+"""Packed attention, the 4-bit cache and page copies without a GPU: refusals that come before any launch, the page
+allocator's sharing, forking and compacting, and the 64-bit reference against differences."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import b200_llama as B
+import packed_reference as R
+
+P = ctypes.c_void_p(16)   # a non-null, aligned address that no refused call touches
+
+
+def test_packed_attention_refusals():
+    f = B.lib().b200_attention_packed
+    call = lambda q=P, k=P, v=P, o=P, cu=P, n=1, rows=8, h=4, hk=2, hs=64, ldq=256, ldk=128, ldv=128, ldo=256, dt=1, impl=0: f(
+        q, k, v, o, None, cu, n, rows, h, hk, hs, ldq, ldk, ldv, ldo, dt, impl, None)
+    assert call(q=None) == 1 and call(cu=None) == 1 and call(impl=5) == 1
+    assert call(h=3) == 2 and call(hk=0) == 2 and call(hs=40) == 2 and call(rows=-1) == 2 and call(ldk=100) == 2
+    assert call(dt=7) == 3
+    assert call(rows=0, q=None) == 0 and call(n=0, q=None) == 0       # nothing to do
+    g = B.lib().b200_attention_packed_backward
+    assert g(P, P, P, P, P, P, P, P, P, None, P, 1, 8, 4, 2, 64, 256, 128, 128, 256, 256, 256, 128, 128, 1, 0, None) == 1
+    assert g(P, P, P, P, P, P, P, P, P, P, P, 1, 8, 4, 2, 64, 256, 128, 128, 256, 256, 256, 64, 128, 1, 0, None) == 2
+
+
+def test_kv4_refusals():
+    lib = B.lib()
+    app = lambda k=P, codes=P, table=P, n=1, rows=4, hk=2, hs=64, ldk=128, pages=4, page=16, width=2, dt=1: lib.b200_kv4_append(
+        k, P, codes, P, table, P, None, n, rows, hk, hs, ldk, 128, pages, page, width, dt, None)
+    assert app(k=None) == 1 and app(table=None) == 1 and app(hs=20) == 2 and app(page=0) == 2 and app(ldk=64) == 2
+    assert app(dt=5) == 3 and app(codes=ctypes.c_void_p(20)) == 4 and app(rows=0, k=None) == 0
+    dec = lambda q=P, scratch=P, nbytes=1 << 30, b=1, h=4, hk=2, hs=64, ldq=256, impl=0: lib.b200_attention_decode_kv4(
+        q, P, P, P, P, P, scratch, nbytes, b, h, hk, hs, ldq, 256, 4, 16, 2, 1, impl, None)
+    assert dec(q=None) == 1 and dec(h=3) == 2 and dec(ldq=8) == 2 and dec(b=-1) == 2 and dec(impl=9) == 1
+    assert dec(b=0, q=None) == 0 and dec(scratch=ctypes.c_void_p(8)) == 4
+    n = ctypes.c_size_t(0)
+    assert lib.b200_attention_decode_kv4_scratch_bytes(4, 4, 3, 64, ctypes.byref(n)) == 2
+    assert lib.b200_attention_decode_kv4_scratch_bytes(4, 4, 2, 64, None) == 1
+
+
+def test_copy_pages_refusals():
+    f = B.lib().b200_copy_pages
+    call = lambda pool=P, planes=2, pages=4, heads=2, page=16, row=128, src=P, n=1, table=None, entries=0, pmap=None: f(
+        pool, planes, pages, heads, page, row, src, P, None, n, table, entries, pmap, None)
+    assert call(pool=None) == 1 and call(src=None) == 1 and call(table=P, entries=4) == 1
+    assert call(planes=0) == 2 and call(n=-1) == 2 and call(row=0) == 2 and call(page=1 << 30) == 2
+    assert call(n=0, pool=None) == 0
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(4, 128).bfloat16()
+    cu = torch.zeros(2, dtype=torch.int32)
+    for call in (lambda: B.attention_packed(x, x, x, cu, 2), lambda: B.copy_pages(torch.zeros(2, 4, 2, 16, 64), [0], [1])):
+        with pytest.raises(B.B200Error) as e:
+            call()
+        assert e.value.status == 1
+
+
+def test_allocator_shares_and_forks():
+    a = B.PageAllocator(8)
+    x = a.alloc(3)
+    child, copies = a.fork(x, 40, 16)               # two full pages, 8 rows of the third
+    assert child[:2] == x[:2] and child[2] not in x and copies == [(x[2], child[2], 8)]
+    assert [a.refs(p) for p in x] == [2, 2, 1] and a.free_pages == 4
+    whole, none = a.fork(x, 32, 16)                 # ends with a page: nothing to copy
+    assert whole == x[:2] and none == [] and a.refs(x[0]) == 3
+    assert a.fork(x, 0, 16) == ([], [])
+    a.free(x)
+    assert a.free_pages == 5 and a.refs(x[2]) == 0 and a.refs(x[0]) == 2
+    a.free(child)
+    a.free(whole)
+    assert a.free_pages == 8
+    with pytest.raises(B.B200Error):
+        a.free([x[0]])                              # not held any more
+    y = a.alloc(2)
+    with pytest.raises(B.B200Error):
+        a.free([y[0], y[0]])                        # once per holder: nothing is given back
+    assert a.refs(y[0]) == 1
+    with pytest.raises(B.B200Error):
+        a.fork(y, 33, 16)
+    full = a.alloc(6)
+    with pytest.raises(B.B200Error) as e:
+        a.fork(y, 5, 16)                            # no page for the partly filled one: nothing is shared
+    assert e.value.status == 5 and a.refs(y[0]) == 1
+    with pytest.raises(B.B200Error):
+        a.share([full[0], 99])
+    assert a.refs(full[0]) == 1
+
+
+def test_allocator_compacts():
+    a = B.PageAllocator(10)
+    x, y, z = a.alloc(3), a.alloc(3), a.alloc(2)
+    a.share([z[1]])
+    a.free(x)
+    src, dst, page_map = a.compact()
+    live = sorted(page_map[p] for p in y + z)
+    assert live == [0, 1, 2, 3, 4] and len(set(dst)) == len(dst) and not set(src) & set(dst)
+    assert all(page_map[s] == d for s, d in zip(src, dst)) and a.refs(page_map[z[1]]) == 2
+    assert a.free_pages == 5 and a.alloc(1) == [5]
+    assert a.compact()[0] == []                     # already compact
+    a.free([page_map[p] for p in y + z])
+    assert a.refs(page_map[z[1]]) == 1
+
+
+def test_reference_gradient_against_differences():
+    g = torch.Generator().manual_seed(0)
+    lens, heads, kv, hs = [5, 1, 7], 4, 2, 8
+    q, k, v, d_o = (torch.randn(13, n * hs, generator=g, dtype=torch.float64) for n in (heads, kv, kv, heads))
+    R.U[torch.float64] = 0.0
+    try:
+        grads, _ = R.backward(q, k, v, d_o, lens, heads, kv)
+        value = lambda a, b, c: float((R.forward(a, b, c, lens, heads, kv)[0] * d_o).sum())
+        h = 1e-6
+        for i, grad in enumerate(grads):
+            d = torch.randn(grad.shape, generator=g, dtype=torch.float64)
+            up, down = [q, k, v], [q, k, v]
+            up[i], down[i] = up[i] + h * d, down[i] - h * d
+            diff = (value(*up) - value(*down)) / (2 * h)
+            assert math.isclose(diff, float((grad * d).sum()), rel_tol=1e-7, abs_tol=1e-7)
+    finally:
+        del R.U[torch.float64]
