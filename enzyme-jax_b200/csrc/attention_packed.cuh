@@ -33,6 +33,8 @@ struct PackedBwdArgs {
   float* delta = nullptr;  // scratch [n_heads, rows]: rowsum(dO * O)
 };
 
+bool packed_fwd_tc_supports(const PackedArgs& a);
+int32_t launch_packed_fwd_tc(const PackedArgs& a, cudaStream_t stream);
 int32_t launch_packed_fwd_simt(const PackedArgs& a, cudaStream_t stream);
 int32_t launch_packed_bwd_simt(const PackedBwdArgs& a, cudaStream_t stream);
 

@@ -372,7 +372,7 @@ int32_t b200_attention_packed(const void* q, const void* k, const void* v, void*
   if (rows == 0 || n_seqs == 0) return B200_OK;
   if (!q || !k || !v || !o || !cu_seqlens) return fail(B200_ERR_INVALID_ARG, "null operand");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (impl == 1) return fail(B200_ERR_UNSUPPORTED, "no tensor-core kernel for this shape");
+  if (impl == 1 || (impl == 0 && packed_fwd_tc_supports(a))) return launch_packed_fwd_tc(a, s);
   return launch_packed_fwd_simt(a, s);
 }
 
