@@ -30,12 +30,14 @@ struct PackedBwdArgs {
   void* dk = nullptr;
   void* dv = nullptr;
   int lddo = 0, lddq = 0, lddk = 0, lddv = 0;
-  float* delta = nullptr;  // scratch [n_heads, rows]: rowsum(dO * O)
+  float* delta = nullptr;  // scratch [n_heads, rows]: rowsum(P * dP)
 };
 
 bool packed_fwd_tc_supports(const PackedArgs& a);
 int32_t launch_packed_fwd_tc(const PackedArgs& a, cudaStream_t stream);
 int32_t launch_packed_fwd_simt(const PackedArgs& a, cudaStream_t stream);
+bool packed_bwd_tc_supports(const PackedBwdArgs& a);
+int32_t launch_packed_bwd_tc(const PackedBwdArgs& a, cudaStream_t stream);
 int32_t launch_packed_bwd_simt(const PackedBwdArgs& a, cudaStream_t stream);
 
 // ---- rows and sequences --------------------------------------------------------------------------------------------

@@ -1,0 +1,564 @@
+// Packed causal attention backward on the 5th-generation tensor cores (bf16, head size 64 or 128).  With
+//   P = exp(q k^T / sqrt(hs) - lse),  dP = dO v^T,  delta = rowsum(P * dP),  dS = P * (dP - delta) / sqrt(hs)
+// the gradients are dV = P^T dO, dK = dS^T Q, dQ = dS K.  Two passes of one kernel, both free of atomics:
+//   MODE_DQ   a CTA owns 128 queries of a query head and streams the keys and values they see
+//   MODE_DKV  a CTA owns 128 keys of a key head and streams, for every query head of the group, the queries and their
+//             cotangents that see them (so the gradient of a shared head is one sum in a fixed order)
+// Both have the same shape: two fixed tiles F0, F1 and streamed tiles X0, X1,
+//   S = F0 X0^T,  dP = F1 X1^T  (TMEM, rows = the CTA's own rows)  ->  P, dS as bf16 over S, dP in TMEM
+//   DQ  (F0 = Q, F1 = dO, X0 = K, X1 = V):  acc0 += P X0 (see below),  acc1 += dS X0 = dQ
+//   DKV (F0 = K, F1 = V, X0 = Q, X1 = dO):  acc0 += P X1 = dV,         acc1 += dS X0 = dK
+// so P and dS are TMEM operands of the accumulating products and never pass through shared memory.  The softmax threads'
+// two phases run beside the products of the other phase: exponentials (S -> P) beside acc1(n-1) and dP(n), the score
+// gradient (dP -> dS) beside acc0(n) and S(n+1).  S(n+1) may overwrite P(n), and dP(n+1) dS(n), because the tensor pipe
+// runs the products of one thread in order.
+//
+// delta.  Taken from the output as rowsum(dO * o) it carries the rounding of o to bf16, which is not small beside
+// dP - delta where a row sees few keys.  The query pass therefore also sums eps = rowsum(P * (dP - delta0)) in fp32 and
+// acc0 = P K; dQ = acc1 - eps * acc0 / sqrt(hs) is then the gradient for the exact delta = delta0 + eps, which it leaves
+// behind for the key pass.  A tile whose keys fit one block settles eps before it forms dS.
+//
+// Bound: 8 products of 128 x 128 x hs per (query block, key block), of which 5 are the formula's; 512 cycles each at head
+// size 128, 1024 cycles of exponentials.  Rounding to bf16 happens to P, dS and the results; sums are fp32.  All waits
+// are bounded.
+#include <cuda.h>
+
+#include "attention_packed.cuh"
+#include "ptx_sm100.cuh"
+#include "tensor_map.cuh"
+
+namespace b200 {
+
+namespace {
+
+constexpr int BR = 128;
+constexpr int PB_THREADS = 320;  // TMA warp, MMA warp, 8 softmax warps
+constexpr int BSUB = 128 * 128;  // bytes of one [128 rows x 64 columns] bf16 sub-tile
+constexpr int NX = 5;            // stages of streamed tiles (X0(0), X1(0), X0(1), ...)
+enum { MODE_DKV = 0, MODE_DQ = 1 };
+enum : uint32_t { ST_PACKEDB_TIMEOUT = 1u << 19, ST_PACKEDB_ALIGN = 1u << 20 };
+
+template <int HS> struct BCfg {
+  static constexpr int kSubs = HS / 64;
+  static constexpr int kTile = kSubs * BSUB;
+  static constexpr int kX = 2 * kTile;
+  static constexpr int kStat = kX + NX * kTile;  // 2 stages x {lse2[128], delta[128]} of the streamed queries (DKV)
+  static constexpr int kBars = kStat + 2 * 1024;
+  static constexpr int kSmem = kBars + 256;
+  static constexpr int cS = 0, cDP = 128, cAcc0 = 256, cAcc1 = 384;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// D[tmem] (+)= A[tmem] * B[smem desc]
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+
+struct OwnGeo {
+  int r0;       // first own row
+  int x0;       // first streamed row
+  int per_head; // streamed blocks per query head
+  int n_it;     // blocks in all
+};
+
+template <int HS, int MODE>
+__global__ void __launch_bounds__(PB_THREADS, 1)
+    packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                         const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO, PackedBwdArgs a,
+                         float scale, uint32_t* status) {
+  using C = BCfg<HS>;
+  const PackedArgs& f = a.f;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBars);
+  uint64_t* fix_full = bars;            // fixed tiles landed
+  uint64_t* x_full = bars + 1;          // [NX] streamed tile landed
+  uint64_t* x_empty = x_full + NX;      // [NX] every product that reads the tile is complete
+  uint64_t* stat_full = x_empty + NX;   // [2] lse and delta of the streamed queries are in shared memory (DKV)
+  uint64_t* s_full = stat_full + 2;     // S complete in TMEM
+  uint64_t* dp_full = s_full + 1;       // dP complete in TMEM
+  uint64_t* p_full = dp_full + 1;       // P stands in TMEM
+  uint64_t* ds_full = p_full + 1;       // dS stands in TMEM
+  uint64_t* acc_done = ds_full + 1;     // the accumulators are complete
+  uint64_t* met = acc_done + 1;         // the 256 softmax threads meet (a barrier whose wait is bounded too)
+  OwnGeo* geo = reinterpret_cast<OwnGeo*>(bars + 20);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = f.n_heads / f.n_kv_heads;
+  const int head = blockIdx.x;  // DKV: key head, DQ: query head
+  const int hk = MODE == MODE_DKV ? head : head / group;
+  // the longest loops first: early keys are seen by the most queries, late queries see the most keys
+  const int own = MODE == MODE_DKV ? (int)blockIdx.y : (int)gridDim.y - 1 - (int)blockIdx.y;
+  pdl_launch_dependents();
+
+  if (threadIdx.x == 0) {
+    uint32_t bad = 0u;
+    if (ptx::smem_u32(smem) & 1023u) {
+      atomicOr(status, ST_PACKEDB_ALIGN);
+      bad = 1u;
+    }
+    *abort_flag = bad;
+    ptx::mbar_init(fix_full, 1);
+    for (int i = 0; i < NX; ++i) {
+      ptx::mbar_init(&x_full[i], 1);
+      ptx::mbar_init(&x_empty[i], 1);
+    }
+    ptx::mbar_init(&stat_full[0], 32);
+    ptx::mbar_init(&stat_full[1], 32);
+    ptx::mbar_init(s_full, 1);
+    ptx::mbar_init(dp_full, 1);
+    ptx::mbar_init(p_full, 256);
+    ptx::mbar_init(ds_full, 256);
+    ptx::mbar_init(acc_done, 1);
+    ptx::mbar_init(met, 256);
+    ptx::fence_barrier_init();
+    ptx::tma_prefetch_desc(&tmQ);
+    ptx::tma_prefetch_desc(&tmK);
+    ptx::tma_prefetch_desc(&tmV);
+    ptx::tma_prefetch_desc(&tmDO);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(tmem_slot, 512);
+    ptx::tmem_relinquish();
+  }
+  pdl_wait();  // the operands come from the kernels before
+  if (warp == 2) {
+    const int cu_first = max(0, __ldg(f.cu)), end = min(f.rows, __ldg(f.cu + f.n_seqs));
+    OwnGeo g;
+    g.r0 = own * BR;
+    const int last_row = min(g.r0 + BR, end) - 1;  // last own row that belongs to a sequence
+    const int probe = MODE == MODE_DKV ? max(0, last_row) : g.r0;
+    const int s = seq_of_row_warp(f.cu, f.n_seqs, probe);
+    const RowSpan sp = row_span(f.cu, f.n_seqs, s, probe, f.rows);
+    int to;
+    if (MODE == MODE_DKV) {  // queries from the first own row to the end of the last own row's sequence
+      g.x0 = g.r0;
+      to = sp.first <= probe ? sp.last : 0;
+    } else {
+      g.x0 = sp.first <= probe ? sp.first : cu_first;
+      to = last_row + 1;
+    }
+    g.per_head = last_row >= g.r0 && to > g.x0 ? (to - g.x0 + BR - 1) / BR : 0;
+    g.n_it = g.per_head * (MODE == MODE_DKV ? group : 1);
+    if (lane == 0) *geo = g;
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  const bool aborted = *abort_flag != 0u;
+  const OwnGeo g = *geo;
+  const int n_it = g.n_it;
+
+  if (aborted || n_it == 0) {
+    // common exit below
+  } else if (warp == 0) {
+    if (lane == 0) {
+      ptx::mbar_arrive_expect_tx(fix_full, 2 * C::kTile);
+#pragma unroll
+      for (int s = 0; s < C::kSubs; ++s) {
+        ptx::tma_load_2d(smem + s * BSUB, MODE == MODE_DKV ? &tmK : &tmQ, head * HS + 64 * s, g.r0, fix_full);
+        ptx::tma_load_2d(smem + C::kTile + s * BSUB, MODE == MODE_DKV ? &tmV : &tmDO, head * HS + 64 * s, g.r0, fix_full);
+      }
+    }
+    bool ok = true;
+    for (int x = 0; x < 2 * n_it && ok; ++x) {
+      const int st = x % NX, it = x >> 1;
+      const int qh = MODE == MODE_DKV ? hk * group + it / g.per_head : head;
+      const int row = g.x0 + (it % g.per_head) * BR;
+      ok = ptx::mbar_wait_warp(&x_empty[st], ((uint32_t)(x / NX) & 1u) ^ 1u, abort_flag, status, ST_PACKEDB_TIMEOUT);
+      if (!ok) break;
+      if (lane == 0) {
+        const CUtensorMap* map = MODE == MODE_DKV ? ((x & 1) ? &tmDO : &tmQ) : ((x & 1) ? &tmV : &tmK);
+        const int col = (MODE == MODE_DKV ? qh : hk) * HS;
+        ptx::mbar_arrive_expect_tx(&x_full[st], C::kTile);
+#pragma unroll
+        for (int s = 0; s < C::kSubs; ++s)
+          ptx::tma_load_2d(smem + C::kX + st * C::kTile + s * BSUB, map, col + 64 * s, row, &x_full[st]);
+      }
+      if (MODE == MODE_DKV && (x & 1)) {
+        // X1(it) takes the stage X0(it - 2) or an older tile had, so the statistics of it - 2 have been used
+        float* stat = reinterpret_cast<float*>(smem + C::kStat + (it & 1) * 1024);
+#pragma unroll
+        for (int c = lane; c < BR; c += 32) {
+          const int t = row + c;
+          const size_t at = (size_t)qh * f.rows + t;
+          stat[c] = t < f.rows ? f.lse[at] * 1.4426950408889634f : 0.f;
+          stat[BR + c] = t < f.rows ? a.delta[at] : 0.f;
+        }
+        ptx::mbar_arrive(&stat_full[it & 1]);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t id_kk = ptx::idesc_bf16_f32(BR, BR);               // both operands K-major
+      constexpr uint32_t id_tm = ptx::idesc_bf16_f32(BR, HS) | (1u << 16);  // A in TMEM, B MN-major
+      const uint64_t fix_k = ptx::smem_desc_sw128(ptx::smem_u32(smem));
+      const uint64_t x_k = ptx::smem_desc_sw128(ptx::smem_u32(smem + C::kX));
+      const uint64_t x_m = ptx::smem_desc_sw128_mn(ptx::smem_u32(smem + C::kX), BSUB);
+      constexpr uint64_t kT = C::kTile >> 4;
+      bool ok = ptx::mbar_wait(fix_full, 0, abort_flag, status, ST_PACKEDB_TIMEOUT);
+      auto wait_x = [&](int x) {
+        ok = ok && ptx::mbar_wait(&x_full[x % NX], (uint32_t)(x / NX) & 1u, abort_flag, status, ST_PACKEDB_TIMEOUT);
+        if (ok) ptx::tc_fence_after_sync();
+      };
+      auto scores = [&](int which, int it) {  // 0: S = F0 X0^T, 1: dP = F1 X1^T
+        const uint64_t fa = fix_k + (uint64_t)which * kT, xa = x_k + (uint64_t)((2 * it + which) % NX) * kT;
+#pragma unroll
+        for (int k = 0; k < HS / 16; ++k) {
+          const uint64_t off = (uint64_t)(((k >> 2) * BSUB + (k & 3) * 32) >> 4);
+          ptx::mma_bf16_ss(tmem_base + (uint32_t)(which ? C::cDP : C::cS), fa + off, xa + off, id_kk, k > 0 ? 1u : 0u);
+        }
+        ptx::mma_commit(which ? dp_full : s_full);
+      };
+      auto accumulate = [&](int which, int it) {  // 0: acc0 += P X, 1: acc1 += dS X0
+        const int tile = 2 * it + (which == 0 && MODE == MODE_DKV ? 1 : 0);
+        const uint64_t xa = x_m + (uint64_t)(tile % NX) * kT;
+        const uint32_t src = tmem_base + (uint32_t)(which ? C::cDP : C::cS);
+#pragma unroll
+        for (int k = 0; k < BR / 16; ++k)  // P / dS of columns 64h .. 64h+63 stands in TMEM columns 64h .. 64h+31
+          mma_bf16_ts(tmem_base + (uint32_t)(which ? C::cAcc1 : C::cAcc0), src + (uint32_t)((k >> 2) * 64 + (k & 3) * 8),
+                      xa + (uint64_t)(k * (2048 >> 4)), id_tm, (it > 0 || k > 0) ? 1u : 0u);
+      };
+      wait_x(0);
+      if (ok) scores(0, 0);
+      wait_x(1);
+      if (ok) scores(1, 0);
+      if (ok && MODE == MODE_DQ) ptx::mma_commit(&x_empty[1]);  // V has no second reader
+      for (int it = 0; it < n_it && ok; ++it) {
+        const uint32_t ph = (uint32_t)it & 1u;
+        ok = ptx::mbar_wait(p_full, ph, abort_flag, status, ST_PACKEDB_TIMEOUT);
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+        accumulate(0, it);
+        if (MODE == MODE_DKV) ptx::mma_commit(&x_empty[(2 * it + 1) % NX]);
+        if (it + 1 < n_it) {
+          wait_x(2 * it + 2);
+          if (!ok) break;
+          scores(0, it + 1);
+        }
+        ok = ptx::mbar_wait(ds_full, ph, abort_flag, status, ST_PACKEDB_TIMEOUT);
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+        accumulate(1, it);
+        ptx::mma_commit(&x_empty[(2 * it) % NX]);
+        if (it + 1 < n_it) {
+          wait_x(2 * it + 3);
+          if (!ok) break;
+          scores(1, it + 1);
+          if (MODE == MODE_DQ) ptx::mma_commit(&x_empty[(2 * it + 3) % NX]);
+        }
+      }
+      if (ok) ptx::mma_commit(acc_done);
+    }
+    __syncwarp();
+  } else {
+    const int qd = warp & 3;
+    const int hf = (warp - 2) >> 2;   // columns 64 hf .. 64 hf + 63 of a block
+    const int row = qd * 32 + lane;   // TMEM lane: the CTA's own row
+    const int r = g.r0 + row;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(qd * 32) << 16);
+    const uint32_t t_s = lane_base + (uint32_t)(C::cS + hf * 64), t_dp = lane_base + (uint32_t)(C::cDP + hf * 64);
+    const float sl2 = scale * 1.4426950408889634f;
+    const int s = r < f.rows ? seq_of_row(f.cu, 0, f.n_seqs, r) : -1;
+    const RowSpan span = row_span(f.cu, f.n_seqs, s, r, f.rows);
+    const bool live = span.first <= r;
+    float lse2 = 0.f, delta = 0.f, eps = 0.f;
+    if (MODE == MODE_DQ && live) {
+      lse2 = f.lse[(size_t)head * f.rows + r] * 1.4426950408889634f;
+      delta = a.delta[(size_t)head * f.rows + r];
+    }
+    float* share = reinterpret_cast<float*>(smem + C::kStat);  // DQ: [2][128] halves of eps
+    bool ok = true;
+    uint32_t met_phase = 0u;
+    auto meet = [&]() {
+      ptx::mbar_arrive(met);
+      ok = ptx::mbar_wait_warp(met, met_phase, abort_flag, status, ST_PACKEDB_TIMEOUT);
+      met_phase ^= 1u;
+      return ok;
+    };
+    for (int it = 0; it < n_it; ++it) {
+      const uint32_t ph = (uint32_t)it & 1u;
+      const int c0 = g.x0 + (it % g.per_head) * BR + hf * 64;  // streamed row of this thread's first column
+      // columns lo..hi of the 64 form a pair with the own row
+      const int lo = live ? (MODE == MODE_DQ ? span.first : r) - c0 : 64;
+      const int hi = live ? (MODE == MODE_DQ ? r : span.last - 1) - c0 : -1;
+      const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < 63);
+      const float* stat = reinterpret_cast<const float*>(smem + C::kStat + (it & 1) * 1024) + hf * 64;
+      if (MODE == MODE_DKV) {
+        ok = ptx::mbar_wait_warp(&stat_full[it & 1], (uint32_t)(it >> 1) & 1u, abort_flag, status, ST_PACKEDB_TIMEOUT);
+        if (!ok) break;
+      }
+      ok = ptx::mbar_wait_warp(s_full, ph, abort_flag, status, ST_PACKEDB_TIMEOUT);
+      if (!ok) break;
+      ptx::tc_fence_after_sync();
+      float p[64];
+      ptx::tmem_ld32_at<0>(t_s, p);
+      ptx::tmem_ld32_at<32>(t_s + 32u, p);
+      ptx::tmem_ld_wait();
+      uint32_t pk[32];
+#pragma unroll
+      for (int e = 0; e < 64; e += 4) {
+        float4 l4 = make_float4(lse2, lse2, lse2, lse2);
+        if (MODE == MODE_DKV) l4 = *reinterpret_cast<const float4*>(stat + e);
+        p[e] = ex2(fmaf(p[e], sl2, -l4.x));
+        p[e + 1] = ex2(fmaf(p[e + 1], sl2, -l4.y));
+        p[e + 2] = ex2(fmaf(p[e + 2], sl2, -l4.z));
+        p[e + 3] = ex2(fmaf(p[e + 3], sl2, -l4.w));
+      }
+      if (cut) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (e < lo || e > hi) p[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(p[2 * e], p[2 * e + 1]);
+        pk[e] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      // the two halves read and write disjoint columns of S
+      tmem_st32u(t_s, pk);
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before_sync();
+      ptx::mbar_arrive(p_full);
+
+      ok = ptx::mbar_wait_warp(dp_full, ph, abort_flag, status, ST_PACKEDB_TIMEOUT);
+      if (!ok) break;
+      ptx::tc_fence_after_sync();
+      float dp[64];
+      ptx::tmem_ld32_at<0>(t_dp, dp);
+      ptx::tmem_ld32_at<32>(t_dp + 32u, dp);
+      ptx::tmem_ld_wait();
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 64; e += 4) {
+        float4 d4 = make_float4(delta, delta, delta, delta);
+        if (MODE == MODE_DKV) d4 = *reinterpret_cast<const float4*>(stat + BR + e);
+        dp[e] = p[e] * (dp[e] - d4.x);
+        dp[e + 1] = p[e + 1] * (dp[e + 1] - d4.y);
+        dp[e + 2] = p[e + 2] * (dp[e + 2] - d4.z);
+        dp[e + 3] = p[e + 3] * (dp[e + 3] - d4.w);
+      }
+      if (cut) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (e < lo || e > hi) dp[e] = 0.f;
+      }
+      if (MODE == MODE_DQ) {
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int e = 0; e < 64; e += 2) {
+          s0 += dp[e];
+          s1 += dp[e + 1];
+        }
+        sum = s0 + s1;
+        if (n_it == 1) {  // all keys of the row are here: settle delta before dS is rounded
+          share[hf * BR + row] = sum;
+          if (!meet()) break;
+          sum += share[(hf ^ 1) * BR + row];
+          delta += sum;
+#pragma unroll
+          for (int e = 0; e < 64; ++e) dp[e] = fmaf(-p[e], sum, dp[e]);
+        } else {
+          eps += sum;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(dp[2 * e] * scale, dp[2 * e + 1] * scale);
+        pk[e] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      tmem_st32u(t_dp, pk);
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before_sync();
+      ptx::mbar_arrive(ds_full);
+    }
+    if (ok) ok = ptx::mbar_wait_warp(acc_done, 0, abort_flag, status, ST_PACKEDB_TIMEOUT);
+    if (ok) {
+      ptx::tc_fence_after_sync();
+      bool finite = true;
+      if (MODE == MODE_DKV) {
+        // half 0 writes dV, half 1 dK
+        bf16* dst = hf == 0 ? (bf16*)a.dv + (size_t)r * a.lddv : (bf16*)a.dk + (size_t)r * a.lddk;
+        const uint32_t src = lane_base + (uint32_t)(hf == 0 ? C::cAcc0 : C::cAcc1);
+#pragma unroll 1
+        for (int c = 0; c < HS; c += 32) {
+          float v[32];
+          ptx::tmem_ld32(src + (uint32_t)c, v);
+          ptx::tmem_ld_wait();
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              float w[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                w[j] = v[e + j];
+                finite = finite && fabsf(w[j]) < INFINITY;
+              }
+              store8(dst + head * HS + c + e, w);
+            }
+          }
+        }
+      } else {
+        if (n_it > 1) {
+          share[hf * BR + row] = eps;
+          meet();
+          eps += share[(hf ^ 1) * BR + row];
+          delta += eps;
+        }
+        if (live && hf == 0) a.delta[(size_t)head * f.rows + r] = delta;
+        const float back = eps * scale;
+        bf16* dst = (bf16*)a.dq + (size_t)r * a.lddq + head * HS;
+#pragma unroll 1
+        for (int c = hf * (HS / 2); c < (hf + 1) * (HS / 2); c += 32) {
+          float v[32], u[32];
+          ptx::tmem_ld32(lane_base + (uint32_t)(C::cAcc1 + c), v);
+          ptx::tmem_ld32(lane_base + (uint32_t)(C::cAcc0 + c), u);
+          ptx::tmem_ld_wait();
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              float w[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                w[j] = fmaf(-back, u[e + j], v[e + j]);
+                finite = finite && fabsf(w[j]) < INFINITY;
+              }
+              store8(dst + c + e, w);
+            }
+          }
+        }
+      }
+      // Zero weight times an infinity or NaN of a row that is masked here would not be zero: rows that did not come out
+      // finite are computed again over the pairs they are part of alone.  Both halves meet first, so that neither
+      // writes a row again while the other still writes it for the first time.
+      meet();
+      unsigned redo = __ballot_sync(0xffffffffu, ok && live && !finite);
+      while (redo) {
+        const int b = __ffs(redo) - 1;
+        redo &= redo - 1;
+        const int rr = g.r0 + qd * 32 + b;
+        const int first = __shfl_sync(0xffffffffu, span.first, b), last = __shfl_sync(0xffffffffu, span.last, b);
+        const bf16* kr = (const bf16*)f.k + hk * HS;
+        const bf16* vr = (const bf16*)f.v + hk * HS;
+        if (MODE == MODE_DKV) {
+          const size_t st = (size_t)hk * group * f.rows;
+          packed_dkv_row<bf16, HS>((const bf16*)f.q + hk * group * HS, kr + (size_t)rr * f.ldk, vr + (size_t)rr * f.ldv,
+                                   (const bf16*)a.d_o + hk * group * HS, f.lse + st, a.delta + st,
+                                   (bf16*)a.dk + (size_t)rr * a.lddk + hk * HS, (bf16*)a.dv + (size_t)rr * a.lddv + hk * HS,
+                                   f.ldq, a.lddo, f.rows, group, rr, last, scale);
+        } else {
+          const float dl = __shfl_sync(0xffffffffu, delta, b);
+          packed_dq_row<bf16, HS>((const bf16*)f.q + (size_t)rr * f.ldq + head * HS, kr, vr,
+                                  (const bf16*)a.d_o + (size_t)rr * a.lddo + head * HS, f.lse[(size_t)head * f.rows + rr], dl,
+                                  (bf16*)a.dq + (size_t)rr * a.lddq + head * HS, f.ldk, f.ldv, first, rr, scale);
+        }
+      }
+    }
+  }
+
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag) {
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies in flight land before the shared memory is given back
+  }
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// delta0[h, t] = rowsum(dO * o): HS/8 lanes share a row, 16 bytes each.
+template <int HS>
+__global__ void __launch_bounds__(256) packed_delta_vec_kernel(PackedBwdArgs a) {
+  constexpr int L = HS / 8;
+  const PackedArgs& f = a.f;
+  const long long item = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
+  const int li = threadIdx.x % L;
+  const long long items = (long long)f.rows * f.n_heads;
+  const int t = item < items ? (int)(item / f.n_heads) : 0, h = item < items ? (int)(item % f.n_heads) : 0;
+  pdl_launch_dependents();
+  pdl_wait();
+  float x[8], y[8], s = 0.f;
+  load8((const bf16*)f.o + (size_t)t * f.ldo + h * HS + li * 8, x);
+  load8((const bf16*)a.d_o + (size_t)t * a.lddo + h * HS + li * 8, y);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s = fmaf(x[i], y[i], s);
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (item < items && li == 0) a.delta[(size_t)h * f.rows + t] = s;
+}
+
+template <int HS>
+int32_t launch_hs(const PackedBwdArgs& a, cudaStream_t stream) {
+  using C = BCfg<HS>;
+  const PackedArgs& f = a.f;
+  CUtensorMap tq, tk, tv, tdo;
+  B200_TRY(make_map_2d(&tq, f.q, f.rows, f.n_heads * HS, f.ldq, BR));
+  B200_TRY(make_map_2d(&tk, f.k, f.rows, f.n_kv_heads * HS, f.ldk, BR));
+  B200_TRY(make_map_2d(&tv, f.v, f.rows, f.n_kv_heads * HS, f.ldv, BR));
+  B200_TRY(make_map_2d(&tdo, a.d_o, f.rows, f.n_heads * HS, a.lddo, BR));
+  auto dq = packed_bwd_tc_kernel<HS, MODE_DQ>;
+  auto dkv = packed_bwd_tc_kernel<HS, MODE_DKV>;
+  static PerDeviceOnce attr_once;
+  B200_TRY(attr_once.run([&](int&) -> int32_t {
+    B200_CUDA_OK(cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    B200_CUDA_OK(cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    return B200_OK;
+  }));
+  const float scale = 1.f / sqrtf((float)HS);
+  const long long lanes = (long long)f.rows * f.n_heads * (HS / 8);
+  B200_CUDA_OK(launch_pdl(packed_delta_vec_kernel<HS>, dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, stream, a));
+  B200_LAUNCH_OK("packed_delta_vec_kernel");
+  const unsigned blocks = (unsigned)cdiv(f.rows, BR);
+  B200_CUDA_OK(launch_pdl(dq, dim3(f.n_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, tq, tk, tv, tdo, a, scale,
+                          device_status_word()));
+  B200_LAUNCH_OK("packed_bwd_tc_kernel<dq>");
+  B200_CUDA_OK(launch_pdl(dkv, dim3(f.n_kv_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, tq, tk, tv, tdo, a, scale,
+                          device_status_word()));
+  B200_LAUNCH_OK("packed_bwd_tc_kernel<dkv>");
+  return B200_OK;
+}
+
+}  // namespace
+
+bool packed_bwd_tc_supports(const PackedBwdArgs& a) {
+  const PackedArgs& f = a.f;
+  return f.dtype == B200_BF16 && (f.head_size == 64 || f.head_size == 128) && f.ldq % 8 == 0 && f.ldk % 8 == 0 &&
+         f.ldv % 8 == 0 && f.ldo % 8 == 0 && a.lddo % 8 == 0 && a.lddq % 8 == 0 && a.lddk % 8 == 0 && a.lddv % 8 == 0 &&
+         aligned16(f.q) && aligned16(f.k) && aligned16(f.v) && aligned16(f.o) && aligned16(a.d_o) && aligned16(a.dq) &&
+         aligned16(a.dk) && aligned16(a.dv) && cdiv(f.rows, BR) <= 65535 &&
+         (long long)f.rows * f.n_heads * (f.head_size / 8) / 256 < 0x7fffffffLL;
+}
+
+int32_t launch_packed_bwd_tc(const PackedBwdArgs& a, cudaStream_t stream) {
+  if (!packed_bwd_tc_supports(a))
+    return fail(B200_ERR_UNSUPPORTED, "packed attention backward on tensor cores needs bf16, head size 64 or 128 and 16-byte aligned rows");
+  if (a.f.head_size == 64) return launch_hs<64>(a, stream);
+  return launch_hs<128>(a, stream);
+}
+
+}  // namespace b200

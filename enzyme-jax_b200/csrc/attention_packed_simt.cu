@@ -177,7 +177,9 @@ __global__ void __launch_bounds__(128) packed_delta_kernel(PackedBwdArgs a) {
   if (t < a.f.rows && part == 0) a.delta[(size_t)h * a.f.rows + t] = s;
 }
 
-// dQ: a CTA owns 32 query rows and streams the keys and values they see.
+// dQ: a CTA owns 32 query rows and streams the keys and values they see.  With bf16 outputs rowsum(dO * o) carries the
+// rounding of o, which is not small beside dP - delta where a row sees few keys: the pass then also sums
+// eps = rowsum(P * (dP - delta0)) and P K, subtracts eps P K / sqrt(hs) and leaves delta0 + eps for the key pass.
 template <typename T, int HS>
 __global__ void __launch_bounds__(128) packed_dq_simt_kernel(PackedBwdArgs a, float scale, bool vec) {
   using Q = Quarter<HS>;
@@ -190,12 +192,14 @@ __global__ void __launch_bounds__(128) packed_dq_simt_kernel(PackedBwdArgs a, fl
   const int row0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * RB, t = row0 + (threadIdx.x >> 2);
   const int h = blockIdx.y, hk = h / (f.n_heads / f.n_kv_heads);
   const CtaRows me = cta_rows(f.cu, f.n_seqs, row0, f.rows, &lo, &hi);
-  float qr[DPT], gr[DPT], acc[DPT];
+  constexpr bool kExact = sizeof(T) == 2;
+  float qr[DPT], gr[DPT], acc[DPT], pk[kExact ? DPT : 4], eps = 0.f;
 #pragma unroll
   for (int i = 0; i < DPT; ++i) {
     qr[i] = me.live ? to_f32(((const T*)f.q)[(size_t)t * f.ldq + h * HS + part * DPT + i]) : 0.f;
     gr[i] = me.live ? to_f32(((const T*)a.d_o)[(size_t)t * a.lddo + h * HS + part * DPT + i]) : 0.f;
     acc[i] = 0.f;
+    if (kExact) pk[i] = 0.f;
   }
   const float lse = me.live ? f.lse[(size_t)h * f.rows + t] : 0.f;
   const float delta = me.live ? a.delta[(size_t)h * f.rows + t] : 0.f;
@@ -214,14 +218,20 @@ __global__ void __launch_bounds__(128) packed_dq_simt_kernel(PackedBwdArgs a, fl
       const float dp = dot_quarter(gr, vq + uu * Q::kRow);
       if (uu >= from && uu <= to) {
         const float p = exp_by_build(s * scale - lse);
-        axpy_quarter(acc, p * (dp - delta) * scale, kq + uu * Q::kRow);
+        const float w = p * (dp - delta);
+        axpy_quarter(acc, w * scale, kq + uu * Q::kRow);
+        if constexpr (kExact) {
+          eps += w;
+          axpy_quarter(pk, p, kq + uu * Q::kRow);
+        }
       }
     }
   }
   if (me.live) {
     T* dq = (T*)a.dq + (size_t)t * a.lddq + h * HS + part * DPT;
 #pragma unroll
-    for (int i = 0; i < DPT; ++i) dq[i] = from_f32<T>(acc[i]);
+    for (int i = 0; i < DPT; ++i) dq[i] = from_f32<T>(kExact ? fmaf(-eps * scale, pk[i], acc[i]) : acc[i]);
+    if (kExact && part == 0) a.delta[(size_t)h * f.rows + t] = delta + eps;
   }
 }
 
@@ -397,7 +407,7 @@ int32_t b200_attention_packed_backward(const void* q, const void* k, const void*
   if (!q || !k || !v || !o || !lse || !d_o || !dq || !dk || !dv || !delta_scratch || !cu_seqlens)
     return fail(B200_ERR_INVALID_ARG, "null operand");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (impl == 1) return fail(B200_ERR_UNSUPPORTED, "no tensor-core kernel for this shape");
+  if (impl == 1 || (impl == 0 && packed_bwd_tc_supports(a))) return launch_packed_bwd_tc(a, s);
   return launch_packed_bwd_simt(a, s);
 }
 
