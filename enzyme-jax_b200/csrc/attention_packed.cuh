@@ -48,7 +48,7 @@ __device__ __forceinline__ int seq_of_row(const int32_t* __restrict__ cu, int lo
   --lo;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (__ldg(cu + mid) <= t) lo = mid;
+    if (*(cu + mid) <= t) lo = mid;
     else hi = mid - 1;
   }
   return lo;
@@ -61,7 +61,7 @@ __device__ __forceinline__ int seq_of_row_warp(const int32_t* __restrict__ cu, i
   while (lo < hi) {
     const int step = (hi - lo + 31) / 32;
     const int probe = lo + 1 + lane * step;  // ascending; the answer is behind every probe that holds
-    const bool holds = probe <= hi && __ldg(cu + probe) <= t;
+    const bool holds = probe <= hi && *(cu + probe) <= t;
     const unsigned m = __ballot_sync(0xffffffffu, holds);
     // with cu ascending the lanes that hold are the lowest ones; their number alone bounds the answer in any case
     const int n = __popc(m);
@@ -79,8 +79,8 @@ struct RowSpan { int first, last; };
 __device__ __forceinline__ RowSpan row_span(const int32_t* __restrict__ cu, int n_seqs, int s, int t, int rows) {
   RowSpan r{t + 1, t + 1};
   if (s >= 0 && s < n_seqs && t < rows) {
-    r.first = max(0, min(t, __ldg(cu + s)));
-    r.last = min(rows, max(t + 1, __ldg(cu + s + 1)));
+    r.first = max(0, min(t, *(cu + s)));
+    r.last = min(rows, max(t + 1, *(cu + s + 1)));
   }
   return r;
 }

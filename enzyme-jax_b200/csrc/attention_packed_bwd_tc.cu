@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(PB_THREADS, 1)
   }
   pdl_wait();  // the operands come from the kernels before
   if (warp == 2) {
-    const int cu_first = max(0, __ldg(f.cu)), end = min(f.rows, __ldg(f.cu + f.n_seqs));
+    const int cu_first = max(0, *(f.cu)), end = min(f.rows, *(f.cu + f.n_seqs));
     OwnGeo g;
     g.r0 = own * BR;
     const int last_row = min(g.r0 + BR, end) - 1;  // last own row that belongs to a sequence

@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
   pdl_wait();  // q, k, v and cu_seqlens come from the kernels before
   if (warp == 2) {
     // rows and keys of the two tiles
-    const int cu_first = max(0, __ldg(a.cu)), end = min(a.rows, __ldg(a.cu + a.n_seqs));
+    const int cu_first = max(0, *(a.cu)), end = min(a.rows, *(a.cu + a.n_seqs));
     int from[2], to[2], base = 0x7fffffff;
     TileGeo g[2];
 #pragma unroll
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
       from[i] = cu_first;
       if (idx < n_tiles) {
         const int s = seq_of_row_warp(a.cu, a.n_seqs, g[i].t0);
-        if (s >= 0 && s < a.n_seqs) from[i] = max(0, min(g[i].t0, __ldg(a.cu + s)));
+        if (s >= 0 && s < a.n_seqs) from[i] = max(0, min(g[i].t0, *(a.cu + s)));
       } else {
         to[i] = -1;
       }

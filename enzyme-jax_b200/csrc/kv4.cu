@@ -42,17 +42,17 @@ __device__ __forceinline__ bool place_of(const Kv4RowsArgs& a, int t, int hk, si
   int lo = -1, hi = a.n_seqs;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (__ldg(a.cu + mid) <= t) lo = mid;
+    if (*(a.cu + mid) <= t) lo = mid;
     else hi = mid - 1;
   }
   if (lo < 0 || lo >= a.n_seqs) return false;
-  const long long pos = (long long)(t - __ldg(a.cu + lo)) + (a.before ? __ldg(a.before + lo) : 0);
+  const long long pos = (long long)(t - *(a.cu + lo)) + (a.before ? *(a.before + lo) : 0);
   const long long slot = pos / a.pool.page_size;
   if (pos < 0 || slot >= a.pool.max_pages) {
     atomicOr(a.status, ST_BAD_PAGE);
     return false;
   }
-  const int page = __ldg(a.pool.table + (size_t)lo * a.pool.max_pages + slot);
+  const int page = *(a.pool.table + (size_t)lo * a.pool.max_pages + slot);
   if ((unsigned)page >= (unsigned)a.pool.n_pages) {
     atomicOr(a.status, ST_BAD_PAGE);
     return false;
@@ -165,6 +165,8 @@ __global__ void __launch_bounds__(SW * 32) kv4_decode_simt_kernel(Kv4DecodeArgs 
   __shared__ float s_acc[SW][HS], s_m[SW], s_l[SW];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LPK, li = lane % LPK;
   const bool lane_on = li * 8 < HS;
+  pdl_launch_dependents();
+  pdl_wait();  // everything below comes from the kernels before
   unit_prefix<SW * 32>(a, pre, warp_sums);
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i <= a.batch; i += blockDim.x) a.prefix[i] = pre[i];
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(SW * 32) kv4_decode_simt_kernel(Kv4DecodeArgs 
         live[g] = u < c1;
         kw[g] = vw[g] = kp[g] = vp[g] = 0u;
         if (live[g]) {
-          const int page = __ldg(table + u / p.page_size);
+          const int page = *(table + u / p.page_size);
           live[g] = (unsigned)page < (unsigned)p.n_pages;
           if (live[g]) {
             const size_t row = ((size_t)page * p.n_kv_heads + hk) * p.page_size + u % p.page_size;
@@ -301,6 +303,7 @@ template <typename T, int HS>
 __global__ void __launch_bounds__(128) kv4_join_kernel(Kv4DecodeArgs a, int grid) {
   const int nseg = a.pool.n_kv_heads * a.subs;
   const int b = blockIdx.x / nseg, seg = blockIdx.x % nseg;
+  pdl_launch_dependents();
   pdl_wait();
   const int p0 = a.prefix[b], nb = a.prefix[b + 1] - p0;
   const long long units = (long long)a.prefix[a.batch] * nseg;
@@ -363,15 +366,13 @@ int32_t check_pool_ptrs(const char* what, const Kv4Pool& p) {
   return B200_OK;
 }
 
-// Grid of the decode kernels: two resident CTAs of 4 warps per SM would not cover HBM latency, so up to kCtasPerSm are
-// launched; a range may hold less than a whole segment, so a single long sequence fills the GPU too.
-constexpr int kCtasPerSm = 8;
+// Grid of the CUDA-core decode kernel: the CTAs an SM can hold (a range may hold less than a whole segment, so a single
+// long sequence fills the GPU too).
+int decode_simt_grid() { return 7 * sm_count(); }
 
-int decode_grid() { return kCtasPerSm * sm_count(); }
+size_t partial_floats(int ctas, int cols, int head_size) { return (size_t)2 * ctas * cols * (head_size + 2); }
 
 }  // namespace
-
-size_t kv4_partial_floats(int ctas, int cols, int head_size) { return (size_t)2 * ctas * cols * (head_size + 2); }
 
 }  // namespace b200
 
@@ -448,7 +449,8 @@ int32_t b200_attention_decode_kv4_scratch_bytes(int32_t batch, int32_t n_heads, 
   if (batch < 0 || n_heads <= 0 || n_kv_heads <= 0 || head_size <= 0 || n_heads % n_kv_heads)
     return fail(B200_ERR_BAD_SHAPE, "kv4 decode: batch=%d heads=%d kv_heads=%d head_size=%d", batch, n_heads, n_kv_heads, head_size);
   const int cols = std::min(8, n_heads / n_kv_heads);
-  *bytes = align_up(((size_t)std::min(batch, kMaxSlice) + 1) * 4, 256) + kv4_partial_floats(decode_grid(), cols, head_size) * 4;
+  const size_t floats = std::max(partial_floats(decode_simt_grid(), 1, head_size), partial_floats(kv4_decode_mma_grid(), cols, head_size));
+  *bytes = align_up(((size_t)std::min(batch, kMaxSlice) + 1) * 4, 256) + floats * 4;
   return B200_OK;
 }
 
@@ -482,23 +484,31 @@ int32_t b200_attention_decode_kv4(const void* q, const void* codes, const void* 
   a.scale = 1.f / sqrtf((float)head_size);
   a.prefix = (int32_t*)scratch;
   a.partials = (float*)((char*)scratch + align_up(((size_t)std::min(batch, kMaxSlice) + 1) * 4, 256));
-  if (impl == 1) return fail(B200_ERR_UNSUPPORTED, "no tensor-core kernel for this shape");
+  const bool mma = impl != 2 && kv4_decode_mma_supports(a);
+  if (impl == 1 && !mma)
+    return fail(B200_ERR_UNSUPPORTED, "kv4 decode on tensor cores needs bf16, head size 64 or 128 and pages of a multiple of 16 rows");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  a.subs = n_heads / n_kv_heads; a.cols = 1;
+  const int group = n_heads / n_kv_heads;
+  a.cols = mma ? std::min(8, group) : 1;
+  a.subs = (group + a.cols - 1) / a.cols;
   const size_t es = dtype == B200_BF16 ? 2 : 4;
-  const long long units_per_seq = ((long long)max_pages * page_size + kUnit - 1) / kUnit * n_heads;
+  const long long units_per_seq = ((long long)max_pages * page_size + kUnit - 1) / kUnit * n_kv_heads * a.subs;
   for (int b0 = 0; b0 < batch; b0 += kMaxSlice) {
     a.batch = std::min(kMaxSlice, batch - b0);
     a.q = (const char*)q + (size_t)b0 * ldq * es;
     a.o = (char*)o + (size_t)b0 * ldo * es;
     a.ctx = ctx_lens + b0;
     a.pool.table = page_table + (size_t)b0 * max_pages;
-    const int grid = (int)std::max(1LL, std::min<long long>(decode_grid(), units_per_seq * a.batch));
+    const int grid = (int)std::max(1LL, std::min<long long>(mma ? kv4_decode_mma_grid() : decode_simt_grid(), units_per_seq * a.batch));
     B200_TRY(by_type("kv4 decode", dtype, head_size, [&](auto t, auto hs) -> int32_t {
       using T = decltype(t);
       constexpr int HS = decltype(hs)::value;
-      kv4_decode_simt_kernel<T, HS><<<grid, SW * 32, (a.batch + 1) * sizeof(int32_t), s>>>(a);
-      B200_LAUNCH_OK("kv4_decode_simt_kernel");
+      if (mma) {
+        B200_TRY(launch_kv4_decode_mma(a, grid, s));
+      } else {
+        B200_CUDA_OK(launch_pdl(kv4_decode_simt_kernel<T, HS>, dim3(grid), dim3(SW * 32), (a.batch + 1) * sizeof(int32_t), s, a));
+        B200_LAUNCH_OK("kv4_decode_simt_kernel");
+      }
       B200_CUDA_OK(launch_pdl(kv4_join_kernel<T, HS>, dim3(a.batch * n_kv_heads * a.subs), dim3(128), 0, s, a, grid));
       B200_LAUNCH_OK("kv4_join_kernel");
       return B200_OK;

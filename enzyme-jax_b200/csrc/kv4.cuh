@@ -48,7 +48,7 @@ constexpr int kMaxSlice = 4096;  // sequences per launch: their unit prefix is h
 
 __device__ __forceinline__ int kv4_len(const Kv4DecodeArgs& a, int b) {
   const long long cap = (long long)a.pool.max_pages * a.pool.page_size;
-  const int n = __ldg(a.ctx + b);
+  const int n = *(a.ctx + b);
   return n <= 0 ? 0 : (n < cap ? n : (int)cap);
 }
 __device__ __forceinline__ long long range_start(long long units, int ctas, int c) { return units * c / ctas; }
@@ -83,6 +83,8 @@ template <int THREADS> __device__ __forceinline__ void unit_prefix(const Kv4Deco
   __syncthreads();
 }
 
-size_t kv4_partial_floats(int ctas, int cols, int head_size);
+bool kv4_decode_mma_supports(const Kv4DecodeArgs& a);
+int kv4_decode_mma_grid();
+int32_t launch_kv4_decode_mma(const Kv4DecodeArgs& a, int grid, cudaStream_t stream);
 
 }  // namespace b200
