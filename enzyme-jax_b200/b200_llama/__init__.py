@@ -10,6 +10,7 @@ status.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from ctypes import POINTER, byref, c_char_p, c_float, c_int32, c_size_t, c_uint32, c_void_p
 from typing import Dict, Optional
@@ -310,37 +311,34 @@ def _device_of(what: str, **tensors):
     return dev
 
 
-class _On:
-    """Makes ``device`` current for a call, so that the stream and the launches are that device's."""
-
-    def __init__(self, device):
-        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-        return _stream()
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
-        return False
+def _call(dev: torch.device, fn, *args) -> None:
+    """``fn(*args, stream)`` with ``dev`` current, on its current stream (the raw handle: building the Stream object costs
+    more than the launch)."""
+    if dev.index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if status != 0:
+        check(status)
 
 
 def _rows(what: str, name: str, t: torch.Tensor, cols: int, rows: Optional[int] = None,
           dtype: Optional[torch.dtype] = None) -> int:
     """Row pitch of a [rows, cols] tensor with unit column stride."""
-    if t.dim() != 2 or t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
-        raise B200Error(2, f"{what}: {name} has shape {tuple(t.shape)}, expected [{'rows' if rows is None else rows}, {cols}]")
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != cols or (rows is not None and shape[0] != rows):
+        raise B200Error(2, f"{what}: {name} has shape {tuple(shape)}, expected [{'rows' if rows is None else rows}, {cols}]")
     if dtype is not None and t.dtype != dtype:
         raise B200Error(3, f"{what}: {name} is {t.dtype}, expected {dtype}")
-    if t.shape[0] <= 1:
-        if cols > 1 and t.shape[0] == 1 and t.stride(1) != 1:
+    ld, unit = t.stride()
+    if shape[0] <= 1:
+        if cols > 1 and shape[0] == 1 and unit != 1:
             raise B200Error(2, f"{what}: {name} needs unit column stride")
         return max(cols, 1)
-    if t.stride(1) != 1 or t.stride(0) < cols:
+    if unit != 1 or ld < cols:
         raise B200Error(2, f"{what}: {name} needs unit column stride and rows that do not overlap")
-    return t.stride(0)
+    return ld
 
 
 def _index(what: str, name: str, t: torch.Tensor, dim: int = 1) -> None:
@@ -380,10 +378,9 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         lse = torch.empty(n_heads, rows, dtype=torch.float32, device=dev)
     elif lse.dtype != torch.float32 or tuple(lse.shape) != (n_heads, rows) or not lse.is_contiguous():
         raise B200Error(2, f"{what}: lse must be a contiguous fp32 [{n_heads}, {rows}]")
-    with _On(dev) as stream:
-        check(lib().b200_attention_packed(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-                                          cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, rows, n_heads, n_kv_heads, hs,
-                                          ldq, ldk, ldv, ldo, _dt(dt), impl, stream))
+    _call(dev, lib().b200_attention_packed, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+          cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, rows, n_heads, n_kv_heads, hs, ldq, ldk, ldv, ldo, _dt(dt),
+          impl)
     return out, lse
 
 
@@ -416,11 +413,10 @@ def attention_packed_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     lddk = _rows(what, "dk", dk, wk, rows, dt)
     lddv = _rows(what, "dv", dv, wk, rows, dt)
     delta = torch.empty(n_heads * rows, dtype=torch.float32, device=dev)
-    with _On(dev) as stream:
-        check(lib().b200_attention_packed_backward(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), d_o.data_ptr(), dq.data_ptr(),
-            dk.data_ptr(), dv.data_ptr(), delta.data_ptr(), cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, rows, n_heads,
-            n_kv_heads, hs, ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv, _dt(dt), impl, stream))
+    _call(dev, lib().b200_attention_packed_backward, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+          lse.data_ptr(), d_o.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(),
+          cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, rows, n_heads, n_kv_heads, hs, ldq, ldk, ldv, ldo, lddo,
+          lddq, lddk, lddv, _dt(dt), impl)
     return dq, dk, dv
 
 
@@ -469,11 +465,9 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, params: to
     n_seqs = _kv4_rows(what, page_table, cu_seqlens, ctx_before)
     ldk = _rows(what, "k", k, n_kv_heads * hs)
     ldv = _rows(what, "v", v, n_kv_heads * hs, k.shape[0], k.dtype)
-    with _On(dev) as stream:
-        check(lib().b200_kv4_append(k.data_ptr(), v.data_ptr(), codes.data_ptr(), params.data_ptr(),
-                                    page_table.data_ptr(), cu_seqlens.data_ptr(), _ptr(ctx_before), n_seqs, k.shape[0],
-                                    n_kv_heads, hs, ldk, ldv, n_pages, page_size, page_table.shape[1], _dt(k.dtype),
-                                    stream))
+    _call(dev, lib().b200_kv4_append, k.data_ptr(), v.data_ptr(), codes.data_ptr(), params.data_ptr(),
+          page_table.data_ptr(), cu_seqlens.data_ptr(), _ptr(ctx_before), n_seqs, k.shape[0], n_kv_heads, hs, ldk,
+          ldv, n_pages, page_size, page_table.shape[1], _dt(k.dtype))
 
 
 def kv4_read(codes: torch.Tensor, params: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -491,11 +485,17 @@ def kv4_read(codes: torch.Tensor, params: torch.Tensor, page_table: torch.Tensor
     v = torch.empty(rows, n_kv_heads * hs, dtype=dtype, device=dev) if v is None else v
     ldk = _rows(what, "k", k, n_kv_heads * hs, rows, dtype)
     ldv = _rows(what, "v", v, n_kv_heads * hs, rows, dtype)
-    with _On(dev) as stream:
-        check(lib().b200_kv4_read(k.data_ptr(), v.data_ptr(), codes.data_ptr(), params.data_ptr(),
-                                  page_table.data_ptr(), cu_seqlens.data_ptr(), _ptr(ctx_before), n_seqs, rows,
-                                  n_kv_heads, hs, ldk, ldv, n_pages, page_size, page_table.shape[1], _dt(dtype), stream))
+    _call(dev, lib().b200_kv4_read, k.data_ptr(), v.data_ptr(), codes.data_ptr(), params.data_ptr(),
+          page_table.data_ptr(), cu_seqlens.data_ptr(), _ptr(ctx_before), n_seqs, rows, n_kv_heads, hs, ldk, ldv,
+          n_pages, page_size, page_table.shape[1], _dt(dtype))
     return k, v
+
+
+@functools.lru_cache(maxsize=256)
+def _kv4_scratch_bytes(batch: int, n_heads: int, n_kv_heads: int, hs: int) -> int:
+    n = c_size_t(0)
+    check(lib().b200_attention_decode_kv4_scratch_bytes(batch, n_heads, n_kv_heads, hs, byref(n)))
+    return n.value
 
 
 def attention_decode_kv4(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, page_table: torch.Tensor,
@@ -519,16 +519,12 @@ def attention_decode_kv4(q: torch.Tensor, codes: torch.Tensor, params: torch.Ten
     if out is None:
         out = torch.empty(batch, n_heads * hs, dtype=q.dtype, device=dev)
     ldo = _rows(what, "out", out, n_heads * hs, batch, q.dtype)
-    with _On(dev) as stream:
-        if scratch is None:
-            n = c_size_t(0)
-            check(lib().b200_attention_decode_kv4_scratch_bytes(batch, n_heads, n_kv_heads, hs, byref(n)))
-            scratch = torch.empty(n.value, dtype=torch.uint8, device=dev)
-        check(lib().b200_attention_decode_kv4(q.data_ptr(), codes.data_ptr(), params.data_ptr(), page_table.data_ptr(),
-                                              ctx_lens.data_ptr(), out.data_ptr(), scratch.data_ptr(),
-                                              scratch.numel() * scratch.element_size(), batch, n_heads, n_kv_heads, hs,
-                                              ldq, ldo, n_pages, page_size, page_table.shape[1], _dt(q.dtype), impl,
-                                              stream))
+    if scratch is None:
+        scratch = torch.empty(_kv4_scratch_bytes(batch, n_heads, n_kv_heads, hs), dtype=torch.uint8, device=dev)
+    _call(dev, lib().b200_attention_decode_kv4, q.data_ptr(), codes.data_ptr(), params.data_ptr(),
+          page_table.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), scratch.data_ptr(),
+          scratch.numel() * scratch.element_size(), batch, n_heads, n_kv_heads, hs, ldq, ldo, n_pages, page_size,
+          page_table.shape[1], _dt(q.dtype), impl)
     return out
 
 
@@ -571,10 +567,9 @@ def _copy_pages(what, pool, src, dst, rows, page_table, page_map) -> None:
     dev = _device_of(what, pool=pool, src=src, dst=dst, rows=rows, page_table=page_table, page_map=page_map)
     if pool.numel() == 0:
         return
-    with _On(dev) as stream:
-        check(lib().b200_copy_pages(pool.data_ptr(), planes, n_pages, n_heads, page_size, row * pool.element_size(),
-                                    src.data_ptr(), dst.data_ptr(), _ptr(rows), src.numel(), _ptr(page_table),
-                                    0 if page_table is None else page_table.numel(), _ptr(page_map), stream))
+    _call(dev, lib().b200_copy_pages, pool.data_ptr(), planes, n_pages, n_heads, page_size, row * pool.element_size(),
+          src.data_ptr(), dst.data_ptr(), _ptr(rows), src.numel(), _ptr(page_table),
+          0 if page_table is None else page_table.numel(), _ptr(page_map))
 
 
 def copy_pages(pool: torch.Tensor, src, dst, rows=None) -> None:

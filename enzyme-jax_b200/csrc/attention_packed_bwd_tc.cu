@@ -529,16 +529,18 @@ int32_t launch_hs(const PackedBwdArgs& a, cudaStream_t stream) {
     B200_CUDA_OK(cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     return B200_OK;
   }));
+  uint32_t* status = device_status_word();
+  if (!status) return fail(B200_ERR_CUDA, "no device status word");
   const float scale = 1.f / sqrtf((float)HS);
   const long long lanes = (long long)f.rows * f.n_heads * (HS / 8);
   B200_CUDA_OK(launch_pdl(packed_delta_vec_kernel<HS>, dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, stream, a));
   B200_LAUNCH_OK("packed_delta_vec_kernel");
   const unsigned blocks = (unsigned)cdiv(f.rows, BR);
   B200_CUDA_OK(launch_pdl(dq, dim3(f.n_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, tq, tk, tv, tdo, a, scale,
-                          device_status_word()));
+                          status));
   B200_LAUNCH_OK("packed_bwd_tc_kernel<dq>");
   B200_CUDA_OK(launch_pdl(dkv, dim3(f.n_kv_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, tq, tk, tv, tdo, a, scale,
-                          device_status_word()));
+                          status));
   B200_LAUNCH_OK("packed_bwd_tc_kernel<dkv>");
   return B200_OK;
 }

@@ -406,9 +406,11 @@ int32_t launch_hs(const PackedArgs& a, cudaStream_t stream) {
     B200_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     return B200_OK;
   }));
+  uint32_t* status = device_status_word();
+  if (!status) return fail(B200_ERR_CUDA, "no device status word");
   const long long pairs = ((long long)cdiv(a.rows, TR) * (a.n_heads / a.n_kv_heads) + 1) / 2;
   B200_CUDA_OK(launch_pdl(kern, dim3(a.n_kv_heads, (unsigned)pairs), dim3(PK_THREADS), C::kSmem, stream, tq, tk, tv, a,
-                          1.f / sqrtf((float)HS), device_status_word()));
+                          1.f / sqrtf((float)HS), status));
   B200_LAUNCH_OK("packed_fwd_tc_kernel");
   return B200_OK;
 }

@@ -449,7 +449,7 @@ int32_t b200_attention_decode_kv4_scratch_bytes(int32_t batch, int32_t n_heads, 
   if (batch < 0 || n_heads <= 0 || n_kv_heads <= 0 || head_size <= 0 || n_heads % n_kv_heads)
     return fail(B200_ERR_BAD_SHAPE, "kv4 decode: batch=%d heads=%d kv_heads=%d head_size=%d", batch, n_heads, n_kv_heads, head_size);
   const int cols = std::min(8, n_heads / n_kv_heads);
-  const size_t floats = std::max(partial_floats(decode_simt_grid(), 1, head_size), partial_floats(kv4_decode_mma_grid(), cols, head_size));
+  const size_t floats = std::max(partial_floats(decode_simt_grid(), 1, head_size), partial_floats(kv4_decode_mma_grid(cols), cols, head_size));
   *bytes = align_up(((size_t)std::min(batch, kMaxSlice) + 1) * 4, 256) + floats * 4;
   return B200_OK;
 }
@@ -499,7 +499,7 @@ int32_t b200_attention_decode_kv4(const void* q, const void* codes, const void* 
     a.o = (char*)o + (size_t)b0 * ldo * es;
     a.ctx = ctx_lens + b0;
     a.pool.table = page_table + (size_t)b0 * max_pages;
-    const int grid = (int)std::max(1LL, std::min<long long>(mma ? kv4_decode_mma_grid() : decode_simt_grid(), units_per_seq * a.batch));
+    const int grid = (int)std::max(1LL, std::min<long long>(mma ? kv4_decode_mma_grid(a.cols) : decode_simt_grid(), units_per_seq * a.batch));
     B200_TRY(by_type("kv4 decode", dtype, head_size, [&](auto t, auto hs) -> int32_t {
       using T = decltype(t);
       constexpr int HS = decltype(hs)::value;

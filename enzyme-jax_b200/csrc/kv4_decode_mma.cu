@@ -2,18 +2,19 @@
 // multiple of 16 rows, grouped heads).
 //
 // A byte of codes holds two elements, so at HBM speed an SM receives 23 bytes and would have to expand and multiply 46
-// elements per cycle for q.k and for p.v -- more than its FP32 lanes do.  The codes therefore go into mma.sync
-// (m16n8k16, bf16, fp32 sums) as they are: a 4-bit code n shifted into bits 3..6 of a bf16 whose exponent is that of 1.0
-// IS the number 1 + n/16, exactly, so two elements cost one shift and one logic operation.  The row's scale s and
-// minimum m enter afterwards, once per row:
-//   q.k = 16 s sum q (1 + n/16) + (m - 16 s) sum q
-//   o   = sum_j (16 s_j p_j) (1 + n_j/16) + sum_j p_j (m_j - 16 s_j)
-// The 16 rows of an A operand are 16 keys (q.k) or 16 head dimensions (p.v); its 8 columns are the query heads of the
-// group.  The order of the elements inside a contraction is free, so a lane takes 16 contiguous bytes of a key row and
-// the query fragments are laid out to match; nothing is shuffled.  The weights 16 s p are kept to 16 bits as the sum of
-// two bf16 numbers: with up to four heads both parts share one product (columns 0..3 and 4..7 carry the same heads, the
-// first the leading part, the last the rest), with five to eight heads a second product adds the rest.  Groups beyond
-// eight are cut into subsets of eight.
+// elements per cycle for q.k and for p.v -- more than its FP32 lanes do.  The codes therefore go into the integer
+// mma.sync (m16n8k32, 8 x 8 bits, 32-bit sums) as they are: eight codes of a word become bytes with one shift and two
+// masks.  (The same product on e4m3 numbers, which hold the codes too, is made of conversions here and took 1.3 times as
+// long as bf16 operands; the integer one runs at twice their rate.)  The row's scale s and minimum m enter afterwards:
+//   q.k = s sum q n + m sum q              o = sum_j (s_j p_j) n_j + sum_j p_j m_j
+// The 16 rows of an A operand are 16 keys (q.k) or 16 head dimensions (p.v); its 8 columns are four query heads twice,
+// because the other operand is a 16-bit integer in two bytes: query elements in steps of 1/32512 of their head's largest
+// (two products), weights s p -- kept in fp32 until then -- in steps of 2^-16 of a reference that is at most 8 times the
+// largest (columns 0..3 take the high bytes, 4..7 the low bytes of the same heads).  Sums of products are exact; they are
+// brought into fp32 when a reference changes and at the end.  Five to eight heads are two such sets over the same codes,
+// larger groups are cut into subsets of eight.
+// The order of the elements inside a contraction is free: a lane takes 16 contiguous bytes of a key row with the query
+// laid out to match, and the keys of a value operand are the ones whose weights the lane gets out of one 8x8 transpose.
 // Warps walk their keys 32 at a time with the next 32 keys in flight in registers (4.3 KB per warp).
 // HBM-bound: hs + 8 bytes per (key, key head), each read once.
 #include <algorithm>
@@ -32,25 +33,24 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_u8u8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// codes J and J + 4 of a word as the bf16 pair (1 + n/16)
-template <int J> __device__ __forceinline__ uint32_t expand(uint32_t x) {
-  const uint32_t y = J == 0 ? x << 3 : x >> (J == 0 ? 0 : 4 * J - 3);
-  return (y & 0x00780078u) | 0x3f803f80u;
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
+// even and odd codes of a word, a byte each
+__device__ __forceinline__ uint32_t even(uint32_t x) { return x & 0x0f0f0f0fu; }
+__device__ __forceinline__ uint32_t odd(uint32_t x) { return (x >> 4) & 0x0f0f0f0fu; }
 
 template <int W> struct Words;
 template <> struct Words<1> { using V = uint32_t; };
@@ -73,14 +73,14 @@ template <int HS> struct Tile {
   bool on[2];                         // the half exists (its page is in the pool and it begins before the end)
 };
 
-// WIDE: five to eight heads per subset.
-template <int HS, bool WIDE>
-__global__ void __launch_bounds__(MW * 32, 3) kv4_decode_mma_kernel(Kv4DecodeArgs a, int page_shift) {
+// NS: sets of four heads.  P32: pages of a multiple of 32 rows, so that a tile lies in one page.
+template <int HS, int NS, bool P32>
+__global__ void __launch_bounds__(MW * 32, NS == 1 ? 3 : 2) kv4_decode_mma_kernel(Kv4DecodeArgs a, int page_shift) {
   using T = Tile<HS>;
-  constexpr int KW = T::KW, VW = T::VW, MT = HS / 16;
+  constexpr int KW = T::KW, VW = T::VW, MT = HS / 16, RW = HS / 8;  // RW: words of a row
   extern __shared__ int32_t pre[];
   __shared__ int32_t warp_sums[MW];
-  __shared__ float s_o[MW][8][HS + 4], s_m[MW][8], s_l[MW][8];
+  __shared__ float s_o[MW][8 * NS][HS + 4], s_m[MW][4 * NS], s_l[MW][4 * NS], s_c[MW][4 * NS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   pdl_launch_dependents();
   pdl_wait();  // everything below comes from the kernels before
@@ -93,10 +93,15 @@ __global__ void __launch_bounds__(MW * 32, 3) kv4_decode_mma_kernel(Kv4DecodeArg
   const int ctas = (int)(units < (long long)gridDim.x ? units : (long long)gridDim.x);
   if ((int)blockIdx.x >= ctas) return;
   const long long r0 = range_start(units, ctas, blockIdx.x), r1 = range_start(units, ctas, blockIdx.x + 1);
-  const uint32_t* codes = reinterpret_cast<const uint32_t*>(p.codes);
   const size_t half = kv4_half(p);
+  // this lane's part of a row block: 16 bytes of key row g, the value rows 2t.., the parameters of row g
+  const uint32_t* kbase = reinterpret_cast<const uint32_t*>(p.codes) + g * RW + t * KW;
+  const uint32_t* vbase = reinterpret_cast<const uint32_t*>(p.codes) + half * RW + 2 * t * RW + g * VW;
+  const uint32_t* kprm = p.params + g;
+  const uint32_t* vprm = p.params + half + g;
   const int group = a.n_heads / p.n_kv_heads;
   const float sl2 = a.scale * 1.4426950408889634f;
+  const uint32_t part_sel = g < 4 ? 0x7531u : 0x6420u;  // high bytes, low bytes
   int b = 0;
   for (long long x = r0; x < r1;) {
     while ((long long)pre[b + 1] * nseg <= x) ++b;
@@ -112,19 +117,25 @@ __global__ void __launch_bounds__(MW * 32, 3) kv4_decode_mma_kernel(Kv4DecodeArg
     const int c0 = (int)(x - s0) * kUnit, c1 = min(len, (int)(x1 - s0) * kUnit);
     const int32_t* table = p.table + (size_t)b * p.max_pages;
 
+    struct Place { int page[2], row[2]; };
     auto place = [&](int u, int* page, int* row) {  // u: first key of a 16-key half
       const int slot = page_shift >= 0 ? u >> page_shift : u / p.page_size;
       *row = u - slot * p.page_size;
-      *page = u < c1 ? *(table + slot) : -1;
+      *page = u < c1 ? table[slot] : -1;
     };
-    struct Place { int page[2], row[2]; };
     auto places = [&](int u) {
       Place q;
       place(u, &q.page[0], &q.row[0]);
-      place(u + 16, &q.page[1], &q.row[1]);
+      if (P32) {
+        q.page[1] = q.page[0];
+        q.row[1] = q.row[0] + 16;
+      } else {
+        place(u + 16, &q.page[1], &q.row[1]);
+      }
       return q;
     };
     auto load = [&](T& w, const Place& q, int u) {
+      size_t at = 0;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         w.on[s] = u + 16 * s < c1;
@@ -132,132 +143,211 @@ __global__ void __launch_bounds__(MW * 32, 3) kv4_decode_mma_kernel(Kv4DecodeArg
           w.on[s] = false;
           if (lane == 0) atomicOr(a.status, ST_BAD_PAGE);
         }
+        if (s == 0 || !P32) at = ((size_t)q.page[s] * p.n_kv_heads + hk) * p.page_size + q.row[s];
+        const int more = P32 ? 16 * s : 0;  // rows behind `at`
         if (w.on[s]) {
-          const size_t row = ((size_t)q.page[s] * p.n_kv_heads + hk) * p.page_size + q.row[s];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            load_words<KW>(codes + (row + g + 8 * r) * (HS / 8) + t * KW, w.k[s][r]);
-            w.kp[s][r] = *(p.params + row + g + 8 * r);
-            w.vp[s][r] = *(p.params + half + row + g + 8 * r);
+            load_words<KW>(kbase + at * RW + (more + 8 * r) * RW, w.k[s][r]);
+            w.kp[s][r] = kprm[at + more + 8 * r];
+            w.vp[s][r] = vprm[at + more + 8 * r];
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) load_words<VW>(vbase + at * RW + (more + (j & 1) + 8 * (j >> 1)) * RW, w.v[s][j]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            w.kp[s][r] = w.vp[s][r] = 0u;
+#pragma unroll
+            for (int i = 0; i < KW; ++i) w.k[s][r][i] = 0u;
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            load_words<VW>(codes + (half + row + 2 * t + (j & 1) + 8 * (j >> 1)) * (HS / 8) + g * VW, w.v[s][j]);
+#pragma unroll
+            for (int i = 0; i < VW; ++i) w.v[s][j][i] = 0u;
         }
       }
     };
 
-    // query fragments: column g; the elements a lane's words hold, in their order
-    uint32_t qf[2 * KW][2];
-    float qs = 0.f;
-    {
-      const int col = WIDE ? g : (g & 3);
+    // query fragments: column g; the elements of a lane's words, even codes and odd codes, high bytes and low bytes
+    uint32_t qh[NS][KW][2], ql[NS][KW][2];
+    float q0[NS], q1[NS], f0[NS], f1[NS];  // of columns 2t, 2t + 1: sum of q, and the step of its elements
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      const int col = 4 * n + (g & 3);
       const bool on = col < n_cols;
       const bf16* q = (const bf16*)a.q + (size_t)b * a.ldq + (head0 + (on ? col : 0)) * HS + t * (HS / 4);
+      float e[8 * KW], top = 0.f, qs = 0.f;
 #pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        float e[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          e[i] = on ? to_f32(q[8 * w + i]) : 0.f;
-          qs += e[i];
-        }
-        qf[2 * w][0] = pack2(e[0], e[4]);
-        qf[2 * w][1] = pack2(e[1], e[5]);
-        qf[2 * w + 1][0] = pack2(e[2], e[6]);
-        qf[2 * w + 1][1] = pack2(e[3], e[7]);
+      for (int i = 0; i < 8 * KW; ++i) {
+        e[i] = on ? to_f32(q[i]) : 0.f;
+        qs += e[i];
+        top = fmaxf(top, fabsf(e[i]));
       }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      qs += __shfl_xor_sync(0xffffffffu, qs, 1);
+      qs += __shfl_xor_sync(0xffffffffu, qs, 2);
+      const float up = top > 0.f ? fminf(32512.f / top, 1e30f) : 1.f;
+#pragma unroll
+      for (int i = 0; i < KW; ++i) {
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          uint32_t h = 0u, l = 0u;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int v = __float2int_rn(e[8 * i + 2 * j + o] * up);
+            const int vh = (v + 128) >> 8;
+            h |= ((uint32_t)vh & 0xffu) << (8 * j);
+            l |= ((uint32_t)(v - 256 * vh) & 0xffu) << (8 * j);
+          }
+          qh[n][i][o] = h;
+          ql[n][i][o] = l;
+        }
+      }
+      qs *= sl2;
+      const float fs = sl2 / up;
+      q0[n] = __shfl_sync(0xffffffffu, qs, 8 * (t & 1));
+      q1[n] = __shfl_sync(0xffffffffu, qs, 8 * (t & 1) + 4);
+      f0[n] = __shfl_sync(0xffffffffu, fs, 8 * (t & 1));
+      f1[n] = __shfl_sync(0xffffffffu, fs, 8 * (t & 1) + 4);
     }
-    qs += __shfl_xor_sync(0xffffffffu, qs, 1);
-    qs += __shfl_xor_sync(0xffffffffu, qs, 2);
-    const float q0 = __shfl_sync(0xffffffffu, qs, 8 * t), q1 = __shfl_sync(0xffffffffu, qs, 8 * t + 4);  // columns 2t, 2t + 1
 
-    float acc[MT][4];
+    int acc[NS][MT][4];
+    float m0[NS], m1[NS];                          // references of columns 2t, 2t + 1 (uniform over g): weights are <= 1
+    float l0[NS], l1[NS], c0s[NS], c1s[NS];        // this lane's share of sum p and of sum p m
+    float sc = __uint_as_float(254u << 23);        // power of two that keeps the value scales at most 1 (uniform)
+    bool kept = false;                             // s_o holds sums (uniform)
+    int tiles = 0;                                 // a sum of 255 * 15 a key stays below 2^31 for 2^18 keys and more
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int n = 0; n < NS; ++n) {
+      m0[n] = m1[n] = -INFINITY;
+      l0[n] = l1[n] = c0s[n] = c1s[n] = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY;            // reference maxima of columns 2t, 2t + 1 (uniform over g)
-    float l0 = 0.f, l1 = 0.f, k0s = 0.f, k1s = 0.f;  // this lane's share of sum p and of sum p (m - 16 s)
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[n][i][j] = 0;
+    }
+    // Adds the integer sums of one set to its fp32 sums in shared memory (columns 8n .. 8n + 7), which are then scaled by
+    // e0, e1, and clears them.
+    auto keep = [&](int n, float e0, float e1) {
+      const float step = (t < 2 ? 256.f : 1.f) / 65535.f / sc;
+#pragma unroll
+      for (int i = 0; i < VW; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {  // elements 2j, 2j + 1 of the word, columns 2t, 2t + 1
+            float& at = s_o[warp][8 * n + 2 * t + (c & 1)][g * (HS / 8) + 8 * i + 2 * j + (c >> 1)];
+            const float was = kept ? at : 0.f;
+            at = fmaf((float)acc[n][4 * i + j][c], step, was) * ((c & 1) ? e1 : e0);
+            acc[n][4 * i + j][c] = 0;
+          }
+        }
+      }
+    };
 
     auto compute = [&](const T& w, int u) {
-      float sc[2][4];
-      float bm0 = -INFINITY, bm1 = -INFINITY;
+      float xs[NS][2][4], b0[NS], b1[NS], smax = 0.f;
+      bool raise = (++tiles & 8191) == 0;
+#pragma unroll
+      for (int n = 0; n < NS; ++n) b0[n] = b1[n] = -INFINITY;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
-        if (w.on[s]) {
+        int dh[NS][4], dl[NS][4];
 #pragma unroll
-          for (int i = 0; i < KW; ++i) {
-            const uint32_t ka = w.k[s][0][i], kb = w.k[s][1][i];
-            mma16816(d, expand<0>(ka), expand<0>(kb), expand<1>(ka), expand<1>(kb), qf[2 * i][0], qf[2 * i][1]);
-            mma16816(d, expand<2>(ka), expand<2>(kb), expand<3>(ka), expand<3>(kb), qf[2 * i + 1][0], qf[2 * i + 1][1]);
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) dh[n][j] = dl[n][j] = 0;
+#pragma unroll
+        for (int i = 0; i < KW; ++i) {
+          const uint32_t ka = w.k[s][0][i], kb = w.k[s][1][i];
+          const uint32_t ea = even(ka), eb = even(kb), oa = odd(ka), ob = odd(kb);
+#pragma unroll
+          for (int n = 0; n < NS; ++n) {
+            mma_u8s8(dh[n], ea, eb, oa, ob, qh[n][i][0], qh[n][i][1]);
+            mma_u8s8(dl[n], ea, eb, oa, ob, ql[n][i][0], ql[n][i][1]);
           }
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const bool in = w.on[s] && u + 16 * s + 8 * r + g < c1;
-          const float s16 = 16.f * __uint_as_float(w.kp[s][r] << 16);
-          const float ka = s16 * sl2, kc = (__uint_as_float(w.kp[s][r] & 0xffff0000u) - s16) * sl2;
-          sc[s][2 * r] = in ? fmaf(ka, d[2 * r], kc * q0) : -INFINITY;
-          sc[s][2 * r + 1] = in ? fmaf(ka, d[2 * r + 1], kc * q1) : -INFINITY;
-          bm0 = fmaxf(bm0, sc[s][2 * r]);
-          bm1 = fmaxf(bm1, sc[s][2 * r + 1]);
+          const float ks = __uint_as_float(w.kp[s][r] << 16), km = __uint_as_float(w.kp[s][r] & 0xffff0000u);
+#pragma unroll
+          for (int n = 0; n < NS; ++n) {
+            const float d0 = (float)(256 * dh[n][2 * r] + dl[n][2 * r]), d1 = (float)(256 * dh[n][2 * r + 1] + dl[n][2 * r + 1]);
+            xs[n][s][2 * r] = in ? fmaf(ks, d0 * f0[n], km * q0[n]) : -INFINITY;
+            xs[n][s][2 * r + 1] = in ? fmaf(ks, d1 * f1[n], km * q1[n]) : -INFINITY;
+            b0[n] = fmaxf(b0[n], xs[n][s][2 * r]);
+            b1[n] = fmaxf(b1[n], xs[n][s][2 * r + 1]);
+          }
+          smax = fmaxf(smax, in ? fabsf(__uint_as_float(w.vp[s][r] << 16)) : 0.f);
         }
       }
-      if (__any_sync(0xffffffffu, bm0 > m0 + 8.f || bm1 > m1 + 8.f)) {
-        // raise the references of the columns to the tile's maxima; until then weights stay below 2^8
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          bm0 = fmaxf(bm0, __shfl_xor_sync(0xffffffffu, bm0, o));
-          bm1 = fmaxf(bm1, __shfl_xor_sync(0xffffffffu, bm1, o));
-        }
-        const float n0 = fmaxf(m0, bm0), n1 = fmaxf(m1, bm1);
-        const float f0 = n0 == m0 ? 1.f : ex2(m0 - n0), f1 = n1 == m1 ? 1.f : ex2(m1 - n1);
-        m0 = n0; m1 = n1;
-        l0 *= f0; l1 *= f1; k0s *= f0; k1s *= f1;
+      for (int n = 0; n < NS; ++n) raise = raise || b0[n] > m0[n] || b1[n] > m1[n];
+      if (__any_sync(0xffffffffu, raise || smax * sc > 1.f)) {
+        // Set the references 2 above the largest score, so that weights begin at 1/4 and may grow to 1, and the scales'
+        // factor so that they lie between 1/2 and 1.
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          acc[i][0] *= f0; acc[i][1] *= f1; acc[i][2] *= f0; acc[i][3] *= f1;
+        for (int o = 1; o < 32; o <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, o));
+        const bool rescale = smax * sc > 1.f;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            b0[n] = fmaxf(b0[n], __shfl_xor_sync(0xffffffffu, b0[n], o));
+            b1[n] = fmaxf(b1[n], __shfl_xor_sync(0xffffffffu, b1[n], o));
+          }
+          const float n0 = b0[n] > m0[n] ? b0[n] + 2.f : m0[n], n1 = b1[n] > m1[n] ? b1[n] + 2.f : m1[n];
+          const float e0 = n0 == m0[n] ? 1.f : ex2(m0[n] - n0), e1 = n1 == m1[n] ? 1.f : ex2(m1[n] - n1);
+          m0[n] = n0; m1[n] = n1;
+          l0[n] *= e0; l1[n] *= e1; c0s[n] *= e0; c1s[n] *= e1;
+          keep(n, e0, e1);
         }
+        kept = true;
+        if (rescale) sc = __uint_as_float((uint32_t)max(1, 253 - (int)(__float_as_uint(smax) >> 23)) << 23);
       }
+      uint32_t wb[NS][2];
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        if (!w.on[s]) continue;
-        uint32_t hi[2], lo[2];
+        uint32_t tr[NS][2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const bool in = u + 16 * s + 8 * r + g < c1;
-          const float p0 = in ? ex2(sc[s][2 * r] - m0) : 0.f, p1 = in ? ex2(sc[s][2 * r + 1] - m1) : 0.f;
-          const float s16 = in ? 16.f * __uint_as_float(w.vp[s][r] << 16) : 0.f;
-          const float mc = in ? __uint_as_float(w.vp[s][r] & 0xffff0000u) - s16 : 0.f;
-          l0 += p0; l1 += p1;
-          k0s = fmaf(p0, mc, k0s); k1s = fmaf(p1, mc, k1s);
-          const float w0 = p0 * s16, w1 = p1 * s16;
-          const uint32_t h = pack2(w0, w1);
-          const uint32_t rest = pack2(w0 - __uint_as_float(h << 16), w1 - __uint_as_float(h & 0xffff0000u));
-          if (WIDE) {
-            hi[r] = transpose8x8(h);
-            lo[r] = transpose8x8(rest);
-          } else {
-            hi[r] = transpose8x8(t < 2 ? h : rest);
+          const bool in = w.on[s] && u + 16 * s + 8 * r + g < c1;
+          const float vs = in ? __uint_as_float(w.vp[s][r] << 16) * sc * 65535.f : 0.f;
+          const float vm = in ? __uint_as_float(w.vp[s][r] & 0xffff0000u) : 0.f;
+#pragma unroll
+          for (int n = 0; n < NS; ++n) {
+            const float p0 = in ? ex2(xs[n][s][2 * r] - m0[n]) : 0.f, p1 = in ? ex2(xs[n][s][2 * r + 1] - m1[n]) : 0.f;
+            l0[n] += p0; l1[n] += p1;
+            c0s[n] = fmaf(p0, vm, c0s[n]); c1s[n] = fmaf(p1, vm, c1s[n]);
+            // rounded to integers in the low 16 bits of 2^23 + w, column 2t in the low half, column 2t + 1 in the high one
+            const uint32_t i0 = __float_as_uint(fmaf(p0, vs, 8388608.f)), i1 = __float_as_uint(fmaf(p1, vs, 8388608.f));
+            tr[n][r] = transpose8x8(__byte_perm(i0, i1, 0x5410u));
           }
         }
+        // now the weights of column g for keys 2t, 2t + 1 of each eight: the byte this column takes
 #pragma unroll
-        for (int i = 0; i < VW; ++i) {
+        for (int n = 0; n < NS; ++n) wb[n][s] = __byte_perm(tr[n][0], tr[n][1], part_sel);
+      }
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {  // codes 0..3, then 4..7 of the words
-            const uint32_t sel = y ? 0x7632u : 0x5410u;
-            const uint32_t a01 = __byte_perm(w.v[s][0][i], w.v[s][1][i], sel), a23 = __byte_perm(w.v[s][2][i], w.v[s][3][i], sel);
-            const uint32_t e0 = expand<0>(a01), e1 = expand<1>(a01), e2 = expand<2>(a01), e3 = expand<3>(a01);
-            const uint32_t f0 = expand<0>(a23), f1 = expand<1>(a23), f2 = expand<2>(a23), f3 = expand<3>(a23);
-            mma16816(acc[4 * i + 2 * y], e0, e1, f0, f1, hi[0], hi[1]);
-            mma16816(acc[4 * i + 2 * y + 1], e2, e3, f2, f3, hi[0], hi[1]);
-            if (WIDE) {
-              mma16816(acc[4 * i + 2 * y], e0, e1, f0, f1, lo[0], lo[1]);
-              mma16816(acc[4 * i + 2 * y + 1], e2, e3, f2, f3, lo[0], lo[1]);
-            }
-          }
+      for (int i = 0; i < VW; ++i) {
+        uint32_t y[2][4];  // [half][j]: codes 2j (low nibbles) and 2j + 1 of the lane's four keys, a byte per key
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const uint32_t z0 = __byte_perm(w.v[s][0][i], w.v[s][1][i], 0x5140u), z1 = __byte_perm(w.v[s][2][i], w.v[s][3][i], 0x5140u);
+          const uint32_t z2 = __byte_perm(w.v[s][0][i], w.v[s][1][i], 0x7362u), z3 = __byte_perm(w.v[s][2][i], w.v[s][3][i], 0x7362u);
+          y[s][0] = __byte_perm(z0, z1, 0x5410u);
+          y[s][1] = __byte_perm(z0, z1, 0x7632u);
+          y[s][2] = __byte_perm(z2, z3, 0x5410u);
+          y[s][3] = __byte_perm(z2, z3, 0x7632u);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t a0 = even(y[0][j]), a1 = odd(y[0][j]), a2 = even(y[1][j]), a3 = odd(y[1][j]);
+#pragma unroll
+          for (int n = 0; n < NS; ++n) mma_u8u8(acc[n][4 * i + j], a0, a1, a2, a3, wb[n][0], wb[n][1]);
         }
       }
     };
@@ -281,35 +371,21 @@ __global__ void __launch_bounds__(MW * 32, 3) kv4_decode_mma_kernel(Kv4DecodeArg
         if (u >= c1) break;
       }
     }
-    // the lanes of a column
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) {
-      l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, o);
-      k0s += __shfl_xor_sync(0xffffffffu, k0s, o);
-      k1s += __shfl_xor_sync(0xffffffffu, k1s, o);
-    }
-    if (!WIDE) {  // the rest of the weights stands four columns to the right
+    for (int n = 0; n < NS; ++n) {
+      // the lanes of a column
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += __shfl_xor_sync(0xffffffffu, acc[i][j], 2);
-    }
-    if (WIDE || t < 2) {
-#pragma unroll
-      for (int i = 0; i < VW; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {  // elements 2j, 2j + 1 of the word
-          const int d = g * (HS / 8) + 8 * i + 2 * j;
-          s_o[warp][2 * t][d] = acc[4 * i + j][0] + k0s;
-          s_o[warp][2 * t + 1][d] = acc[4 * i + j][1] + k1s;
-          s_o[warp][2 * t][d + 1] = acc[4 * i + j][2] + k0s;
-          s_o[warp][2 * t + 1][d + 1] = acc[4 * i + j][3] + k1s;
-        }
+      for (int o = 4; o < 32; o <<= 1) {
+        l0[n] += __shfl_xor_sync(0xffffffffu, l0[n], o);
+        l1[n] += __shfl_xor_sync(0xffffffffu, l1[n], o);
+        c0s[n] += __shfl_xor_sync(0xffffffffu, c0s[n], o);
+        c1s[n] += __shfl_xor_sync(0xffffffffu, c1s[n], o);
       }
-      if (g == 0) {
-        s_m[warp][2 * t] = m0; s_m[warp][2 * t + 1] = m1;
-        s_l[warp][2 * t] = l0; s_l[warp][2 * t + 1] = l1;
+      keep(n, 1.f, 1.f);
+      if (t < 2 && g == 0) {
+        s_m[warp][4 * n + 2 * t] = m0[n]; s_m[warp][4 * n + 2 * t + 1] = m1[n];
+        s_l[warp][4 * n + 2 * t] = l0[n]; s_l[warp][4 * n + 2 * t + 1] = l1[n];
+        s_c[warp][4 * n + 2 * t] = c0s[n]; s_c[warp][4 * n + 2 * t + 1] = c1s[n];
       }
     }
     __syncthreads();
@@ -324,7 +400,8 @@ __global__ void __launch_bounds__(MW * 32, 3) kv4_decode_mma_kernel(Kv4DecodeArg
 #pragma unroll
       for (int w = 0; w < MW; ++w) {
         const float f = s_m[w][c] == gm ? 1.f : ex2(s_m[w][c] - gm);
-        v = fmaf(s_o[w][c][d], f, v);
+        const int at = 8 * (c >> 2) + (c & 3);  // high bytes; low bytes four columns further
+        v = fmaf(s_o[w][at][d] + s_o[w][at + 4][d] + s_c[w][c], f, v);
         gl = fmaf(s_l[w][c], f, gl);
       }
       if (whole) {
@@ -346,10 +423,12 @@ template <int HS> int32_t launch_hs(const Kv4DecodeArgs& a, int grid, cudaStream
   const int ps = a.pool.page_size;
   const int shift = (ps & (ps - 1)) == 0 ? __builtin_ctz((unsigned)ps) : -1;
   const size_t smem = (size_t)(a.batch + 1) * sizeof(int32_t);
+  auto go = [&](auto kern) { return launch_pdl(kern, dim3(grid), dim3(MW * 32), smem, stream, a, shift); };
+  const bool p32 = ps % 32 == 0;
   if (a.cols > 4) {
-    B200_CUDA_OK(launch_pdl(kv4_decode_mma_kernel<HS, true>, dim3(grid), dim3(MW * 32), smem, stream, a, shift));
+    B200_CUDA_OK(p32 ? go(kv4_decode_mma_kernel<HS, 2, true>) : go(kv4_decode_mma_kernel<HS, 2, false>));
   } else {
-    B200_CUDA_OK(launch_pdl(kv4_decode_mma_kernel<HS, false>, dim3(grid), dim3(MW * 32), smem, stream, a, shift));
+    B200_CUDA_OK(p32 ? go(kv4_decode_mma_kernel<HS, 1, true>) : go(kv4_decode_mma_kernel<HS, 1, false>));
   }
   B200_LAUNCH_OK("kv4_decode_mma_kernel");
   return B200_OK;
@@ -361,7 +440,7 @@ bool kv4_decode_mma_supports(const Kv4DecodeArgs& a) {
   return a.dtype == B200_BF16 && (a.pool.head_size == 64 || a.pool.head_size == 128) && a.pool.page_size % 16 == 0;
 }
 
-int kv4_decode_mma_grid() { return 3 * sm_count(); }
+int kv4_decode_mma_grid(int cols) { return (cols > 4 ? 2 : 3) * sm_count(); }
 
 int32_t launch_kv4_decode_mma(const Kv4DecodeArgs& a, int grid, cudaStream_t stream) {
   if (a.pool.head_size == 64) return launch_hs<64>(a, grid, stream);

@@ -139,13 +139,16 @@ def cache(lens, hk, page, hs, seed=0):
 
 
 def decode_reference(q, codes, params, table, lens, heads):
-    """fp64 output and the bound of a kernel with fp32 scores and sums whose weights keep 16 bits in the bf16 form:
-    |do| <= U|o| + (2 ds + dw + (n + 16) U32) * sum p (|lo| + 31 scale)   (codes enter as 16 + code)"""
+    """fp64 output and the bound of a kernel.  Scores and sums are fp32; in the bf16 form query elements stand to half a
+    step of 1/32512 of the head's largest and the weights scale * p of the codes to half a step of 1/65535 of a reference
+    that is at most 8 times the largest weight (4 for p, 2 for the scale).
+      |do| <= U|o| + (2 ds + (n + 16) U32) sum p (|lo| + 15 scale) + n 2^-14 max(p) max(scale) 15,
+      ds <= (hs + 16) U32 sum|q| (|lo| + 15 scale) / sqrt(hs) + 2^-16 max|q| hs 15 scale / sqrt(hs)"""
     hk, page, hs = codes.shape[2], codes.shape[3], codes.shape[4] * 2
     group = heads // hk
     out = torch.zeros(len(lens), heads, hs, dtype=torch.float64, device=DEV)
     bound = torch.zeros_like(out)
-    dw = 2.0 ** -16 if q.dtype == torch.bfloat16 else 0.0
+    small = q.dtype == torch.bfloat16
     for b, n in enumerate(lens):
         if n == 0:
             continue
@@ -158,14 +161,20 @@ def decode_reference(q, codes, params, table, lens, heads):
                 prm = params[half, pg, j, r].double()
                 x = torch.stack((c & 15, c >> 4), -1).view(n, hs).double()
                 rows.append(x * prm[:, :1] + prm[:, 1:])
-                mags.append(31 * prm[:, :1] + prm[:, 1:].abs())
+                mags.append(15 * prm[:, :1] + prm[:, 1:].abs())
+            ksc, vsc = params[0, pg, j, r, :1].double(), params[1, pg, j, r, :1].double()
             hd = slice(j * group, (j + 1) * group)
             Q = q[b].view(heads, hs)[hd].double()
             s = Q @ rows[0].T / math.sqrt(hs)
             p = torch.softmax(s, -1)
-            ds = ((hs + 16) * U32 * Q.abs().sum(-1, keepdim=True) * mags[0].T / math.sqrt(hs)).max(-1, keepdim=True).values
+            ds = (hs + 16) * U32 * Q.abs().sum(-1, keepdim=True) * mags[0].T / math.sqrt(hs)
+            if small:
+                ds = ds + 2.0 ** -16 * Q.abs().amax(-1, keepdim=True) * hs * 15 * ksc.T / math.sqrt(hs)
+            ds = ds.max(-1, keepdim=True).values
             out[b, hd] = p @ rows[1]
-            bound[b, hd] = U[q.dtype] * out[b, hd].abs() + ((2 * ds + dw + (n + 16) * U32) * p) @ mags[1].expand(n, hs)
+            bound[b, hd] = U[q.dtype] * out[b, hd].abs() + ((2 * ds + (n + 16) * U32) * p) @ mags[1].expand(n, hs)
+            if small:
+                bound[b, hd] += n * 2.0 ** -14 * p.amax(-1, keepdim=True) * vsc.max() * 15
     return out.view(len(lens), -1), bound.view(len(lens), -1) + 1e-30
 
 
