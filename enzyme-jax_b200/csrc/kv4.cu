@@ -299,20 +299,26 @@ __global__ void __launch_bounds__(SW * 32) kv4_decode_simt_kernel(Kv4DecodeArgs 
 }
 
 // Joins the partial blocks of the segments that several CTAs shared, and writes zeros for sequences without cached rows.
+// One CTA per (segment, query head): its warps share the partials out (a single long sequence has one per SM and more).
+constexpr int JW = 8;
+
 template <typename T, int HS>
-__global__ void __launch_bounds__(128) kv4_join_kernel(Kv4DecodeArgs a, int grid) {
+__global__ void __launch_bounds__(JW * 32) kv4_join_kernel(Kv4DecodeArgs a, int grid) {
+  constexpr int N = (HS + 31) / 32;
+  __shared__ float s_acc[JW][HS], s_l[JW];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nseg = a.pool.n_kv_heads * a.subs;
-  const int b = blockIdx.x / nseg, seg = blockIdx.x % nseg;
+  const int c = blockIdx.x % a.cols, seg = blockIdx.x / a.cols % nseg, b = blockIdx.x / a.cols / nseg;
+  const int group = a.n_heads / a.pool.n_kv_heads;
+  const int first = (seg % a.subs) * a.cols;
+  if (c >= group - first) return;  // the last subset of a head may be smaller
   pdl_launch_dependents();
   pdl_wait();
   const int p0 = a.prefix[b], nb = a.prefix[b + 1] - p0;
   const long long units = (long long)a.prefix[a.batch] * nseg;
-  const int group = a.n_heads / a.pool.n_kv_heads;
-  const int first = (seg % a.subs) * a.cols, n = min(a.cols, group - first);
-  const int head0 = (seg / a.subs) * group + first;
-  T* o = (T*)a.o + (size_t)b * a.ldo + head0 * HS;
+  T* o = (T*)a.o + (size_t)b * a.ldo + ((seg / a.subs) * group + first + c) * HS;
   if (nb == 0) {
-    for (int e = threadIdx.x; e < n * HS; e += blockDim.x) o[e] = from_f32<T>(0.f);
+    for (int e = threadIdx.x; e < HS; e += blockDim.x) o[e] = from_f32<T>(0.f);
     return;
   }
   const int ctas = (int)(units < (long long)grid ? units : (long long)grid);
@@ -320,19 +326,37 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(Kv4DecodeArgs a, int grid
   const int ca = range_owner(units, ctas, s0), cb = range_owner(units, ctas, s1 - 1);
   if (ca == cb) return;  // finished by its CTA
   const size_t slot = (size_t)a.cols * (HS + 2);
-  const int sa = range_start(units, ctas, ca) == s0 ? 0 : 1;
-  for (int e = threadIdx.x; e < n * HS; e += blockDim.x) {
-    const int c = e / HS, d = e % HS;
-    float m = -INFINITY, l = 0.f, acc = 0.f;
-    for (int i = ca; i <= cb; ++i) {
-      const float* part = a.partials + (2 * (size_t)i + (i == ca ? sa : 0)) * slot + (size_t)c * (HS + 2);
-      const float mo = part[HS], nm = fmaxf(m, mo);
-      const float f0 = m == nm ? 1.f : exp_by_build(m - nm), f1 = mo == nm ? 1.f : exp_by_build(mo - nm);
-      l = l * f0 + part[HS + 1] * f1;
-      acc = acc * f0 + part[d] * f1;
-      m = nm;
+  // only the first of the CTAs can have had another segment before this one
+  const size_t first_slot = range_start(units, ctas, ca) == s0 ? 0 : 1;
+  auto part = [&](int i) { return a.partials + (2 * (size_t)i + (i == ca ? first_slot : 0)) * slot + (size_t)c * (HS + 2); };
+  float m = -INFINITY;
+  for (int i = ca + lane; i <= cb; i += 32) m = fmaxf(m, part(i)[HS]);
+  m = warp_max(m);
+  float l = 0.f, acc[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) acc[j] = 0.f;
+#pragma unroll 4
+  for (int i = ca + warp; i <= cb; i += JW) {
+    const float* q = part(i);
+    const float f = q[HS] == m ? 1.f : exp_by_build(q[HS] - m);
+    l = fmaf(q[HS + 1], f, l);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (HS % 32 == 0 || lane + 32 * j < HS) acc[j] = fmaf(q[lane + 32 * j], f, acc[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (HS % 32 == 0 || lane + 32 * j < HS) s_acc[warp][lane + 32 * j] = acc[j];
+  if (lane == 0) s_l[warp] = l;
+  __syncthreads();
+  for (int e = threadIdx.x; e < HS; e += blockDim.x) {
+    float v = 0.f, gl = 0.f;
+#pragma unroll
+    for (int w = 0; w < JW; ++w) {
+      v += s_acc[w][e];
+      gl += s_l[w];
     }
-    o[e] = from_f32<T>(l == 0.f ? 0.f : acc / l);
+    o[e] = from_f32<T>(gl == 0.f ? 0.f : v / gl);
   }
 }
 
@@ -449,7 +473,7 @@ int32_t b200_attention_decode_kv4_scratch_bytes(int32_t batch, int32_t n_heads, 
   if (batch < 0 || n_heads <= 0 || n_kv_heads <= 0 || head_size <= 0 || n_heads % n_kv_heads)
     return fail(B200_ERR_BAD_SHAPE, "kv4 decode: batch=%d heads=%d kv_heads=%d head_size=%d", batch, n_heads, n_kv_heads, head_size);
   const int cols = std::min(8, n_heads / n_kv_heads);
-  const size_t floats = std::max(partial_floats(decode_simt_grid(), 1, head_size), partial_floats(kv4_decode_mma_grid(cols), cols, head_size));
+  const size_t floats = std::max(partial_floats(decode_simt_grid(), 1, head_size), partial_floats(kv4_decode_mma_grid(head_size, cols), cols, head_size));
   *bytes = align_up(((size_t)std::min(batch, kMaxSlice) + 1) * 4, 256) + floats * 4;
   return B200_OK;
 }
@@ -499,7 +523,7 @@ int32_t b200_attention_decode_kv4(const void* q, const void* codes, const void* 
     a.o = (char*)o + (size_t)b0 * ldo * es;
     a.ctx = ctx_lens + b0;
     a.pool.table = page_table + (size_t)b0 * max_pages;
-    const int grid = (int)std::max(1LL, std::min<long long>(mma ? kv4_decode_mma_grid(a.cols) : decode_simt_grid(), units_per_seq * a.batch));
+    const int grid = (int)std::max(1LL, std::min<long long>(mma ? kv4_decode_mma_grid(head_size, a.cols) : decode_simt_grid(), units_per_seq * a.batch));
     B200_TRY(by_type("kv4 decode", dtype, head_size, [&](auto t, auto hs) -> int32_t {
       using T = decltype(t);
       constexpr int HS = decltype(hs)::value;
@@ -509,7 +533,7 @@ int32_t b200_attention_decode_kv4(const void* q, const void* codes, const void* 
         B200_CUDA_OK(launch_pdl(kv4_decode_simt_kernel<T, HS>, dim3(grid), dim3(SW * 32), (a.batch + 1) * sizeof(int32_t), s, a));
         B200_LAUNCH_OK("kv4_decode_simt_kernel");
       }
-      B200_CUDA_OK(launch_pdl(kv4_join_kernel<T, HS>, dim3(a.batch * n_kv_heads * a.subs), dim3(128), 0, s, a, grid));
+      B200_CUDA_OK(launch_pdl(kv4_join_kernel<T, HS>, dim3(a.batch * n_kv_heads * a.subs * a.cols), dim3(JW * 32), 0, s, a, grid));
       B200_LAUNCH_OK("kv4_join_kernel");
       return B200_OK;
     }));

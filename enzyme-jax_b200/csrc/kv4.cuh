@@ -84,7 +84,7 @@ template <int THREADS> __device__ __forceinline__ void unit_prefix(const Kv4Deco
 }
 
 bool kv4_decode_mma_supports(const Kv4DecodeArgs& a);
-int kv4_decode_mma_grid(int cols);  // resident CTAs
+int kv4_decode_mma_grid(int head_size, int cols);  // resident CTAs
 int32_t launch_kv4_decode_mma(const Kv4DecodeArgs& a, int grid, cudaStream_t stream);
 
 }  // namespace b200
