@@ -5,9 +5,13 @@
 //   code    = round-half-even((x - minimum) / scale) in 0..15.
 // With those directions of rounding every x lies between the values of code 0 and code 15, so the error is at most half
 // a scale.  A row that holds an infinity or NaN (or whose spread overflows) gets NaN parameters and reads back as NaN:
-// one bad value must not come back as a plausible one.  hs/8 lanes share a row: 8 elements and one 32-bit word of codes
-// each; the row's minimum and maximum are 4 shuffles.  HBM-bound (bytes of the inputs plus hs/2 + 4 per row and half).
+// one bad value must not come back as a plausible one.
+// A warp takes a packed row (or, when rows are few, a part of its heads): it finds the row's sequence and page once, then
+// hs/8 lanes share a (head, half), 8 elements and one 32-bit word of codes each.  A quotient is a product with the
+// reciprocal, rounded, and then checked against its exact remainder, which costs half of a division.
+// Bound: bytes of the inputs plus hs/2 + 4 per row and half at HBM speed; about 75 instructions per (head, half).
 #include "kv4.cuh"
+#include "attention_packed.cuh"
 
 #include <algorithm>
 #include <type_traits>
@@ -22,10 +26,7 @@ __device__ __forceinline__ float bf16_down(float x) {
   const uint32_t b = __float_as_uint(x), cut = b & 0xffff0000u;
   return __uint_as_float((b >> 31) && cut != b ? cut + 0x10000u : cut);
 }
-__device__ __forceinline__ float bf16_up_nonneg(float x) {
-  const uint32_t b = __float_as_uint(x), cut = b & 0xffff0000u;
-  return __uint_as_float(cut != b ? cut + 0x10000u : cut);
-}
+__device__ __forceinline__ float bf16_up_nonneg(float x) { return __uint_as_float((__float_as_uint(x) + 0xffffu) & 0xffff0000u); }
 
 struct Kv4RowsArgs {
   Kv4Pool pool;
@@ -35,121 +36,252 @@ struct Kv4RowsArgs {
   uint32_t* status = nullptr;
 };
 
-// Cache row (inside the key half) of packed row t for head hk; false when the row belongs to no sequence or the page
-// table has no valid page for it.
-__device__ __forceinline__ bool place_of(const Kv4RowsArgs& a, int t, int hk, size_t* row) {
-  // the sequence of row t: largest s with cu[s] <= t
-  int lo = -1, hi = a.n_seqs;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (*(a.cu + mid) <= t) lo = mid;
-    else hi = mid - 1;
-  }
-  if (lo < 0 || lo >= a.n_seqs) return false;
-  const long long pos = (long long)(t - *(a.cu + lo)) + (a.before ? *(a.before + lo) : 0);
-  const long long slot = pos / a.pool.page_size;
-  if (pos < 0 || slot >= a.pool.max_pages) {
-    atomicOr(a.status, ST_BAD_PAGE);
+// Page and row inside the page of packed row t, the same for all lanes of the warp; false when the row belongs to no
+// sequence or the page table has no valid page for it.
+__device__ __forceinline__ bool place_of(const Kv4RowsArgs& a, int t, int* page, int* in_page) {
+  const int s = seq_of_row_warp(a.cu, a.n_seqs, t);
+  if (s < 0 || s >= a.n_seqs) return false;
+  const long long pos = (long long)(t - a.cu[s]) + (a.before ? a.before[s] : 0);
+  if (pos < 0 || pos >= (long long)a.pool.max_pages * a.pool.page_size || pos > 0x7fffffffLL) {
+    if ((threadIdx.x & 31) == 0) atomicOr(a.status, ST_BAD_PAGE);
     return false;
   }
-  const int page = *(a.pool.table + (size_t)lo * a.pool.max_pages + slot);
-  if ((unsigned)page >= (unsigned)a.pool.n_pages) {
-    atomicOr(a.status, ST_BAD_PAGE);
+  const int slot = (int)pos / a.pool.page_size;
+  *in_page = (int)pos - slot * a.pool.page_size;
+  *page = a.pool.table[(size_t)s * a.pool.max_pages + slot];
+  if ((unsigned)*page >= (unsigned)a.pool.n_pages) {
+    if ((threadIdx.x & 31) == 0) atomicOr(a.status, ST_BAD_PAGE);
     return false;
   }
-  *row = ((size_t)page * a.pool.n_kv_heads + hk) * a.pool.page_size + (size_t)(pos - slot * a.pool.page_size);
   return true;
 }
 
 constexpr int AT = 256;  // threads of the append and read kernels
 
-// Threads: LPR lanes per (row, head, half); consecutive groups take consecutive heads of one row.
-template <typename T, int HS>
-__global__ void __launch_bounds__(AT) kv4_append_kernel(Kv4RowsArgs a, const T* __restrict__ k, const T* __restrict__ v,
-                                                        int ldk, int ldv, bool vec) {
-  constexpr int LPR = lanes_of(HS), GPB = AT / LPR;
-  const int li = threadIdx.x % LPR;
-  const long long item = (long long)blockIdx.x * GPB + threadIdx.x / LPR;
-  const int nk = a.pool.n_kv_heads;
-  const long long items = (long long)a.rows * nk * 2;
-  const bool real = item < items;
-  const int t = real ? (int)(item / (2 * nk)) : 0, rest = real ? (int)(item % (2 * nk)) : 0;
-  const int half = rest / nk, hk = rest % nk;
-  size_t row = 0;
-  const bool ok = real && place_of(a, t, hk, &row);
-  const bool active = ok && li * 8 < HS;
-  const T* src = (half ? v + (size_t)t * ldv : k + (size_t)t * ldk) + hk * HS + li * 8;
-  float x[8];
-  if (active) {
-    if (vec) {
-      load8(src, x);
-    } else {
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Minimum and maximum over the L lanes of a group, NaN if there is one.
+template <int L> __device__ __forceinline__ float group_min(float v) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = to_f32(src[i]);
-    }
-  }
-  float lo = INFINITY, hi = -INFINITY;
-  bool bad = false;
-  if (active) {
+  for (int o = L / 2; o > 0; o >>= 1) v = min_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+template <int L> __device__ __forceinline__ float group_max(float v) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      lo = fminf(lo, x[i]);
-      hi = fmaxf(hi, x[i]);
-      bad |= !(fabsf(x[i]) < INFINITY);
-    }
-  }
-#pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
-  }
-  if (!ok) return;
-  const float mn = bf16_down(lo);
-  const float spread = hi - mn;
-  bad |= !(spread < INFINITY) || !(mn > -INFINITY);
+  for (int o = L / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// a / b from the correctly rounded reciprocal of b: the product corrected once by its exact remainder is the rounded
+// quotient (Markstein), so halves come out as halves.  For numbers away from the ends of the range.
+__device__ __forceinline__ float divide(float a, float b, float inv_b) {
+  const float q = a * inv_b;
+  return fmaf(fmaf(-q, b, a), inv_b, q);
+}
+
+// Rows of equal elements, of a spread at the ends of the fp32 range, and rows that are not finite.
+__device__ __noinline__ uint2 quantise_rare(float4 x, float4 y, float mn, float spread) {
+  if (!(spread < INFINITY) || !(mn > -INFINITY)) return make_uint2(0u, 0x7fc07fc0u);
   const float scale = bf16_up_nonneg(__fdiv_rn(spread, 15.f));
-  if (half) row += kv4_half(a.pool);
-  if (active) {
-    uint32_t w = 0u;
-    if (!bad && scale > 0.f) {
+  uint32_t w = 0u;
+  if (scale > 0.f) {
+    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float c = fminf(rintf(__fdiv_rn(x[i] - mn, scale)), 15.f);
-        w |= (uint32_t)c << (4 * i);
+    for (int e = 0; e < 8; ++e) w |= (uint32_t)fminf(rintf(__fdiv_rn(v[e] - mn, scale)), 15.f) << (4 * e);
+  }
+  return make_uint2(w, __byte_perm(__float_as_uint(scale), __float_as_uint(mn), 0x7632));
+}
+
+// Eight elements as they stand in memory.
+template <typename T> struct Raw8;
+template <> struct Raw8<bf16> {
+  uint4 r;
+  __device__ __forceinline__ void load(const bf16* p) { r = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void set(int e, bf16 v) {
+    uint32_t& w = (&r.x)[e >> 1];
+    const uint32_t b = *reinterpret_cast<const uint16_t*>(&v);
+    w = (e & 1) ? (w & 0xffffu) | (b << 16) : (w & 0xffff0000u) | b;
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+template <> struct Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = *reinterpret_cast<const float4*>(p);
+    b = *reinterpret_cast<const float4*>(p + 4);
+  }
+  __device__ __forceinline__ void set(int e, float v) { (e < 4 ? (&a.x)[e] : (&b.x)[e - 4]) = v; }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+};
+
+// `part` of `parts` equal shares of the 2 n_kv_heads (half, head) items of a row; U items per lane group in flight, the
+// first of them requested before the row's place is looked up.
+template <typename T, int HS>
+__global__ void __launch_bounds__(AT, 4) kv4_append_kernel(Kv4RowsArgs a, const T* __restrict__ k, const T* __restrict__ v,
+                                                           int ldk, int ldv, bool vec, int parts, int per_part) {
+  constexpr int LPR = lanes_of(HS), GPW = 32 / LPR, U = sizeof(T) == 2 ? 4 : 2;
+  const int lane = threadIdx.x & 31, li = lane % LPR, sub = lane / LPR;
+  const long long w = (long long)blockIdx.x * (AT / 32) + (threadIdx.x >> 5);
+  const int t = (int)(w / parts), part = (int)(w - (long long)t * parts);
+  if (t >= a.rows) return;
+  const int nk = a.pool.n_kv_heads;
+  const int first = part * per_part, last = min(2 * nk, first + per_part);
+  const bool lane_on = li * 8 < HS;
+  const T* kt = k + (size_t)t * ldk + li * 8;
+  const T* vt = v + (size_t)t * ldv + li * 8;
+  Raw8<T> raw[U];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int item = i0 + j * GPW + sub;
+      if (item < last && lane_on) {
+        const T* src = item >= nk ? vt + (item - nk) * HS : kt + item * HS;
+        if (vec) {
+          raw[j].load(src);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) raw[j].set(e, src[e]);
+        }
       }
     }
-    reinterpret_cast<uint32_t*>(a.pool.codes)[row * (HS / 8) + li] = w;
+  };
+  load(first);
+  int page, in_page;
+  if (!place_of(a, t, &page, &in_page)) return;
+  const size_t row0 = (size_t)page * nk * a.pool.page_size + in_page, half = kv4_half(a.pool);
+  for (int i0 = first; i0 < last; i0 += U * GPW) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int item = i0 + j * GPW + sub;
+      if (i0 + j * GPW >= last) break;  // the same for the warp
+      float x[8], lo = INFINITY, hi = -INFINITY;
+      raw[j].get(x);
+      if (item < last && lane_on) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          lo = min3_nan(lo, x[e], x[e + 1]);
+          hi = max3_nan(hi, x[e], x[e + 1]);
+        }
+      }
+      lo = group_min<LPR>(lo);
+      hi = group_max<LPR>(hi);
+      const float mn = sizeof(T) == 2 ? lo : bf16_down(lo);  // a 16-bit minimum is one already
+      const float spread = hi - mn;
+      uint32_t word, prm;
+      if (spread > 0x1p-90f && spread < 0x1p90f) {
+        const float scale = bf16_up_nonneg(divide(spread, 15.f, 1.f / 15.f));
+        float inv;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+        inv = fmaf(fmaf(-scale, inv, 1.f), inv, inv);  // correctly rounded: no 8-bit number has a reciprocal near a midpoint
+        float c[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)  // adding 1.5 * 2^23 rounds to integers, ties to even
+          c[e] = (divide(x[e] - mn, scale, inv) + 12582912.f) - 12582912.f;
+        // four codes are a number below 2^16: packed by the multiply-add pipe, the integer pipe being the busier one
+        const float w0 = fmaf(fmaf(c[3], 16.f, c[2]), 256.f, fmaf(c[1], 16.f, c[0]));
+        const float w1 = fmaf(fmaf(c[7], 16.f, c[6]), 256.f, fmaf(c[5], 16.f, c[4]));
+        word = __byte_perm(__float_as_uint(w0 + 8388608.f), __float_as_uint(w1 + 8388608.f), 0x5410);
+        prm = __byte_perm(__float_as_uint(scale), __float_as_uint(mn), 0x7632);
+      } else {
+        const uint2 r = quantise_rare(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), mn, spread);
+        word = r.x;
+        prm = r.y;
+      }
+      if (item < last) {
+        const size_t row = row0 + (size_t)(item >= nk ? item - nk : item) * a.pool.page_size + (item >= nk ? half : 0);
+        if (lane_on) reinterpret_cast<uint32_t*>(a.pool.codes)[row * (HS / 8) + li] = word;
+        if (li == 0) a.pool.params[row] = prm;
+      }
+    }
+    load(i0 + U * GPW);
   }
-  if (li == 0) a.pool.params[row] = bad ? 0x7fc07fc0u : (__float_as_uint(scale) >> 16) | (__float_as_uint(mn) & 0xffff0000u);
 }
 
 // Reads packed rows back: minimum + scale * code (the product is exact in fp32), rounded to T.
 template <typename T, int HS>
-__global__ void __launch_bounds__(AT) kv4_read_kernel(Kv4RowsArgs a, T* __restrict__ k, T* __restrict__ v, int ldk, int ldv, bool vec) {
-  constexpr int LPR = lanes_of(HS), GPB = AT / LPR;
-  const int li = threadIdx.x % LPR;
-  const long long item = (long long)blockIdx.x * GPB + threadIdx.x / LPR;
+__global__ void __launch_bounds__(AT) kv4_read_kernel(Kv4RowsArgs a, T* __restrict__ k, T* __restrict__ v, int ldk, int ldv,
+                                                      bool vec, int parts, int per_part) {
+  constexpr int LPR = lanes_of(HS), GPW = 32 / LPR, U = 4;
+  const int lane = threadIdx.x & 31, li = lane % LPR, sub = lane / LPR;
+  const long long w = (long long)blockIdx.x * (AT / 32) + (threadIdx.x >> 5);
+  const int t = (int)(w / parts), part = (int)(w - (long long)t * parts);
+  if (t >= a.rows) return;
+  int page, in_page;
+  if (!place_of(a, t, &page, &in_page)) return;
   const int nk = a.pool.n_kv_heads;
-  if (item >= (long long)a.rows * nk * 2 || li * 8 >= HS) return;
-  const int t = (int)(item / (2 * nk)), rest = (int)(item % (2 * nk));
-  const int half = rest / nk, hk = rest % nk;
-  size_t row = 0;
-  if (!place_of(a, t, hk, &row)) return;
-  if (half) row += kv4_half(a.pool);
-  const uint32_t w = reinterpret_cast<const uint32_t*>(a.pool.codes)[row * (HS / 8) + li];
-  const uint32_t prm = a.pool.params[row];
-  const float scale = __uint_as_float(prm << 16), mn = __uint_as_float(prm & 0xffff0000u);
-  float x[8];
+  const int first = part * per_part, last = min(2 * nk, first + per_part);
+  const size_t row0 = (size_t)page * nk * a.pool.page_size + in_page, half = kv4_half(a.pool);
+  if (li * 8 >= HS) return;
+  for (int i0 = first; i0 < last; i0 += U * GPW) {
+    uint32_t word[U], prm[U];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((w >> (4 * i)) & 15u), scale, mn);
-  T* dst = (half ? v + (size_t)t * ldv : k + (size_t)t * ldk) + hk * HS + li * 8;
-  if (vec) {
-    store8(dst, x);
-  } else {
+    for (int j = 0; j < U; ++j) {
+      const int item = i0 + j * GPW + sub;
+      const bool is_v = item >= nk;
+      if (item < last) {
+        const size_t row = row0 + (size_t)(is_v ? item - nk : item) * a.pool.page_size + (is_v ? half : 0);
+        word[j] = reinterpret_cast<const uint32_t*>(a.pool.codes)[row * (HS / 8) + li];
+        prm[j] = a.pool.params[row];
+      }
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dst[i] = from_f32<T>(x[i]);
+    for (int j = 0; j < U; ++j) {
+      const int item = i0 + j * GPW + sub;
+      if (item >= last) break;
+      const bool is_v = item >= nk;
+      const float scale = __uint_as_float(prm[j] << 16), mn = __uint_as_float(prm[j] & 0xffff0000u);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)  // 2^23 + code, less 2^23: exact
+        x[e] = fmaf(__uint_as_float(((word[j] >> (4 * e)) & 15u) | 0x4b000000u) - 8388608.f, scale, mn);
+      T* dst = (is_v ? v + (size_t)t * ldv : k + (size_t)t * ldk) + (is_v ? item - nk : item) * HS + li * 8;
+      if (vec) {
+        store8(dst, x);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dst[e] = from_f32<T>(x[e]);
+      }
+    }
   }
+}
+
+// How many warps share a packed row: enough to fill the GPU when rows are few, never less than one item per lane group.
+void split_rows(int rows, int n_kv_heads, int head_size, int* parts, int* per_part) {
+  const int groups = 32 / lanes_of(head_size), items = 2 * n_kv_heads;
+  const int want = std::max(1, 32 * sm_count() / std::max(1, rows));
+  const int most = (items + groups - 1) / groups;
+  *parts = std::min(want, most);
+  *per_part = ((items + *parts - 1) / *parts + groups - 1) / groups * groups;
+  *parts = (items + *per_part - 1) / *per_part;
 }
 
 // ---- decode attention on the CUDA cores ----------------------------------------------------------------------------
@@ -424,12 +556,14 @@ int32_t b200_kv4_append(const void* k, const void* v, void* codes, void* params,
   a.status = device_status_word();
   if (!a.status) return fail(B200_ERR_CUDA, "no device status word");
   const bool vec = aligned16(k) && aligned16(v) && ldk % 8 == 0 && ldv % 8 == 0;
+  int parts, per_part;
+  split_rows(rows, n_kv_heads, head_size, &parts, &per_part);
+  const long long blocks = ((long long)rows * parts + AT / 32 - 1) / (AT / 32);
+  if (blocks > 0x7fffffffLL) return fail(B200_ERR_BAD_SHAPE, "kv4 append: too many rows");
   return by_type("kv4 append", dtype, head_size, [&](auto t, auto hs) -> int32_t {
     using T = decltype(t);
     constexpr int HS = decltype(hs)::value;
-    const long long groups = (long long)rows * n_kv_heads * 2, per = AT / lanes_of(HS), blocks = (groups + per - 1) / per;
-    if (blocks > 0x7fffffffLL) return fail(B200_ERR_BAD_SHAPE, "kv4 append: too many rows");
-    kv4_append_kernel<T, HS><<<(unsigned)blocks, AT, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, (const T*)k, (const T*)v, ldk, ldv, vec);
+    kv4_append_kernel<T, HS><<<(unsigned)blocks, AT, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, (const T*)k, (const T*)v, ldk, ldv, vec, parts, per_part);
     B200_LAUNCH_OK("kv4_append_kernel");
     return B200_OK;
   });
@@ -456,12 +590,14 @@ int32_t b200_kv4_read(void* k, void* v, const void* codes, const void* params, c
   a.status = device_status_word();
   if (!a.status) return fail(B200_ERR_CUDA, "no device status word");
   const bool vec = aligned16(k) && aligned16(v) && ldk % 8 == 0 && ldv % 8 == 0;
+  int parts, per_part;
+  split_rows(rows, n_kv_heads, head_size, &parts, &per_part);
+  const long long blocks = ((long long)rows * parts + AT / 32 - 1) / (AT / 32);
+  if (blocks > 0x7fffffffLL) return fail(B200_ERR_BAD_SHAPE, "kv4 read: too many rows");
   return by_type("kv4 read", dtype, head_size, [&](auto t, auto hs) -> int32_t {
     using T = decltype(t);
     constexpr int HS = decltype(hs)::value;
-    const long long groups = (long long)rows * n_kv_heads * 2, per = AT / lanes_of(HS), blocks = (groups + per - 1) / per;
-    if (blocks > 0x7fffffffLL) return fail(B200_ERR_BAD_SHAPE, "kv4 read: too many rows");
-    kv4_read_kernel<T, HS><<<(unsigned)blocks, AT, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, (T*)k, (T*)v, ldk, ldv, vec);
+    kv4_read_kernel<T, HS><<<(unsigned)blocks, AT, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, (T*)k, (T*)v, ldk, ldv, vec, parts, per_part);
     B200_LAUNCH_OK("kv4_read_kernel");
     return B200_OK;
   });

@@ -55,6 +55,11 @@ def test_append_and_read(hs, hk, page, dtype, lens, before):
     kv = torch.randn(T, 2 * hk * hs, generator=g, device=DEV).to(dtype)
     kv[0, :hs] = 0.25                       # a row of equal elements: scale 0
     kv[T - 1, :hs] = torch.linspace(-3, 3, hs, device=DEV).to(dtype)
+    if T > 20:                              # exact ties: (k + 1/2) steps of 1/4, and of the smallest and largest scales
+        kv[1, :hs] = (torch.arange(hs, device=DEV) % 31).to(dtype) / 8
+        kv[2, :hs] = kv[1, :hs] * 2.0 ** -124
+        kv[3, :hs] = kv[1, :hs] * 2.0 ** 124
+        kv[4, :hs] = -kv[1, :hs]
     k, v = kv[:, :hk * hs], kv[:, hk * hs:]
     table, n_pages = tables([n + b for n, b in zip(lens, before)], page)
     codes, params = B.new_kv4_pages(1, n_pages, hk, page, hs)
