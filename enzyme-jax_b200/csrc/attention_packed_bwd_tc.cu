@@ -1,21 +1,25 @@
 // Packed causal attention backward on the 5th-generation tensor cores (bf16, head size 64 or 128).  With
-//   P = exp(q k^T / sqrt(hs) - lse),  dP = dO v^T,  delta = rowsum(P * dP),  dS = P * (dP - delta) / sqrt(hs)
-// the gradients are dV = P^T dO, dK = dS^T Q, dQ = dS K.  Two passes of one kernel, both free of atomics:
+//   P = exp(q k^T / sqrt(hs) - lse),  dP = dO v^T,  delta = rowsum(P * dP),  dS = P * (dP - delta)
+// the gradients are dV = P^T dO, dK = dS^T Q / sqrt(hs), dQ = dS K / sqrt(hs).  Two passes of one kernel, both free of atomics:
 //   MODE_DQ   a CTA owns 128 queries of a query head and streams the keys and values they see
 //   MODE_DKV  a CTA owns 128 keys of a key head and streams, for every query head of the group, the queries and their
 //             cotangents that see them (so the gradient of a shared head is one sum in a fixed order)
 // Both have the same shape: two fixed tiles F0, F1 and streamed tiles X0, X1,
 //   S = F0 X0^T,  dP = F1 X1^T  (TMEM, rows = the CTA's own rows)  ->  P, dS as bf16 over S, dP in TMEM
-//   DQ  (F0 = Q, F1 = dO, X0 = K, X1 = V):  acc0 += P X0 (see below),  acc1 += dS X0 = dQ
-//   DKV (F0 = K, F1 = V, X0 = Q, X1 = dO):  acc0 += P X1 = dV,         acc1 += dS X0 = dK
+//   DQ  (F0 = Q, F1 = dO, X0 = K, X1 = V):  acc0 += P X0 (see below),  acc1 += dS X0 -> dQ
+//   DKV (F0 = K, F1 = V, X0 = Q, X1 = dO):  acc0 += P X1 = dV,         acc1 += dS X0 -> dK
 // so P and dS are TMEM operands of the accumulating products and never pass through shared memory.  The softmax threads'
 // two phases run beside the products of the other phase: exponentials (S -> P) beside acc1(n-1) and dP(n), the score
 // gradient (dP -> dS) beside acc0(n) and S(n+1).  S(n+1) may overwrite P(n), and dP(n+1) dS(n), because the tensor pipe
 // runs the products of one thread in order.
 //
+// Head size 64 streams blocks of 64 rows: S, dP and the accumulators are then 256 TMEM columns and 75 KB of shared memory,
+// two CTAs share an SM and one's set-up, waits and epilogue hide behind the other's products (8 x 1024 tokens, 12 heads:
+// 167 -> XX us).  Head size 128 takes all 512 columns with blocks of 128 rows.
+//
 // delta.  Taken from the output as rowsum(dO * o) it carries the rounding of o to bf16, which is not small beside
 // dP - delta where a row sees few keys.  The query pass therefore also sums eps = rowsum(P * (dP - delta0)) in fp32 and
-// acc0 = P K; dQ = acc1 - eps * acc0 / sqrt(hs) is then the gradient for the exact delta = delta0 + eps, which it leaves
+// acc0 = P K; dQ = (acc1 - eps * acc0) / sqrt(hs) is then the gradient for the exact delta = delta0 + eps, which it leaves
 // behind for the key pass.  A tile whose keys fit one block settles eps before it forms dS.
 //
 // Bound: 8 products of 128 x 128 x hs per (query block, key block), of which 5 are the formula's; 512 cycles each at head
@@ -39,13 +43,17 @@ enum { MODE_DKV = 0, MODE_DQ = 1 };
 enum : uint32_t { ST_PACKEDB_TIMEOUT = 1u << 19, ST_PACKEDB_ALIGN = 1u << 20 };
 
 template <int HS> struct BCfg {
+  static constexpr int kBlock = HS;                    // streamed rows per block
   static constexpr int kSubs = HS / 64;
-  static constexpr int kTile = kSubs * BSUB;
+  static constexpr int kTile = kSubs * BSUB;           // fixed tile
+  static constexpr int kXSub = kBlock * 128;           // one [kBlock rows x 64 columns] sub-tile
+  static constexpr int kXTile = kSubs * kXSub;         // streamed tile
   static constexpr int kX = 2 * kTile;
-  static constexpr int kStat = kX + NX * kTile;  // 2 stages x {lse2[128], delta[128]} of the streamed queries (DKV)
+  static constexpr int kStat = kX + NX * kXTile;  // 2 stages x {-lse2[kBlock], -delta[kBlock]} of the streamed queries (DKV)
   static constexpr int kBars = kStat + 2 * 1024;
   static constexpr int kSmem = kBars + 256;
-  static constexpr int cS = 0, cDP = 128, cAcc0 = 256, cAcc1 = 384;
+  static constexpr int cS = 0, cDP = kBlock, cAcc0 = 2 * kBlock, cAcc1 = 2 * kBlock + HS, kCols = 2 * kBlock + 2 * HS;
+  static constexpr int kCtas = HS == 64 ? 2 : 1;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -64,7 +72,16 @@ __device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t* v) {
+// N 32-bit columns of this thread's lane
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::
+          "r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
@@ -73,6 +90,11 @@ __device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t* v) {
       "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
       "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[32]) { ptx::tmem_ld32(taddr, v); }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[64]) {
+  ptx::tmem_ld32_at<0>(taddr, v);
+  ptx::tmem_ld32_at<32>(taddr + 32u, v);
 }
 
 struct OwnGeo {
@@ -83,11 +105,12 @@ struct OwnGeo {
 };
 
 template <int HS, int MODE>
-__global__ void __launch_bounds__(PB_THREADS, 1)
-    packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                         const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO, PackedBwdArgs a,
+__global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
+    packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmF0, const __grid_constant__ CUtensorMap tmF1,
+                         const __grid_constant__ CUtensorMap tmX0, const __grid_constant__ CUtensorMap tmX1, PackedBwdArgs a,
                          float scale, uint32_t* status) {
   using C = BCfg<HS>;
+  constexpr int BN = C::kBlock, NC = BN / 2;  // streamed rows per block; of them per softmax thread
   const PackedArgs& f = a.f;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBars);
@@ -129,18 +152,18 @@ __global__ void __launch_bounds__(PB_THREADS, 1)
     ptx::mbar_init(&stat_full[1], 32);
     ptx::mbar_init(s_full, 1);
     ptx::mbar_init(dp_full, 1);
-    ptx::mbar_init(p_full, 256);
-    ptx::mbar_init(ds_full, 256);
+    ptx::mbar_init(p_full, 8);
+    ptx::mbar_init(ds_full, 8);
     ptx::mbar_init(acc_done, 1);
     ptx::mbar_init(met, 256);
     ptx::fence_barrier_init();
-    ptx::tma_prefetch_desc(&tmQ);
-    ptx::tma_prefetch_desc(&tmK);
-    ptx::tma_prefetch_desc(&tmV);
-    ptx::tma_prefetch_desc(&tmDO);
+    ptx::tma_prefetch_desc(&tmF0);
+    ptx::tma_prefetch_desc(&tmF1);
+    ptx::tma_prefetch_desc(&tmX0);
+    ptx::tma_prefetch_desc(&tmX1);
   }
   if (warp == 1) {
-    ptx::tmem_alloc(tmem_slot, 512);
+    ptx::tmem_alloc(tmem_slot, C::kCols);
     ptx::tmem_relinquish();
   }
   pdl_wait();  // the operands come from the kernels before
@@ -160,7 +183,7 @@ __global__ void __launch_bounds__(PB_THREADS, 1)
       g.x0 = sp.first <= probe ? sp.first : cu_first;
       to = last_row + 1;
     }
-    g.per_head = last_row >= g.r0 && to > g.x0 ? (to - g.x0 + BR - 1) / BR : 0;
+    g.per_head = last_row >= g.r0 && to > g.x0 ? (to - g.x0 + BN - 1) / BN : 0;
     g.n_it = g.per_head * (MODE == MODE_DKV ? group : 1);
     if (lane == 0) *geo = g;
   }
@@ -179,34 +202,33 @@ __global__ void __launch_bounds__(PB_THREADS, 1)
       ptx::mbar_arrive_expect_tx(fix_full, 2 * C::kTile);
 #pragma unroll
       for (int s = 0; s < C::kSubs; ++s) {
-        ptx::tma_load_2d(smem + s * BSUB, MODE == MODE_DKV ? &tmK : &tmQ, head * HS + 64 * s, g.r0, fix_full);
-        ptx::tma_load_2d(smem + C::kTile + s * BSUB, MODE == MODE_DKV ? &tmV : &tmDO, head * HS + 64 * s, g.r0, fix_full);
+        ptx::tma_load_2d(smem + s * BSUB, &tmF0, head * HS + 64 * s, g.r0, fix_full);
+        ptx::tma_load_2d(smem + C::kTile + s * BSUB, &tmF1, head * HS + 64 * s, g.r0, fix_full);
       }
     }
     bool ok = true;
     for (int x = 0; x < 2 * n_it && ok; ++x) {
       const int st = x % NX, it = x >> 1;
       const int qh = MODE == MODE_DKV ? hk * group + it / g.per_head : head;
-      const int row = g.x0 + (it % g.per_head) * BR;
+      const int row = g.x0 + (it % g.per_head) * BN;
       ok = ptx::mbar_wait_warp(&x_empty[st], ((uint32_t)(x / NX) & 1u) ^ 1u, abort_flag, status, ST_PACKEDB_TIMEOUT);
       if (!ok) break;
       if (lane == 0) {
-        const CUtensorMap* map = MODE == MODE_DKV ? ((x & 1) ? &tmDO : &tmQ) : ((x & 1) ? &tmV : &tmK);
         const int col = (MODE == MODE_DKV ? qh : hk) * HS;
-        ptx::mbar_arrive_expect_tx(&x_full[st], C::kTile);
+        ptx::mbar_arrive_expect_tx(&x_full[st], C::kXTile);
 #pragma unroll
         for (int s = 0; s < C::kSubs; ++s)
-          ptx::tma_load_2d(smem + C::kX + st * C::kTile + s * BSUB, map, col + 64 * s, row, &x_full[st]);
+          ptx::tma_load_2d(smem + C::kX + st * C::kXTile + s * C::kXSub, (x & 1) ? &tmX1 : &tmX0, col + 64 * s, row, &x_full[st]);
       }
       if (MODE == MODE_DKV && (x & 1)) {
         // X1(it) takes the stage X0(it - 2) or an older tile had, so the statistics of it - 2 have been used
         float* stat = reinterpret_cast<float*>(smem + C::kStat + (it & 1) * 1024);
 #pragma unroll
-        for (int c = lane; c < BR; c += 32) {
+        for (int c = lane; c < BN; c += 32) {
           const int t = row + c;
           const size_t at = (size_t)qh * f.rows + t;
-          stat[c] = t < f.rows ? f.lse[at] * 1.4426950408889634f : 0.f;
-          stat[BR + c] = t < f.rows ? a.delta[at] : 0.f;
+          stat[c] = t < f.rows ? -f.lse[at] * 1.4426950408889634f : 0.f;
+          stat[BN + c] = t < f.rows ? -a.delta[at] : 0.f;
         }
         ptx::mbar_arrive(&stat_full[it & 1]);
       }
@@ -214,33 +236,34 @@ __global__ void __launch_bounds__(PB_THREADS, 1)
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t id_kk = ptx::idesc_bf16_f32(BR, BR);               // both operands K-major
+      constexpr uint32_t id_kk = ptx::idesc_bf16_f32(BR, BN);               // both operands K-major
       constexpr uint32_t id_tm = ptx::idesc_bf16_f32(BR, HS) | (1u << 16);  // A in TMEM, B MN-major
       const uint64_t fix_k = ptx::smem_desc_sw128(ptx::smem_u32(smem));
       const uint64_t x_k = ptx::smem_desc_sw128(ptx::smem_u32(smem + C::kX));
-      const uint64_t x_m = ptx::smem_desc_sw128_mn(ptx::smem_u32(smem + C::kX), BSUB);
-      constexpr uint64_t kT = C::kTile >> 4;
+      const uint64_t x_m = ptx::smem_desc_sw128_mn(ptx::smem_u32(smem + C::kX), C::kXSub);
+      constexpr uint64_t kT = C::kTile >> 4, kXT = C::kXTile >> 4;
       bool ok = ptx::mbar_wait(fix_full, 0, abort_flag, status, ST_PACKEDB_TIMEOUT);
       auto wait_x = [&](int x) {
         ok = ok && ptx::mbar_wait(&x_full[x % NX], (uint32_t)(x / NX) & 1u, abort_flag, status, ST_PACKEDB_TIMEOUT);
         if (ok) ptx::tc_fence_after_sync();
       };
       auto scores = [&](int which, int it) {  // 0: S = F0 X0^T, 1: dP = F1 X1^T
-        const uint64_t fa = fix_k + (uint64_t)which * kT, xa = x_k + (uint64_t)((2 * it + which) % NX) * kT;
+        const uint64_t fa = fix_k + (uint64_t)which * kT, xa = x_k + (uint64_t)((2 * it + which) % NX) * kXT;
 #pragma unroll
         for (int k = 0; k < HS / 16; ++k) {
-          const uint64_t off = (uint64_t)(((k >> 2) * BSUB + (k & 3) * 32) >> 4);
-          ptx::mma_bf16_ss(tmem_base + (uint32_t)(which ? C::cDP : C::cS), fa + off, xa + off, id_kk, k > 0 ? 1u : 0u);
+          const uint64_t foff = (uint64_t)(((k >> 2) * BSUB + (k & 3) * 32) >> 4);
+          const uint64_t xoff = (uint64_t)(((k >> 2) * C::kXSub + (k & 3) * 32) >> 4);
+          ptx::mma_bf16_ss(tmem_base + (uint32_t)(which ? C::cDP : C::cS), fa + foff, xa + xoff, id_kk, k > 0 ? 1u : 0u);
         }
         ptx::mma_commit(which ? dp_full : s_full);
       };
       auto accumulate = [&](int which, int it) {  // 0: acc0 += P X, 1: acc1 += dS X0
         const int tile = 2 * it + (which == 0 && MODE == MODE_DKV ? 1 : 0);
-        const uint64_t xa = x_m + (uint64_t)(tile % NX) * kT;
+        const uint64_t xa = x_m + (uint64_t)(tile % NX) * kXT;
         const uint32_t src = tmem_base + (uint32_t)(which ? C::cDP : C::cS);
 #pragma unroll
-        for (int k = 0; k < BR / 16; ++k)  // P / dS of columns 64h .. 64h+63 stands in TMEM columns 64h .. 64h+31
-          mma_bf16_ts(tmem_base + (uint32_t)(which ? C::cAcc1 : C::cAcc0), src + (uint32_t)((k >> 2) * 64 + (k & 3) * 8),
+        for (int k = 0; k < BN / 16; ++k)  // P / dS of a half's NC columns stands in the first NC / 2 of them
+          mma_bf16_ts(tmem_base + (uint32_t)(which ? C::cAcc1 : C::cAcc0), src + (uint32_t)(k / (NC / 16) * NC + k % (NC / 16) * 8),
                       xa + (uint64_t)(k * (2048 >> 4)), id_tm, (it > 0 || k > 0) ? 1u : 0u);
       };
       wait_x(0);
@@ -277,11 +300,11 @@ __global__ void __launch_bounds__(PB_THREADS, 1)
     __syncwarp();
   } else {
     const int qd = warp & 3;
-    const int hf = (warp - 2) >> 2;   // columns 64 hf .. 64 hf + 63 of a block
+    const int hf = (warp - 2) >> 2;   // columns NC hf .. NC hf + NC - 1 of a block
     const int row = qd * 32 + lane;   // TMEM lane: the CTA's own row
     const int r = g.r0 + row;
     const uint32_t lane_base = tmem_base + ((uint32_t)(qd * 32) << 16);
-    const uint32_t t_s = lane_base + (uint32_t)(C::cS + hf * 64), t_dp = lane_base + (uint32_t)(C::cDP + hf * 64);
+    const uint32_t t_s = lane_base + (uint32_t)(C::cS + hf * NC), t_dp = lane_base + (uint32_t)(C::cDP + hf * NC);
     const float sl2 = scale * 1.4426950408889634f;
     const int s = r < f.rows ? seq_of_row(f.cu, 0, f.n_seqs, r) : -1;
     const RowSpan span = row_span(f.cu, f.n_seqs, s, r, f.rows);
@@ -302,12 +325,12 @@ __global__ void __launch_bounds__(PB_THREADS, 1)
     };
     for (int it = 0; it < n_it; ++it) {
       const uint32_t ph = (uint32_t)it & 1u;
-      const int c0 = g.x0 + (it % g.per_head) * BR + hf * 64;  // streamed row of this thread's first column
-      // columns lo..hi of the 64 form a pair with the own row
-      const int lo = live ? (MODE == MODE_DQ ? span.first : r) - c0 : 64;
+      const int c0 = g.x0 + (it % g.per_head) * BN + hf * NC;  // streamed row of this thread's first column
+      // columns lo..hi of the NC form a pair with the own row
+      const int lo = live ? (MODE == MODE_DQ ? span.first : r) - c0 : NC;
       const int hi = live ? (MODE == MODE_DQ ? r : span.last - 1) - c0 : -1;
-      const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < 63);
-      const float* stat = reinterpret_cast<const float*>(smem + C::kStat + (it & 1) * 1024) + hf * 64;
+      const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < NC - 1);
+      const float* stat = reinterpret_cast<const float*>(smem + C::kStat + (it & 1) * 1024) + hf * NC;
       if (MODE == MODE_DKV) {
         ok = ptx::mbar_wait_warp(&stat_full[it & 1], (uint32_t)(it >> 1) & 1u, abort_flag, status, ST_PACKEDB_TIMEOUT);
         if (!ok) break;
@@ -315,86 +338,90 @@ __global__ void __launch_bounds__(PB_THREADS, 1)
       ok = ptx::mbar_wait_warp(s_full, ph, abort_flag, status, ST_PACKEDB_TIMEOUT);
       if (!ok) break;
       ptx::tc_fence_after_sync();
-      float p[64];
-      ptx::tmem_ld32_at<0>(t_s, p);
-      ptx::tmem_ld32_at<32>(t_s + 32u, p);
+      float p[NC];
+      tmem_ld(t_s, p);
       ptx::tmem_ld_wait();
-      uint32_t pk[32];
+      uint32_t pk[NC / 2];
+      const float2 sl2v = make_float2(sl2, sl2);
 #pragma unroll
-      for (int e = 0; e < 64; e += 4) {
-        float4 l4 = make_float4(lse2, lse2, lse2, lse2);
+      for (int e = 0; e < NC; e += 4) {
+        float4 l4 = make_float4(-lse2, -lse2, -lse2, -lse2);
         if (MODE == MODE_DKV) l4 = *reinterpret_cast<const float4*>(stat + e);
-        p[e] = ex2(fmaf(p[e], sl2, -l4.x));
-        p[e + 1] = ex2(fmaf(p[e + 1], sl2, -l4.y));
-        p[e + 2] = ex2(fmaf(p[e + 2], sl2, -l4.z));
-        p[e + 3] = ex2(fmaf(p[e + 3], sl2, -l4.w));
+        const float2 x0 = __ffma2_rn(make_float2(p[e], p[e + 1]), sl2v, make_float2(l4.x, l4.y));
+        const float2 x1 = __ffma2_rn(make_float2(p[e + 2], p[e + 3]), sl2v, make_float2(l4.z, l4.w));
+        p[e] = ex2(x0.x);
+        p[e + 1] = ex2(x0.y);
+        p[e + 2] = ex2(x1.x);
+        p[e + 3] = ex2(x1.y);
       }
       if (cut) {
 #pragma unroll
-        for (int e = 0; e < 64; ++e)
+        for (int e = 0; e < NC; ++e)
           if (e < lo || e > hi) p[e] = 0.f;
       }
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
+      for (int e = 0; e < NC / 2; ++e) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(p[2 * e], p[2 * e + 1]);
         pk[e] = *reinterpret_cast<const uint32_t*>(&h);
       }
       // the two halves read and write disjoint columns of S
-      tmem_st32u(t_s, pk);
+      tmem_st(t_s, pk);
       ptx::tmem_st_wait();
       ptx::tc_fence_before_sync();
-      ptx::mbar_arrive(p_full);
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(p_full);
 
       ok = ptx::mbar_wait_warp(dp_full, ph, abort_flag, status, ST_PACKEDB_TIMEOUT);
       if (!ok) break;
       ptx::tc_fence_after_sync();
-      float dp[64];
-      ptx::tmem_ld32_at<0>(t_dp, dp);
-      ptx::tmem_ld32_at<32>(t_dp + 32u, dp);
+      float dp[NC];
+      tmem_ld(t_dp, dp);
       ptx::tmem_ld_wait();
-      float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 64; e += 4) {
-        float4 d4 = make_float4(delta, delta, delta, delta);
-        if (MODE == MODE_DKV) d4 = *reinterpret_cast<const float4*>(stat + BR + e);
-        dp[e] = p[e] * (dp[e] - d4.x);
-        dp[e + 1] = p[e + 1] * (dp[e + 1] - d4.y);
-        dp[e + 2] = p[e + 2] * (dp[e + 2] - d4.z);
-        dp[e + 3] = p[e + 3] * (dp[e + 3] - d4.w);
+      for (int e = 0; e < NC; e += 4) {
+        float4 d4 = make_float4(-delta, -delta, -delta, -delta);
+        if (MODE == MODE_DKV) d4 = *reinterpret_cast<const float4*>(stat + BN + e);
+        const float2 y0 = __fmul2_rn(__fadd2_rn(make_float2(dp[e], dp[e + 1]), make_float2(d4.x, d4.y)), make_float2(p[e], p[e + 1]));
+        const float2 y1 = __fmul2_rn(__fadd2_rn(make_float2(dp[e + 2], dp[e + 3]), make_float2(d4.z, d4.w)), make_float2(p[e + 2], p[e + 3]));
+        dp[e] = y0.x;
+        dp[e + 1] = y0.y;
+        dp[e + 2] = y1.x;
+        dp[e + 3] = y1.y;
       }
       if (cut) {
 #pragma unroll
-        for (int e = 0; e < 64; ++e)
+        for (int e = 0; e < NC; ++e)
           if (e < lo || e > hi) dp[e] = 0.f;
       }
       if (MODE == MODE_DQ) {
-        float s0 = 0.f, s1 = 0.f;
+        float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int e = 0; e < 64; e += 2) {
-          s0 += dp[e];
-          s1 += dp[e + 1];
+        for (int e = 0; e < NC; e += 4) {
+          s0 = __fadd2_rn(s0, make_float2(dp[e], dp[e + 1]));
+          s1 = __fadd2_rn(s1, make_float2(dp[e + 2], dp[e + 3]));
         }
-        sum = s0 + s1;
+        float sum = (s0.x + s0.y) + (s1.x + s1.y);
         if (n_it == 1) {  // all keys of the row are here: settle delta before dS is rounded
           share[hf * BR + row] = sum;
           if (!meet()) break;
           sum += share[(hf ^ 1) * BR + row];
           delta += sum;
 #pragma unroll
-          for (int e = 0; e < 64; ++e) dp[e] = fmaf(-p[e], sum, dp[e]);
+          for (int e = 0; e < NC; ++e) dp[e] = fmaf(-p[e], sum, dp[e]);
         } else {
           eps += sum;
         }
       }
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(dp[2 * e] * scale, dp[2 * e + 1] * scale);
+      for (int e = 0; e < NC / 2; ++e) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(dp[2 * e], dp[2 * e + 1]);
         pk[e] = *reinterpret_cast<const uint32_t*>(&h);
       }
-      tmem_st32u(t_dp, pk);
+      tmem_st(t_dp, pk);
       ptx::tmem_st_wait();
       ptx::tc_fence_before_sync();
-      ptx::mbar_arrive(ds_full);
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ds_full);
     }
     if (ok) ok = ptx::mbar_wait_warp(acc_done, 0, abort_flag, status, ST_PACKEDB_TIMEOUT);
     if (ok) {
@@ -404,6 +431,7 @@ __global__ void __launch_bounds__(PB_THREADS, 1)
         // half 0 writes dV, half 1 dK
         bf16* dst = hf == 0 ? (bf16*)a.dv + (size_t)r * a.lddv : (bf16*)a.dk + (size_t)r * a.lddk;
         const uint32_t src = lane_base + (uint32_t)(hf == 0 ? C::cAcc0 : C::cAcc1);
+        const float out_scale = hf == 0 ? 1.f : scale;
 #pragma unroll 1
         for (int c = 0; c < HS; c += 32) {
           float v[32];
@@ -415,7 +443,7 @@ __global__ void __launch_bounds__(PB_THREADS, 1)
               float w[8];
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                w[j] = v[e + j];
+                w[j] = v[e + j] * out_scale;
                 finite = finite && fabsf(w[j]) < INFINITY;
               }
               store8(dst + head * HS + c + e, w);
@@ -430,7 +458,6 @@ __global__ void __launch_bounds__(PB_THREADS, 1)
           delta += eps;
         }
         if (live && hf == 0) a.delta[(size_t)head * f.rows + r] = delta;
-        const float back = eps * scale;
         bf16* dst = (bf16*)a.dq + (size_t)r * a.lddq + head * HS;
 #pragma unroll 1
         for (int c = hf * (HS / 2); c < (hf + 1) * (HS / 2); c += 32) {
@@ -444,7 +471,7 @@ __global__ void __launch_bounds__(PB_THREADS, 1)
               float w[8];
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                w[j] = fmaf(-back, u[e + j], v[e + j]);
+                w[j] = fmaf(-eps, u[e + j], v[e + j]) * scale;
                 finite = finite && fabsf(w[j]) < INFINITY;
               }
               store8(dst + c + e, w);
@@ -487,7 +514,7 @@ __global__ void __launch_bounds__(PB_THREADS, 1)
   }
   if (warp == 1) {
     ptx::tc_fence_after_sync();
-    ptx::tmem_dealloc(tmem_base, 512);
+    ptx::tmem_dealloc(tmem_base, C::kCols);
   }
 }
 
@@ -516,11 +543,16 @@ template <int HS>
 int32_t launch_hs(const PackedBwdArgs& a, cudaStream_t stream) {
   using C = BCfg<HS>;
   const PackedArgs& f = a.f;
-  CUtensorMap tq, tk, tv, tdo;
-  B200_TRY(make_map_2d(&tq, f.q, f.rows, f.n_heads * HS, f.ldq, BR));
-  B200_TRY(make_map_2d(&tk, f.k, f.rows, f.n_kv_heads * HS, f.ldk, BR));
-  B200_TRY(make_map_2d(&tv, f.v, f.rows, f.n_kv_heads * HS, f.ldv, BR));
-  B200_TRY(make_map_2d(&tdo, a.d_o, f.rows, f.n_heads * HS, a.lddo, BR));
+  // as the fixed tile of one pass (128 rows) and as the streamed tile of the other
+  CUtensorMap fq, fk, fv, fdo, xq, xk, xv, xdo;
+  B200_TRY(make_map_2d(&fq, f.q, f.rows, f.n_heads * HS, f.ldq, BR));
+  B200_TRY(make_map_2d(&fk, f.k, f.rows, f.n_kv_heads * HS, f.ldk, BR));
+  B200_TRY(make_map_2d(&fv, f.v, f.rows, f.n_kv_heads * HS, f.ldv, BR));
+  B200_TRY(make_map_2d(&fdo, a.d_o, f.rows, f.n_heads * HS, a.lddo, BR));
+  B200_TRY(make_map_2d(&xq, f.q, f.rows, f.n_heads * HS, f.ldq, C::kBlock));
+  B200_TRY(make_map_2d(&xk, f.k, f.rows, f.n_kv_heads * HS, f.ldk, C::kBlock));
+  B200_TRY(make_map_2d(&xv, f.v, f.rows, f.n_kv_heads * HS, f.ldv, C::kBlock));
+  B200_TRY(make_map_2d(&xdo, a.d_o, f.rows, f.n_heads * HS, a.lddo, C::kBlock));
   auto dq = packed_bwd_tc_kernel<HS, MODE_DQ>;
   auto dkv = packed_bwd_tc_kernel<HS, MODE_DKV>;
   static PerDeviceOnce attr_once;
@@ -536,10 +568,10 @@ int32_t launch_hs(const PackedBwdArgs& a, cudaStream_t stream) {
   B200_CUDA_OK(launch_pdl(packed_delta_vec_kernel<HS>, dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, stream, a));
   B200_LAUNCH_OK("packed_delta_vec_kernel");
   const unsigned blocks = (unsigned)cdiv(f.rows, BR);
-  B200_CUDA_OK(launch_pdl(dq, dim3(f.n_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, tq, tk, tv, tdo, a, scale,
+  B200_CUDA_OK(launch_pdl(dq, dim3(f.n_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, fq, fdo, xk, xv, a, scale,
                           status));
   B200_LAUNCH_OK("packed_bwd_tc_kernel<dq>");
-  B200_CUDA_OK(launch_pdl(dkv, dim3(f.n_kv_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, tq, tk, tv, tdo, a, scale,
+  B200_CUDA_OK(launch_pdl(dkv, dim3(f.n_kv_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, fk, fv, xq, xdo, a, scale,
                           status));
   B200_LAUNCH_OK("packed_bwd_tc_kernel<dkv>");
   return B200_OK;

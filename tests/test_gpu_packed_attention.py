@@ -171,7 +171,10 @@ def test_equals_rectangular_attention():
     q, k, v, d_o = make([s] * b, heads, heads, hs, torch.bfloat16, seed=8)
     o, lse = B.attention_packed(q, k, v, cu_of([s] * b), heads)
     o2, lse2 = B.attention(q, k, v, b, s, heads)
-    assert torch.allclose(o.float(), o2.float(), rtol=2 ** -7, atol=2 ** -7)
+    # both are within the bound of the exact result (weights and outputs rounded to bf16), so within twice that of each
+    # other; a fixed 2^-7 (1 + |o|) was no bound, as sum p|v| exceeds 1 where few keys are seen
+    bound = R.forward(q, k, v, [s] * b, heads, heads)[2]
+    assert bool(((o.double() - o2.double()).abs() <= 2 * bound).all())
     assert torch.allclose(lse.view(heads, b, s).transpose(0, 1), lse2, rtol=1e-5, atol=1e-5)
 
 
