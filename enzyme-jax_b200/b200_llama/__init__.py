@@ -296,24 +296,36 @@ def attention_decode_static(q: torch.Tensor, kv_layer: torch.Tensor, page_table:
 # packed prompts, the 4-bit cache, page copies
 # --------------------------------------------------------------------------
 
-def _device_of(what: str, **tensors):
-    """The one CUDA device all given tensors are on."""
-    dev = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+def _device_of(what: str, names: str, *tensors) -> torch.device:
+    """The one CUDA device all given tensors (None: left out) are on; ``names``: their names, for the message."""
+    first = None
+    try:
+        for t in tensors:
+            if t is None:
+                continue
+            d = t.get_device()
+            if first is None:
+                first = d
+            if d != first or d < 0:
+                break
+        else:
+            return _DEVICES[first]
+    except AttributeError:
+        pass
+    except IndexError:
+        return torch.device("cuda", first)
+    for name, t in zip(names.split(), tensors):
+        if t is not None and (not isinstance(t, torch.Tensor) or not t.is_cuda):
             raise B200Error(1, f"{what}: {name} must be a CUDA tensor")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise B200Error(1, f"{what}: {name} is on {t.device}, the others on {dev}")
-    return dev
+    raise B200Error(1, f"{what}: the tensors {names} are not all on one device")
+
+
+_DEVICES = [torch.device("cuda", i) for i in range(16)]
 
 
 def _call(dev: torch.device, fn, *args) -> None:
-    """``fn(*args, stream)`` with ``dev`` current, on its current stream (the raw handle: building the Stream object costs
-    more than the launch)."""
+    """``fn(*args, stream)`` with ``dev`` current, on its current stream (the raw handle: building the Stream object
+    costs more than the launch)."""
     if dev.index == torch._C._cuda_getDevice():
         status = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
@@ -328,7 +340,8 @@ def _rows(what: str, name: str, t: torch.Tensor, cols: int, rows: Optional[int] 
     """Row pitch of a [rows, cols] tensor with unit column stride."""
     shape = t.shape
     if len(shape) != 2 or shape[1] != cols or (rows is not None and shape[0] != rows):
-        raise B200Error(2, f"{what}: {name} has shape {tuple(shape)}, expected [{'rows' if rows is None else rows}, {cols}]")
+        raise B200Error(2, f"{what}: {name} has shape {tuple(shape)}, expected "
+                           f"[{'rows' if rows is None else rows}, {cols}]")
     if dtype is not None and t.dtype != dtype:
         raise B200Error(3, f"{what}: {name} is {t.dtype}, expected {dtype}")
     ld, unit = t.stride()
@@ -342,7 +355,7 @@ def _rows(what: str, name: str, t: torch.Tensor, cols: int, rows: Optional[int] 
 
 
 def _index(what: str, name: str, t: torch.Tensor, dim: int = 1) -> None:
-    if t.dtype != torch.int32 or t.dim() != dim or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.dim() != dim or not t.is_contiguous():
         raise B200Error(3, f"{what}: {name} must be a contiguous int32 tensor of {dim} dimension(s)")
 
 
@@ -362,7 +375,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     fp32 [n_heads, rows].  Rows of no sequence are not written: give ``out`` / ``lse`` to choose what stands there."""
     what = "attention_packed"
     n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
-    dev = _device_of(what, q=q, k=k, v=v, cu_seqlens=cu_seqlens, out=out, lse=lse)
+    dev = _device_of(what, "q k v cu_seqlens out lse", q, k, v, cu_seqlens, out, lse)
     hs = _heads(what, q, n_heads, n_kv_heads)
     rows, dt = q.shape[0], q.dtype
     ldq = _rows(what, "q", q, n_heads * hs)
@@ -392,7 +405,8 @@ def attention_packed_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     are summed over the query heads of a group.  Rows of no sequence are not written."""
     what = "attention_packed_backward"
     n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
-    dev = _device_of(what, q=q, k=k, v=v, o=o, lse=lse, d_o=d_o, cu_seqlens=cu_seqlens, dq=dq, dk=dk, dv=dv)
+    dev = _device_of(what, "q k v o lse d_o cu_seqlens dq dk dv",
+                     q, k, v, o, lse, d_o, cu_seqlens, dq, dk, dv)
     hs = _heads(what, q, n_heads, n_kv_heads)
     rows, dt = q.shape[0], q.dtype
     wq, wk = n_heads * hs, n_kv_heads * hs
@@ -434,7 +448,7 @@ def new_kv4_pages(n_layers: int, n_pages: int, n_kv_heads: int, page_size: int, 
 def _kv4_layer(what: str, codes: torch.Tensor, params: torch.Tensor):
     if codes.dim() != 5 or codes.shape[0] != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous():
         raise B200Error(2, f"{what}: codes must be a contiguous uint8 [2, n_pages, n_kv_heads, page_size, hs/2]")
-    if params.dtype != torch.bfloat16 or tuple(params.shape) != tuple(codes.shape[:4]) + (2,) or not params.is_contiguous():
+    if params.dtype != torch.bfloat16 or params.shape != codes.shape[:4] + (2,) or not params.is_contiguous():
         raise B200Error(2, f"{what}: params must be a contiguous bf16 {tuple(codes.shape[:4]) + (2,)}")
     _, n_pages, n_kv_heads, page_size, half = codes.shape
     return n_pages, n_kv_heads, page_size, 2 * half
@@ -459,8 +473,8 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, params: to
     its cached row ``ctx_before[s] + t - cu_seqlens[s]`` (``ctx_before`` None: the sequences start empty).  Rows without
     a place (behind the page table, or a page id outside the pool) are skipped and make :func:`device_status` raise."""
     what = "kv4_append"
-    dev = _device_of(what, k=k, v=v, codes=codes, params=params, page_table=page_table, cu_seqlens=cu_seqlens,
-                     ctx_before=ctx_before)
+    dev = _device_of(what, "k v codes params page_table cu_seqlens ctx_before",
+                     k, v, codes, params, page_table, cu_seqlens, ctx_before)
     n_pages, n_kv_heads, page_size, hs = _kv4_layer(what, codes, params)
     n_seqs = _kv4_rows(what, page_table, cu_seqlens, ctx_before)
     ldk = _rows(what, "k", k, n_kv_heads * hs)
@@ -477,8 +491,8 @@ def kv4_read(codes: torch.Tensor, params: torch.Tensor, page_table: torch.Tensor
     ``cu_seqlens`` and ``ctx_before``, e.g. the keys of a shared prefix for :func:`attention_packed`.  Rows without a
     place are not written."""
     what = "kv4_read"
-    dev = _device_of(what, codes=codes, params=params, page_table=page_table, cu_seqlens=cu_seqlens,
-                     ctx_before=ctx_before, k=k, v=v)
+    dev = _device_of(what, "codes params page_table cu_seqlens ctx_before k v",
+                     codes, params, page_table, cu_seqlens, ctx_before, k, v)
     n_pages, n_kv_heads, page_size, hs = _kv4_layer(what, codes, params)
     n_seqs = _kv4_rows(what, page_table, cu_seqlens, ctx_before)
     k = torch.empty(rows, n_kv_heads * hs, dtype=dtype, device=dev) if k is None else k
@@ -505,8 +519,8 @@ def attention_decode_kv4(q: torch.Tensor, codes: torch.Tensor, params: torch.Ten
     ``ctx_lens[b]`` (int32 [batch] on the device) cached rows; zero rows give a zero output.  Query head h reads key head
     h / (n_heads / n_kv_heads)."""
     what = "attention_decode_kv4"
-    dev = _device_of(what, q=q, codes=codes, params=params, page_table=page_table, ctx_lens=ctx_lens, out=out,
-                     scratch=scratch)
+    dev = _device_of(what, "q codes params page_table ctx_lens out scratch",
+                     q, codes, params, page_table, ctx_lens, out, scratch)
     n_pages, n_kv_heads, page_size, hs = _kv4_layer(what, codes, params)
     if n_heads <= 0 or n_heads % n_kv_heads:
         raise B200Error(2, f"{what}: {n_heads} query heads over {n_kv_heads} key heads")
@@ -515,7 +529,8 @@ def attention_decode_kv4(q: torch.Tensor, codes: torch.Tensor, params: torch.Ten
     _index(what, "page_table", page_table, 2)
     _index(what, "ctx_lens", ctx_lens)
     if page_table.shape[0] != batch or ctx_lens.numel() != batch:
-        raise B200Error(2, f"{what}: page_table {tuple(page_table.shape)} and ctx_lens {tuple(ctx_lens.shape)} for a batch of {batch}")
+        raise B200Error(2, f"{what}: page_table {tuple(page_table.shape)} and ctx_lens {tuple(ctx_lens.shape)} for a "
+                           f"batch of {batch}")
     if out is None:
         out = torch.empty(batch, n_heads * hs, dtype=q.dtype, device=dev)
     ldo = _rows(what, "out", out, n_heads * hs, batch, q.dtype)
@@ -564,7 +579,7 @@ def _copy_pages(what, pool, src, dst, rows, page_table, page_map) -> None:
         raise B200Error(2, f"{what}: src, dst and rows must have one entry per copy")
     if page_map is not None and page_map.numel() != n_pages:
         raise B200Error(2, f"{what}: page_map has {page_map.numel()} entries for {n_pages} pages")
-    dev = _device_of(what, pool=pool, src=src, dst=dst, rows=rows, page_table=page_table, page_map=page_map)
+    dev = _device_of(what, "pool src dst rows page_table page_map", pool, src, dst, rows, page_table, page_map)
     if pool.numel() == 0:
         return
     _call(dev, lib().b200_copy_pages, pool.data_ptr(), planes, n_pages, n_heads, page_size, row * pool.element_size(),
@@ -578,7 +593,7 @@ def copy_pages(pool: torch.Tensor, src, dst, rows=None) -> None:
     ``rows`` is given.  Lists of page numbers are checked on the host; int32 CUDA tensors are taken as they are, and
     their destinations must be distinct and no copy's source."""
     what = "copy_pages"
-    _device_of(what, pool=pool)
+    _device_of(what, "pool", pool)
     lists = [not isinstance(x, torch.Tensor) for x in (src, dst)]
     if all(lists):
         src, dst = [int(p) for p in src], [int(p) for p in dst]
@@ -598,7 +613,7 @@ def compact_pages(pools, src, dst, page_table: torch.Tensor, page_map) -> None:
     pools = list(pools) if isinstance(pools, (list, tuple)) else [pools]
     if not pools:
         raise B200Error(1, f"{what}: no pool")
-    _device_of(what, page_table=page_table, **{f"pools[{i}]": p for i, p in enumerate(pools)})
+    _device_of(what, "page_table pools", page_table, *pools)
     if page_table.dtype != torch.int32 or not page_table.is_contiguous():
         raise B200Error(3, f"{what}: page_table must be a contiguous int32 tensor")
     dev = page_table.device
