@@ -79,8 +79,11 @@ struct RowSpan { int first, last; };
 __device__ __forceinline__ RowSpan row_span(const int32_t* __restrict__ cu, int n_seqs, int s, int t, int rows) {
   RowSpan r{t + 1, t + 1};
   if (s >= 0 && s < n_seqs && t < rows) {
-    r.first = max(0, min(t, *(cu + s)));
-    r.last = min(rows, max(t + 1, *(cu + s + 1)));
+    const int end = cu[s + 1];
+    if (t < end) {  // (a search among some of the sequences only may stop at one before the row)
+      r.first = max(0, min(t, cu[s]));
+      r.last = min(rows, end);
+    }
   }
   return r;
 }

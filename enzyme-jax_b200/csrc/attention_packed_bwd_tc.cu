@@ -15,7 +15,7 @@
 //
 // Head size 64 streams blocks of 64 rows: S, dP and the accumulators are then 256 TMEM columns and 75 KB of shared memory,
 // two CTAs share an SM and one's set-up, waits and epilogue hide behind the other's products (8 x 1024 tokens, 12 heads:
-// 167 -> XX us).  Head size 128 takes all 512 columns with blocks of 128 rows.
+// 167 -> 146 us).  Head size 128 takes all 512 columns with blocks of 128 rows.
 //
 // delta.  Taken from the output as rowsum(dO * o) it carries the rounding of o to bf16, which is not small beside
 // dP - delta where a row sees few keys.  The query pass therefore also sums eps = rowsum(P * (dP - delta0)) in fp32 and
@@ -95,6 +95,22 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[32]) { ptx::t
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[64]) {
   ptx::tmem_ld32_at<0>(taddr, v);
   ptx::tmem_ld32_at<32>(taddr + 32u, v);
+}
+
+// 16 numbers of one row: a thread writes a row by itself, so whole 32-byte sectors at a time where the rows allow it
+__device__ __forceinline__ void store16(bf16* p, const float (&w)[16], bool wide) {
+  uint32_t r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(w[2 * i], w[2 * i + 1]);
+    r[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  if (wide) {
+    store32B(p, r);
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(r[0], r[1], r[2], r[3]);
+    *reinterpret_cast<uint4*>(p + 8) = make_uint4(r[4], r[5], r[6], r[7]);
+  }
 }
 
 struct OwnGeo {
@@ -329,7 +345,8 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
       // columns lo..hi of the NC form a pair with the own row
       const int lo = live ? (MODE == MODE_DQ ? span.first : r) - c0 : NC;
       const int hi = live ? (MODE == MODE_DQ ? r : span.last - 1) - c0 : -1;
-      const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < NC - 1);
+      // (one comparison per score and border: most blocks have none, most others one of the two)
+      const bool cut_lo = __any_sync(0xffffffffu, lo > 0), cut_hi = __any_sync(0xffffffffu, hi < NC - 1);
       const float* stat = reinterpret_cast<const float*>(smem + C::kStat + (it & 1) * 1024) + hf * NC;
       if (MODE == MODE_DKV) {
         ok = ptx::mbar_wait_warp(&stat_full[it & 1], (uint32_t)(it >> 1) & 1u, abort_flag, status, ST_PACKEDB_TIMEOUT);
@@ -354,10 +371,15 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
         p[e + 2] = ex2(x1.x);
         p[e + 3] = ex2(x1.y);
       }
-      if (cut) {
+      if (cut_hi) {
 #pragma unroll
         for (int e = 0; e < NC; ++e)
-          if (e < lo || e > hi) p[e] = 0.f;
+          if (e > hi) p[e] = 0.f;
+      }
+      if (cut_lo) {
+#pragma unroll
+        for (int e = 0; e < NC; ++e)
+          if (e < lo) p[e] = 0.f;
       }
 #pragma unroll
       for (int e = 0; e < NC / 2; ++e) {
@@ -388,10 +410,15 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
         dp[e + 2] = y1.x;
         dp[e + 3] = y1.y;
       }
-      if (cut) {
+      if (cut_hi) {
 #pragma unroll
         for (int e = 0; e < NC; ++e)
-          if (e < lo || e > hi) dp[e] = 0.f;
+          if (e > hi) dp[e] = 0.f;
+      }
+      if (cut_lo) {
+#pragma unroll
+        for (int e = 0; e < NC; ++e)
+          if (e < lo) dp[e] = 0.f;
       }
       if (MODE == MODE_DQ) {
         float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f);
@@ -432,6 +459,7 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
         bf16* dst = hf == 0 ? (bf16*)a.dv + (size_t)r * a.lddv : (bf16*)a.dk + (size_t)r * a.lddk;
         const uint32_t src = lane_base + (uint32_t)(hf == 0 ? C::cAcc0 : C::cAcc1);
         const float out_scale = hf == 0 ? 1.f : scale;
+        const bool wide_rows = ((hf == 0 ? a.lddv : a.lddk) & 15) == 0 && aligned32(hf == 0 ? a.dv : a.dk);
 #pragma unroll 1
         for (int c = 0; c < HS; c += 32) {
           float v[32];
@@ -439,14 +467,14 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
           ptx::tmem_ld_wait();
           if (live) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              float w[8];
+            for (int e = 0; e < 32; e += 16) {
+              float w[16];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
+              for (int j = 0; j < 16; ++j) {
                 w[j] = v[e + j] * out_scale;
                 finite = finite && fabsf(w[j]) < INFINITY;
               }
-              store8(dst + head * HS + c + e, w);
+              store16(dst + head * HS + c + e, w, wide_rows);
             }
           }
         }
@@ -459,6 +487,7 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
         }
         if (live && hf == 0) a.delta[(size_t)head * f.rows + r] = delta;
         bf16* dst = (bf16*)a.dq + (size_t)r * a.lddq + head * HS;
+        const bool wide_rows = (a.lddq & 15) == 0 && aligned32(a.dq);
 #pragma unroll 1
         for (int c = hf * (HS / 2); c < (hf + 1) * (HS / 2); c += 32) {
           float v[32], u[32];
@@ -467,14 +496,14 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
           ptx::tmem_ld_wait();
           if (live) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              float w[8];
+            for (int e = 0; e < 32; e += 16) {
+              float w[16];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
+              for (int j = 0; j < 16; ++j) {
                 w[j] = fmaf(-eps, u[e + j], v[e + j]) * scale;
                 finite = finite && fabsf(w[j]) < INFINITY;
               }
-              store8(dst + c + e, w);
+              store16(dst + c + e, w, wide_rows);
             }
           }
         }

@@ -276,10 +276,15 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
       ptx::tmem_ld_wait();
       const int k0 = k_base + n * TR;
       const int lo = live ? span.first - k0 : TR, hi = live ? t - k0 : -1;  // keys lo..hi of the block are seen
-      if (__any_sync(0xffffffffu, lo > 0 || hi < TR - 1)) {
+      if (__any_sync(0xffffffffu, hi < TR - 1)) {  // the diagonal (one comparison per score: hence the two branches)
 #pragma unroll
         for (int e = 0; e < TR; ++e)
-          if (e < lo || e > hi) sv[e] = -INFINITY;
+          if (e > hi) sv[e] = -INFINITY;
+      }
+      if (__any_sync(0xffffffffu, lo > 0)) {  // a sequence begins inside the block
+#pragma unroll
+        for (int e = 0; e < TR; ++e)
+          if (e < lo) sv[e] = -INFINITY;
       }
       float b0 = -INFINITY, b1 = -INFINITY, b2 = -INFINITY, b3 = -INFINITY;
 #pragma unroll
@@ -345,6 +350,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
     if (ok && g.last >= g.first) {
       ptx::tc_fence_after_sync();
       const float inv = 1.f / l;
+      const bool wide_rows = (a.ldo & 15) == 0 && aligned32(a.o);
       bf16* dst = (bf16*)a.o + (size_t)t * a.ldo + g.head * HS;
       bool finite = true;
 #pragma unroll 1
@@ -354,14 +360,21 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
         ptx::tmem_ld_wait();
         if (live) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            float w[8];
+          for (int e = 0; e < 32; e += 16) {
+            uint32_t w[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              w[j] = v[e + j] * inv;
-              finite = finite && fabsf(w[j]) < INFINITY;
+              const float x = v[e + 2 * j] * inv, y = v[e + 2 * j + 1] * inv;
+              finite = finite && fabsf(x) < INFINITY && fabsf(y) < INFINITY;
+              const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+              w[j] = *reinterpret_cast<const uint32_t*>(&h);
             }
-            store8(dst + c + e, w);
+            if (wide_rows) {  // a thread writes a row: whole 32-byte sectors at a time where the rows allow it
+              store32B(dst + c + e, w);
+            } else {
+              *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(dst + c + e + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+            }
           }
         }
       }
