@@ -127,6 +127,10 @@ __device__ __noinline__ void packed_fwd_row(const T* q, const T* k, const T* v, 
   if (lse && lane == 0) *lse = m + logf(l);
 }
 
+// The first row of a sequence sees one key: its softmax is the constant 1 and dS = P (dP - delta) is zero.  The backward
+// kernels say so themselves (`alone`), since dP and delta are sums in different orders and differ in their last bits.
+__device__ __forceinline__ bool alone(int first, int t) { return first == t; }
+
 template <typename T, int HS>
 __device__ __noinline__ void packed_dq_row(const T* q, const T* k, const T* v, const T* d_o, float lse, float delta, T* dq,
                                            int ldk, int ldv, int first, int t, float scale) {
@@ -135,9 +139,10 @@ __device__ __noinline__ void packed_dq_row(const T* q, const T* k, const T* v, c
   float acc[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  const float out_scale = alone(first, t) ? 0.f : scale;
   for (int u = first; u <= t; ++u) {
     const float p = exp_by_build(row_dot<T, HS>(q, k + (size_t)u * ldk) * scale - lse);
-    const float ds = p * (row_dot<T, HS>(d_o, v + (size_t)u * ldv) - delta) * scale;
+    const float ds = p * (row_dot<T, HS>(d_o, v + (size_t)u * ldv) - delta) * out_scale;
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (HS % 32 == 0 || lane + 32 * i < HS) acc[i] = fmaf(ds, to_f32(k[(size_t)u * ldk + lane + 32 * i]), acc[i]);
@@ -148,11 +153,11 @@ __device__ __noinline__ void packed_dq_row(const T* q, const T* k, const T* v, c
 }
 
 // Key row u of one key head: sums over the `group` query heads (head-major statistics with pitch `rows`) and the query
-// rows u .. last-1 of its sequence.
+// rows u .. last-1 of its sequence, which begins at row `first`.
 template <typename T, int HS>
 __device__ __noinline__ void packed_dkv_row(const T* q, const T* k, const T* v, const T* d_o, const float* lse,
                                             const float* delta, T* dk, T* dv, int ldq, int lddo, int rows, int group,
-                                            int u, int last, float scale) {
+                                            int u, int first, int last, float scale) {
   constexpr int N = (HS + 31) / 32;
   const int lane = threadIdx.x & 31;
   float ak[N], av[N];
@@ -164,7 +169,7 @@ __device__ __noinline__ void packed_dkv_row(const T* q, const T* k, const T* v, 
       const T* gr = d_o + (size_t)t * lddo + g * HS;
       const size_t st = (size_t)g * rows + t;
       const float p = exp_by_build(row_dot<T, HS>(qr, k) * scale - lse[st]);
-      const float ds = p * (row_dot<T, HS>(gr, v) - delta[st]) * scale;
+      const float ds = p * (row_dot<T, HS>(gr, v) - delta[st]) * (alone(first, t) ? 0.f : scale);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         if (HS % 32 == 0 || lane + 32 * i < HS) {

@@ -415,10 +415,12 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
         for (int e = 0; e < NC; ++e)
           if (e > hi) dp[e] = 0.f;
       }
-      if (cut_lo) {
+      if (cut_lo) {  // (holds where an `alone` row meets itself: there lo >= 0, and lo = 0 in lane 0 only, as blocks begin at
+                     // multiples of 32 rows from the warp's first)
+        const int from = lo + (MODE == MODE_DKV && alone(span.first, r) ? 1 : 0);
 #pragma unroll
         for (int e = 0; e < NC; ++e)
-          if (e < lo) dp[e] = 0.f;
+          if (e < from) dp[e] = 0.f;
       }
       if (MODE == MODE_DQ) {
         float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f);
@@ -488,6 +490,7 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
         if (live && hf == 0) a.delta[(size_t)head * f.rows + r] = delta;
         bf16* dst = (bf16*)a.dq + (size_t)r * a.lddq + head * HS;
         const bool wide_rows = (a.lddq & 15) == 0 && aligned32(a.dq);
+        const float out_scale = alone(span.first, r) ? 0.f : scale;
 #pragma unroll 1
         for (int c = hf * (HS / 2); c < (hf + 1) * (HS / 2); c += 32) {
           float v[32], u[32];
@@ -500,7 +503,7 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
               float w[16];
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
-                w[j] = fmaf(-eps, u[e + j], v[e + j]) * scale;
+                w[j] = fmaf(-eps, u[e + j], v[e + j]) * out_scale;
                 finite = finite && fabsf(w[j]) < INFINITY;
               }
               store16(dst + c + e, w, wide_rows);
@@ -525,7 +528,7 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
           packed_dkv_row<bf16, HS>((const bf16*)f.q + hk * group * HS, kr + (size_t)rr * f.ldk, vr + (size_t)rr * f.ldv,
                                    (const bf16*)a.d_o + hk * group * HS, f.lse + st, a.delta + st,
                                    (bf16*)a.dk + (size_t)rr * a.lddk + hk * HS, (bf16*)a.dv + (size_t)rr * a.lddv + hk * HS,
-                                   f.ldq, a.lddo, f.rows, group, rr, last, scale);
+                                   f.ldq, a.lddo, f.rows, group, rr, first, last, scale);
         } else {
           const float dl = __shfl_sync(0xffffffffu, delta, b);
           packed_dq_row<bf16, HS>((const bf16*)f.q + (size_t)rr * f.ldq + head * HS, kr, vr,

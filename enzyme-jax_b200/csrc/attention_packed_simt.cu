@@ -203,6 +203,7 @@ __global__ void __launch_bounds__(128) packed_dq_simt_kernel(PackedBwdArgs a, fl
   }
   const float lse = me.live ? f.lse[(size_t)h * f.rows + t] : 0.f;
   const float delta = me.live ? a.delta[(size_t)h * f.rows + t] : 0.f;
+  const float out_scale = alone(me.span.first, t) ? 0.f : scale;
   const int last = min(row0 + RB, hi);
   for (int u0 = lo; u0 < last; u0 += RB) {
     __syncthreads();
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(128) packed_dq_simt_kernel(PackedBwdArgs a, fl
       if (uu >= from && uu <= to) {
         const float p = exp_by_build(s * scale - lse);
         const float w = p * (dp - delta);
-        axpy_quarter(acc, w * scale, kq + uu * Q::kRow);
+        axpy_quarter(acc, w * out_scale, kq + uu * Q::kRow);
         if constexpr (kExact) {
           eps += w;
           axpy_quarter(pk, p, kq + uu * Q::kRow);
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(128) packed_dq_simt_kernel(PackedBwdArgs a, fl
   if (me.live) {
     T* dq = (T*)a.dq + (size_t)t * a.lddq + h * HS + part * DPT;
 #pragma unroll
-    for (int i = 0; i < DPT; ++i) dq[i] = from_f32<T>(kExact ? fmaf(-eps * scale, pk[i], acc[i]) : acc[i]);
+    for (int i = 0; i < DPT; ++i) dq[i] = from_f32<T>(kExact ? fmaf(-eps * out_scale, pk[i], acc[i]) : acc[i]);
     if (kExact && part == 0) a.delta[(size_t)h * f.rows + t] = delta + eps;
   }
 }
@@ -272,6 +273,7 @@ __global__ void __launch_bounds__(128) packed_dkv_simt_kernel(PackedBwdArgs a, f
       const float* qq = Qs + part * Q::kPitch;
       const float* gq = Gs + part * Q::kPitch;
       const int from = me.live ? u - t0 : RB, to = me.live ? me.span.last - t0 : 0;  // queries from..to-1 see this key
+      const int zero = alone(me.span.first, u) ? from : -1;
 #pragma unroll 4
       for (int tt = 0; tt < RB; ++tt) {
         const float s = dot_quarter(kr, qq + tt * Q::kRow);
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(128) packed_dkv_simt_kernel(PackedBwdArgs a, f
         if (tt >= from && tt < to) {
           const float p = exp_by_build(s * scale - Ls[tt]);
           axpy_quarter(av, p, gq + tt * Q::kRow);
-          axpy_quarter(ak, p * (dp - Ds[tt]) * scale, qq + tt * Q::kRow);
+          axpy_quarter(ak, p * (dp - Ds[tt]) * (tt == zero ? 0.f : scale), qq + tt * Q::kRow);
         }
       }
     }

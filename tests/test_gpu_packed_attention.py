@@ -204,6 +204,24 @@ def test_gradient_against_differences():
         assert abs(got - diff) <= float((bounds[i] * d.abs()).sum()) + 1e-6 * (1 + abs(diff))
 
 
+@pytest.mark.parametrize("impl", [0, 2])
+@pytest.mark.parametrize("lens", [[1] * 300, [1, 130, 1, 1, 63, 1, 200, 2, 1, 1]])
+@pytest.mark.parametrize("hs,dtype", [(64, torch.bfloat16), (128, torch.bfloat16), (48, torch.float32), (32, torch.bfloat16)])
+def test_a_row_that_sees_itself_alone(hs, dtype, lens, impl):
+    # its softmax is the constant 1: no gradient of its scores, not even a rounding error's
+    heads, kv_heads = 6, 2
+    q, k, v, d_o = make(lens, heads, kv_heads, hs, dtype, seed=12)
+    cu = cu_of(lens)
+    o, lse = B.attention_packed(q, k, v, cu, heads, kv_heads, impl=impl)
+    dq, dk, dv = B.attention_packed_backward(q, k, v, o, lse, d_o, cu, heads, kv_heads, impl=impl)
+    assert B.device_status() == 0
+    starts = cu[:-1].long()
+    assert not bool(dq[starts].any())
+    single = starts[torch.tensor(lens, device=DEV) == 1]
+    assert not bool(dk[single].any())
+    assert bool(dq.isfinite().all() and dk.isfinite().all() and dv.isfinite().all())
+
+
 @pytest.mark.parametrize("hs,dtype", [(64, torch.bfloat16), (128, torch.bfloat16), (48, torch.float32)])
 def test_repeats_to_the_bit(hs, dtype):
     lens, heads, kv = [300, 7, 129], 6, 2
