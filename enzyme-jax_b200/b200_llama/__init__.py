@@ -495,6 +495,8 @@ def kv4_read(codes: torch.Tensor, params: torch.Tensor, page_table: torch.Tensor
                      codes, params, page_table, cu_seqlens, ctx_before, k, v)
     n_pages, n_kv_heads, page_size, hs = _kv4_layer(what, codes, params)
     n_seqs = _kv4_rows(what, page_table, cu_seqlens, ctx_before)
+    if rows < 0:
+        raise B200Error(2, f"{what}: {rows} rows")
     k = torch.empty(rows, n_kv_heads * hs, dtype=dtype, device=dev) if k is None else k
     v = torch.empty(rows, n_kv_heads * hs, dtype=dtype, device=dev) if v is None else v
     ldk = _rows(what, "k", k, n_kv_heads * hs, rows, dtype)

@@ -293,13 +293,14 @@ template <typename T, int HS>
 __global__ void __launch_bounds__(SW * 32) kv4_decode_simt_kernel(Kv4DecodeArgs a) {
   constexpr int LPK = lanes_of(HS), KPW = 32 / LPK;
   extern __shared__ int32_t pre[];
+  int32_t* lens = pre + a.batch + 1;
   __shared__ int32_t warp_sums[SW];
   __shared__ float s_acc[SW][HS], s_m[SW], s_l[SW];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LPK, li = lane % LPK;
   const bool lane_on = li * 8 < HS;
   pdl_launch_dependents();
   pdl_wait();  // everything below comes from the kernels before
-  unit_prefix<SW * 32>(a, pre, warp_sums);
+  unit_prefix<SW * 32>(a, pre, lens, warp_sums);
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i <= a.batch; i += blockDim.x) a.prefix[i] = pre[i];
   const Kv4Pool& p = a.pool;
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(SW * 32) kv4_decode_simt_kernel(Kv4DecodeArgs 
     const long long s0 = base + (long long)seg * nb, s1 = s0 + nb;
     const long long x1 = r1 < s1 ? r1 : s1;
     const int hk = seg / a.subs, head = hk * a.subs + seg % a.subs;
-    const int len = kv4_len(a, b);
+    const int len = lens[b];
     const int c0 = (int)(x - s0) * kUnit, c1 = min(len, (int)(x1 - s0) * kUnit);
     const int32_t* table = p.table + (size_t)b * p.max_pages;
 
@@ -518,7 +519,8 @@ int32_t check_pool(const char* what, const Kv4Pool& p) {
 }
 int32_t check_pool_ptrs(const char* what, const Kv4Pool& p) {
   if (!p.codes || !p.params || !p.table) return fail(B200_ERR_INVALID_ARG, "%s: null operand", what);
-  if (!aligned16(p.codes) || !aligned16(p.params)) return fail(B200_ERR_MISALIGNED, "%s: codes and params must be 16-byte aligned", what);
+  if ((reinterpret_cast<uintptr_t>(p.codes) | reinterpret_cast<uintptr_t>(p.params)) & 3u)
+    return fail(B200_ERR_MISALIGNED, "%s: codes and params must be 4-byte aligned", what);
   return B200_OK;
 }
 
@@ -652,7 +654,10 @@ int32_t b200_attention_decode_kv4(const void* q, const void* codes, const void* 
   a.cols = mma ? std::min(8, group) : 1;
   a.subs = (group + a.cols - 1) / a.cols;
   const size_t es = dtype == B200_BF16 ? 2 : 4;
-  const long long units_per_seq = ((long long)max_pages * page_size + kUnit - 1) / kUnit * n_kv_heads * a.subs;
+  const long long cap_units = ((long long)max_pages * page_size + kUnit - 1) / kUnit;
+  if (cap_units * std::min(batch, kMaxSlice) > 0x7fffffffLL)
+    return fail(B200_ERR_BAD_SHAPE, "kv4 decode: %d page tables of %d pages of %d rows are too long together", batch, max_pages, page_size);
+  const long long units_per_seq = cap_units * n_kv_heads * a.subs;
   for (int b0 = 0; b0 < batch; b0 += kMaxSlice) {
     a.batch = std::min(kMaxSlice, batch - b0);
     a.q = (const char*)q + (size_t)b0 * ldq * es;
@@ -666,7 +671,7 @@ int32_t b200_attention_decode_kv4(const void* q, const void* codes, const void* 
       if (mma) {
         B200_TRY(launch_kv4_decode_mma(a, grid, s));
       } else {
-        B200_CUDA_OK(launch_pdl(kv4_decode_simt_kernel<T, HS>, dim3(grid), dim3(SW * 32), (a.batch + 1) * sizeof(int32_t), s, a));
+        B200_CUDA_OK(launch_pdl(kv4_decode_simt_kernel<T, HS>, dim3(grid), dim3(SW * 32), (2 * a.batch + 1) * sizeof(int32_t), s, a));
         B200_LAUNCH_OK("kv4_decode_simt_kernel");
       }
       B200_CUDA_OK(launch_pdl(kv4_join_kernel<T, HS>, dim3(a.batch * n_kv_heads * a.subs * a.cols), dim3(JW * 32), 0, s, a, grid));

@@ -54,13 +54,17 @@ __device__ __forceinline__ int kv4_len(const Kv4DecodeArgs& a, int b) {
 __device__ __forceinline__ long long range_start(long long units, int ctas, int c) { return units * c / ctas; }
 __device__ __forceinline__ int range_owner(long long units, int ctas, long long u) { return (int)(((u + 1) * ctas - 1) / units); }
 
-// Exclusive prefix of the sequences' unit counts into `pre` [batch + 1] (shared memory), by all threads of the block.
-template <int THREADS> __device__ __forceinline__ void unit_prefix(const Kv4DecodeArgs& a, int32_t* pre, int32_t* warp_sums) {
+// Exclusive prefix of the sequences' unit counts into `pre` [batch + 1] and their lengths into `lens` [batch] (shared
+// memory), by all threads of the block.
+template <int THREADS>
+__device__ __forceinline__ void unit_prefix(const Kv4DecodeArgs& a, int32_t* pre, int32_t* lens, int32_t* warp_sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int base = 0;
   for (int b0 = 0; b0 < a.batch; b0 += THREADS) {
     const int b = b0 + threadIdx.x;
-    const int mine = b < a.batch ? (kv4_len(a, b) + kUnit - 1) / kUnit : 0;
+    const int len = b < a.batch ? kv4_len(a, b) : 0;
+    const int mine = (int)(((unsigned)len + kUnit - 1) / kUnit);
+    if (b < a.batch) lens[b] = len;
     int inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

@@ -43,7 +43,7 @@ template <int HS> struct MCfg {
   static constexpr int kPrm = kUnit * 4;
   static constexpr int kStage = 2 * kCode + 2 * kPrm;  // key codes, value codes, key parameters, value parameters
   static constexpr int kBars = kStages * kStage;
-  static constexpr int kPre = kBars + 128;           // unit prefix of the batch
+  static constexpr int kPre = kBars + 128;           // unit prefix and lengths of the batch
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -108,6 +108,7 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBars);
   uint64_t* empty = full + kStages;
   int32_t* pre = reinterpret_cast<int32_t*>(smem + C::kPre);
+  int32_t* lens = pre + a.batch + 1;
   volatile uint32_t* abort_flag = &s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   pdl_launch_dependents();
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
     ptx::tma_prefetch_desc(&tm_codes);
   }
   pdl_wait();  // everything below comes from the kernels before
-  unit_prefix<M_THREADS>(a, pre, warp_sums);
+  unit_prefix<M_THREADS>(a, pre, lens, warp_sums);
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i <= a.batch; i += blockDim.x) a.prefix[i] = pre[i];
   const Kv4Pool& p = a.pool;
@@ -156,7 +157,7 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
       while ((long long)pre[b + 1] * nseg <= x) ++b;
       const int nb = pre[b + 1] - pre[b];
       const int off = (int)(x - (long long)pre[b] * nseg);
-      const int hk = off / nb / a.subs, len = kv4_len(a, b);
+      const int hk = off / nb / a.subs, len = lens[b];
       int n = nb - off % nb;  // units of this range that lie in the segment
       if (n > r1 - x) n = (int)(r1 - x);
       x += n;
@@ -196,6 +197,7 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
   } else {
     const int group = a.n_heads / p.n_kv_heads;
     const float sl2 = a.scale * 1.4426950408889634f;
+    const bool q_vec = (a.ldq & 7) == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15u) == 0;
     const uint32_t part_sel = g < 4 ? 0x7531u : 0x6420u;  // high bytes, low bytes
     // Row g of the key operand's first eight is key 4 (g / 2) + g % 2 of the sixteen, row g of its second eight the key two
     // further.  TMA swizzles the 16-byte chunks of a row: by row / 2 % 4 (rows of 64 bytes) or row / 4 % 2 (of 32).
@@ -222,7 +224,7 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
       const int hk = seg / a.subs, first_head = (seg % a.subs) * a.cols;
       const int n_cols = min(a.cols, group - first_head);
       const int head0 = hk * group + first_head;
-      const int c1 = kv4_len(a, b);
+      const int c1 = lens[b];
 
       // query fragments: column g; the elements of a lane's words, even codes and odd codes, high bytes and low bytes
       uint32_t qh[NS][KW][2], ql[NS][KW][2];
@@ -233,8 +235,18 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
         const bool on = col < n_cols;
         const bf16* q = (const bf16*)a.q + (size_t)b * a.ldq + (head0 + (on ? col : 0)) * HS + t * (HS / 4);
         float e[8 * KW], top = 0.f, qs = 0.f;
+        if (q_vec) {
 #pragma unroll
-        for (int i = 0; i < 8 * KW; ++i) e[i] = on ? to_f32(q[i]) : 0.f;
+          for (int i = 0; i < KW; ++i) {
+            float x[8];
+            load8(q + 8 * i, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[8 * i + j] = on ? x[j] : 0.f;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8 * KW; ++i) e[i] = on ? to_f32(q[i]) : 0.f;
+        }
 #pragma unroll
         for (int i = 0; i < 8 * KW; ++i) {
           qs += e[i];
@@ -496,13 +508,13 @@ template <int HS, int NS> int32_t launch_hs(const Kv4DecodeArgs& a, int grid, cu
   const int ps = a.pool.page_size;
   const int shift = (ps & (ps - 1)) == 0 ? __builtin_ctz((unsigned)ps) : -1;
   const int piece = std::min(kUnit, ps & -ps);  // rows of a unit that never cross a page: 16, 32, 64 or 128
-  const size_t smem = C::kPre + (size_t)(a.batch + 1) * sizeof(int32_t);
+  const size_t smem = C::kPre + (size_t)(2 * a.batch + 1) * sizeof(int32_t);
   auto kern = kv4_decode_mma_kernel<HS, NS>;
   CUtensorMap codes;
   B200_TRY(make_map_codes(&codes, a.pool, piece));
   static PerDeviceOnce attr_once;
   B200_TRY(attr_once.run([&](int&) -> int32_t {
-    B200_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(C::kPre + (kMaxSlice + 1) * sizeof(int32_t))));
+    B200_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(C::kPre + (2 * kMaxSlice + 1) * sizeof(int32_t))));
     return B200_OK;
   }));
   B200_CUDA_OK(launch_pdl(kern, dim3(grid), dim3(M_THREADS), smem, stream, codes, a, shift, piece));
@@ -514,6 +526,7 @@ template <int HS, int NS> int32_t launch_hs(const Kv4DecodeArgs& a, int grid, cu
 
 bool kv4_decode_mma_supports(const Kv4DecodeArgs& a) {
   return a.dtype == B200_BF16 && (a.pool.head_size == 64 || a.pool.head_size == 128) && a.pool.page_size % 16 == 0 &&
+         aligned16(a.pool.codes) && aligned16(a.pool.params) &&
          kv4_half(a.pool) > 0 && kv4_half(a.pool) <= 0x7fffffffu;  // rows are TMA coordinates
 }
 

@@ -196,6 +196,9 @@ DECODE = [  # lens, heads, kv_heads, hs, page, dtype
     ([90] * 70, 2, 1, 64, 16, torch.bfloat16),
     ([200, 33], 5, 1, 128, 20, torch.bfloat16),
     ([9000], 2, 2, 128, 64, torch.bfloat16),
+    ([300, 47], 4, 2, 128, 48, torch.bfloat16),
+    ([513, 96], 8, 8, 64, 96, torch.bfloat16),
+    ([1000, 256, 257], 7, 1, 128, 256, torch.bfloat16),
 ]
 
 
@@ -242,6 +245,24 @@ def test_decode_skips_pages_outside_the_pool(impl):
         b = B.attention_decode_kv4(q, codes, params, table, torch.tensor([same], dtype=torch.int32, device=DEV), heads, impl=impl)
         assert torch.equal(a, b)
     assert B.device_status() == 0
+
+
+def test_layers_of_odd_size():
+    """Pools whose layers are not a multiple of 16 bytes: the second layer begins anywhere on 4 bytes."""
+    hk, hs, page = 1, 16, 7
+    codes, params = B.new_kv4_pages(2, 3, hk, page, hs)
+    assert params[1].data_ptr() % 16
+    g = torch.Generator(device=DEV).manual_seed(1)
+    k, v = (torch.randn(9, hs, generator=g, device=DEV) for _ in range(2))
+    table = torch.tensor([[2, 0]], dtype=torch.int32, device=DEV)
+    B.kv4_append(k, v, codes[1], params[1], table, cu_of([9]))
+    q = torch.randn(1, 2 * hs, generator=g, device=DEV)
+    o = B.attention_decode_kv4(q, codes[1], params[1], table, torch.tensor([9], dtype=torch.int32, device=DEV), 2)
+    want, bound = decode_reference(q, codes[1], params[1], table, [9], 2)
+    assert bool(((o.double() - want).abs() <= bound).all())
+    assert bool((codes[0] == 0).all()) and B.device_status() == 0
+    with pytest.raises(B.B200Error):
+        B.kv4_read(codes[1], params[1], table, cu_of([9]), None, -1)
 
 
 def test_decode_many_sequences():

@@ -30,7 +30,7 @@ def test_kv4_refusals():
     app = lambda k=P, codes=P, table=P, n=1, rows=4, hk=2, hs=64, ldk=128, pages=4, page=16, width=2, dt=1: lib.b200_kv4_append(
         k, P, codes, P, table, P, None, n, rows, hk, hs, ldk, 128, pages, page, width, dt, None)
     assert app(k=None) == 1 and app(table=None) == 1 and app(hs=20) == 2 and app(page=0) == 2 and app(ldk=64) == 2
-    assert app(dt=5) == 3 and app(codes=ctypes.c_void_p(20)) == 4 and app(rows=0, k=None) == 0
+    assert app(dt=5) == 3 and app(codes=ctypes.c_void_p(18)) == 4 and app(rows=0, k=None) == 0
     dec = lambda q=P, scratch=P, nbytes=1 << 30, b=1, h=4, hk=2, hs=64, ldq=256, impl=0: lib.b200_attention_decode_kv4(
         q, P, P, P, P, P, scratch, nbytes, b, h, hk, hs, ldq, 256, 4, 16, 2, 1, impl, None)
     assert dec(q=None) == 1 and dec(h=3) == 2 and dec(ldq=8) == 2 and dec(b=-1) == 2 and dec(impl=9) == 1
