@@ -15,12 +15,15 @@
 //
 // Head size 64 streams blocks of 64 rows: S, dP and the accumulators are then 256 TMEM columns and 75 KB of shared memory,
 // two CTAs share an SM and one's set-up, waits and epilogue hide behind the other's products (8 x 1024 tokens, 12 heads:
-// 167 -> 146 us).  Head size 128 takes all 512 columns with blocks of 128 rows.
+// 167 us with one CTA and blocks of 128 rows, 129 us now).  Head size 128 takes all 512 columns with blocks of 128 rows.
 //
 // delta.  Taken from the output as rowsum(dO * o) it carries the rounding of o to bf16, which is not small beside
 // dP - delta where a row sees few keys.  The query pass therefore also sums eps = rowsum(P * (dP - delta0)) in fp32 and
 // acc0 = P K; dQ = (acc1 - eps * acc0) / sqrt(hs) is then the gradient for the exact delta = delta0 + eps, which it leaves
-// behind for the key pass.  A tile whose keys fit one block settles eps before it forms dS.
+// behind for the key pass.  A tile whose keys fit one block settles eps before it forms dS.  delta0 itself is summed in the
+// query pass from a TMA copy of o's rows (a kernel of its own for it read dO once more: 12 ragged documents 334 -> 329 us,
+// 8 x 1024 tokens at 12 heads 131 -> 129 us; loads by the threads in its place took 334 to 365 us, as their latency
+// stands before the first dS; L2 prefetches of the next CTA's tiles changed nothing).
 //
 // Bound: 8 products of 128 x 128 x hs per (query block, key block), of which 5 are the formula's; 512 cycles each at head
 // size 128, 1024 cycles of exponentials.  Rounding to bf16 happens to P, dS and the results; sums are fp32.  All waits
@@ -49,6 +52,8 @@ template <int HS> struct BCfg {
   static constexpr int kXSub = kBlock * 128;           // one [kBlock rows x 64 columns] sub-tile
   static constexpr int kXTile = kSubs * kXSub;         // streamed tile
   static constexpr int kX = 2 * kTile;
+  static constexpr int kOTiles = kTile / kXTile;       // stages, the last ones, that hold o's rows at first (DQ)
+  static constexpr int kO = kX + (NX - kOTiles) * kXTile;
   static constexpr int kStat = kX + NX * kXTile;  // 2 stages x {-lse2[kBlock], -delta[kBlock]} of the streamed queries (DKV)
   static constexpr int kBars = kStat + 2 * 1024;
   static constexpr int kSmem = kBars + 256;
@@ -123,8 +128,8 @@ struct OwnGeo {
 template <int HS, int MODE>
 __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
     packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmF0, const __grid_constant__ CUtensorMap tmF1,
-                         const __grid_constant__ CUtensorMap tmX0, const __grid_constant__ CUtensorMap tmX1, PackedBwdArgs a,
-                         float scale, uint32_t* status) {
+                         const __grid_constant__ CUtensorMap tmX0, const __grid_constant__ CUtensorMap tmX1,
+                         const __grid_constant__ CUtensorMap tmO, PackedBwdArgs a, float scale, uint32_t* status) {
   using C = BCfg<HS>;
   constexpr int BN = C::kBlock, NC = BN / 2;  // streamed rows per block; of them per softmax thread
   const PackedArgs& f = a.f;
@@ -140,6 +145,8 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
   uint64_t* ds_full = p_full + 1;       // dS stands in TMEM
   uint64_t* acc_done = ds_full + 1;     // the accumulators are complete
   uint64_t* met = acc_done + 1;         // the 256 softmax threads meet (a barrier whose wait is bounded too)
+  uint64_t* o_full = bars + 24;         // the rows of o landed (DQ)
+  uint64_t* o_done = bars + 25;         // they have been read
   OwnGeo* geo = reinterpret_cast<OwnGeo*>(bars + 20);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
   volatile uint32_t* abort_flag = tmem_slot + 1;
@@ -172,6 +179,8 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
     ptx::mbar_init(ds_full, 8);
     ptx::mbar_init(acc_done, 1);
     ptx::mbar_init(met, 256);
+    ptx::mbar_init(o_full, 1);
+    ptx::mbar_init(o_done, 8);
     ptx::fence_barrier_init();
     ptx::tma_prefetch_desc(&tmF0);
     ptx::tma_prefetch_desc(&tmF1);
@@ -183,6 +192,20 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
     ptx::tmem_relinquish();
   }
   pdl_wait();  // the operands come from the kernels before
+  if (threadIdx.x == 0 && !*abort_flag) {  // the fixed tiles do not wait for the look-up of the sequences
+    ptx::mbar_arrive_expect_tx(fix_full, 2 * C::kTile);
+#pragma unroll
+    for (int s = 0; s < C::kSubs; ++s) {
+      ptx::tma_load_2d(smem + s * BSUB, &tmF0, head * HS + 64 * s, own * BR, fix_full);
+      ptx::tma_load_2d(smem + C::kTile + s * BSUB, &tmF1, head * HS + 64 * s, own * BR, fix_full);
+    }
+    if (MODE == MODE_DQ) {
+      ptx::mbar_arrive_expect_tx(o_full, C::kTile);
+#pragma unroll
+      for (int s = 0; s < C::kSubs; ++s)
+        ptx::tma_load_2d(smem + C::kO + s * BSUB, &tmO, head * HS + 64 * s, own * BR, o_full);
+    }
+  }
   if (warp == 2) {
     const int cu_first = max(0, *(f.cu)), end = min(f.rows, *(f.cu + f.n_seqs));
     OwnGeo g;
@@ -211,23 +234,22 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
   const OwnGeo g = *geo;
   const int n_it = g.n_it;
 
-  if (aborted || n_it == 0) {
+  if (aborted) {
     // common exit below
-  } else if (warp == 0) {
-    if (lane == 0) {
-      ptx::mbar_arrive_expect_tx(fix_full, 2 * C::kTile);
-#pragma unroll
-      for (int s = 0; s < C::kSubs; ++s) {
-        ptx::tma_load_2d(smem + s * BSUB, &tmF0, head * HS + 64 * s, g.r0, fix_full);
-        ptx::tma_load_2d(smem + C::kTile + s * BSUB, &tmF1, head * HS + 64 * s, g.r0, fix_full);
-      }
+  } else if (n_it == 0) {
+    if (threadIdx.x == 0) {  // no copy outlives the CTA
+      ptx::mbar_wait(fix_full, 0, abort_flag, status, ST_PACKEDB_TIMEOUT);
+      if (MODE == MODE_DQ) ptx::mbar_wait(o_full, 0, abort_flag, status, ST_PACKEDB_TIMEOUT);
     }
+  } else if (warp == 0) {
     bool ok = true;
     for (int x = 0; x < 2 * n_it && ok; ++x) {
       const int st = x % NX, it = x >> 1;
       const int qh = MODE == MODE_DKV ? hk * group + it / g.per_head : head;
       const int row = g.x0 + (it % g.per_head) * BN;
       ok = ptx::mbar_wait_warp(&x_empty[st], ((uint32_t)(x / NX) & 1u) ^ 1u, abort_flag, status, ST_PACKEDB_TIMEOUT);
+      if (MODE == MODE_DQ && x < NX && st >= NX - C::kOTiles)
+        ok = ok && ptx::mbar_wait_warp(o_done, 0, abort_flag, status, ST_PACKEDB_TIMEOUT);
       if (!ok) break;
       if (lane == 0) {
         const int col = (MODE == MODE_DKV ? qh : hk) * HS;
@@ -326,11 +348,7 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
     const RowSpan span = row_span(f.cu, f.n_seqs, s, r, f.rows);
     const bool live = span.first <= r;
     float lse2 = 0.f, delta = 0.f, eps = 0.f;
-    if (MODE == MODE_DQ && live) {
-      lse2 = f.lse[(size_t)head * f.rows + r] * 1.4426950408889634f;
-      delta = a.delta[(size_t)head * f.rows + r];
-    }
-    float* share = reinterpret_cast<float*>(smem + C::kStat);  // DQ: [2][128] halves of eps
+    float* share = reinterpret_cast<float*>(smem + C::kStat);  // DQ: [2][128] halves of eps, behind them of delta0
     bool ok = true;
     uint32_t met_phase = 0u;
     auto meet = [&]() {
@@ -339,7 +357,27 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
       met_phase ^= 1u;
       return ok;
     };
-    for (int it = 0; it < n_it; ++it) {
+    if (MODE == MODE_DQ) {  // delta0 = dO.o, half a row per thread, beside the first products
+      if (live) lse2 = f.lse[(size_t)head * f.rows + r] * 1.4426950408889634f;
+      ok = ptx::mbar_wait_warp(fix_full, 0, abort_flag, status, ST_PACKEDB_TIMEOUT) &&
+           ptx::mbar_wait_warp(o_full, 0, abort_flag, status, ST_PACKEDB_TIMEOUT);
+      const uint8_t* po = smem + (C::kSubs == 2 ? hf * BSUB : 0) + row * 128;
+#pragma unroll
+      for (int c = 0; c < HS / 16; ++c) {
+        const int at = ((C::kSubs == 2 ? c : hf * 4 + c) ^ (row & 7)) << 4;  // the 128-byte swizzle of a tile's row
+        float x[8], y[8];
+        load8(reinterpret_cast<const bf16*>(po + C::kO + at), x);
+        load8(reinterpret_cast<const bf16*>(po + C::kTile + at), y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) delta = fmaf(x[i], y[i], delta);
+      }
+      share[2 * BR + hf * BR + row] = delta;
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(o_done);
+      ok = ok && meet();
+      delta = live ? delta + share[2 * BR + (hf ^ 1) * BR + row] : 0.f;
+    }
+    for (int it = 0; it < n_it && ok; ++it) {
       const uint32_t ph = (uint32_t)it & 1u;
       const int c0 = g.x0 + (it % g.per_head) * BN + hf * NC;  // streamed row of this thread's first column
       // columns lo..hi of the NC form a pair with the own row
@@ -550,27 +588,6 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
   }
 }
 
-// delta0[h, t] = rowsum(dO * o): HS/8 lanes share a row, 16 bytes each.
-template <int HS>
-__global__ void __launch_bounds__(256) packed_delta_vec_kernel(PackedBwdArgs a) {
-  constexpr int L = HS / 8;
-  const PackedArgs& f = a.f;
-  const long long item = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
-  const int li = threadIdx.x % L;
-  const long long items = (long long)f.rows * f.n_heads;
-  const int t = item < items ? (int)(item / f.n_heads) : 0, h = item < items ? (int)(item % f.n_heads) : 0;
-  pdl_launch_dependents();
-  pdl_wait();
-  float x[8], y[8], s = 0.f;
-  load8((const bf16*)f.o + (size_t)t * f.ldo + h * HS + li * 8, x);
-  load8((const bf16*)a.d_o + (size_t)t * a.lddo + h * HS + li * 8, y);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s = fmaf(x[i], y[i], s);
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (item < items && li == 0) a.delta[(size_t)h * f.rows + t] = s;
-}
-
 template <int HS>
 int32_t launch_hs(const PackedBwdArgs& a, cudaStream_t stream) {
   using C = BCfg<HS>;
@@ -585,6 +602,8 @@ int32_t launch_hs(const PackedBwdArgs& a, cudaStream_t stream) {
   B200_TRY(make_map_2d(&xk, f.k, f.rows, f.n_kv_heads * HS, f.ldk, C::kBlock));
   B200_TRY(make_map_2d(&xv, f.v, f.rows, f.n_kv_heads * HS, f.ldv, C::kBlock));
   B200_TRY(make_map_2d(&xdo, a.d_o, f.rows, f.n_heads * HS, a.lddo, C::kBlock));
+  CUtensorMap fo;
+  B200_TRY(make_map_2d(&fo, f.o, f.rows, f.n_heads * HS, f.ldo, BR));
   auto dq = packed_bwd_tc_kernel<HS, MODE_DQ>;
   auto dkv = packed_bwd_tc_kernel<HS, MODE_DKV>;
   static PerDeviceOnce attr_once;
@@ -596,15 +615,12 @@ int32_t launch_hs(const PackedBwdArgs& a, cudaStream_t stream) {
   uint32_t* status = device_status_word();
   if (!status) return fail(B200_ERR_CUDA, "no device status word");
   const float scale = 1.f / sqrtf((float)HS);
-  const long long lanes = (long long)f.rows * f.n_heads * (HS / 8);
-  B200_CUDA_OK(launch_pdl(packed_delta_vec_kernel<HS>, dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, stream, a));
-  B200_LAUNCH_OK("packed_delta_vec_kernel");
   const unsigned blocks = (unsigned)cdiv(f.rows, BR);
-  B200_CUDA_OK(launch_pdl(dq, dim3(f.n_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, fq, fdo, xk, xv, a, scale,
-                          status));
+  B200_CUDA_OK(launch_pdl(dq, dim3(f.n_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, fq, fdo, xk, xv, fo, a,
+                          scale, status));
   B200_LAUNCH_OK("packed_bwd_tc_kernel<dq>");
-  B200_CUDA_OK(launch_pdl(dkv, dim3(f.n_kv_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, fk, fv, xq, xdo, a, scale,
-                          status));
+  B200_CUDA_OK(launch_pdl(dkv, dim3(f.n_kv_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, fk, fv, xq, xdo, fo, a,
+                          scale, status));
   B200_LAUNCH_OK("packed_bwd_tc_kernel<dkv>");
   return B200_OK;
 }
@@ -616,8 +632,7 @@ bool packed_bwd_tc_supports(const PackedBwdArgs& a) {
   return f.dtype == B200_BF16 && (f.head_size == 64 || f.head_size == 128) && f.ldq % 8 == 0 && f.ldk % 8 == 0 &&
          f.ldv % 8 == 0 && f.ldo % 8 == 0 && a.lddo % 8 == 0 && a.lddq % 8 == 0 && a.lddk % 8 == 0 && a.lddv % 8 == 0 &&
          aligned16(f.q) && aligned16(f.k) && aligned16(f.v) && aligned16(f.o) && aligned16(a.d_o) && aligned16(a.dq) &&
-         aligned16(a.dk) && aligned16(a.dv) && cdiv(f.rows, BR) <= 65535 &&
-         (long long)f.rows * f.n_heads * (f.head_size / 8) / 256 < 0x7fffffffLL;
+         aligned16(a.dk) && aligned16(a.dv) && cdiv(f.rows, BR) <= 65535;
 }
 
 int32_t launch_packed_bwd_tc(const PackedBwdArgs& a, cudaStream_t stream) {
