@@ -41,7 +41,7 @@ EXPORTS = (
     "b200_static_sizes", "b200_jvp_workspace_bytes", "b200_forward_jvp", "b200_token_jvp_workspace_bytes",
     "b200_token_jvp", "b200_plan_set_option", "b200_plan_get_option", "b200_attention_packed",
     "b200_attention_packed_backward", "b200_kv4_append", "b200_kv4_read", "b200_attention_decode_kv4_scratch_bytes",
-    "b200_attention_decode_kv4", "b200_copy_pages",
+    "b200_attention_decode_kv4_scratch_bytes_for", "b200_attention_decode_kv4", "b200_copy_pages",
 )
 
 
@@ -139,6 +139,7 @@ def lib() -> ctypes.CDLL:
         l.b200_kv4_append.argtypes = [c_void_p] * 7 + [c_int32] * 10 + [c_void_p]
         l.b200_kv4_read.argtypes = [c_void_p] * 7 + [c_int32] * 10 + [c_void_p]
         l.b200_attention_decode_kv4_scratch_bytes.argtypes = [c_int32] * 4 + [POINTER(c_size_t)]
+        l.b200_attention_decode_kv4_scratch_bytes_for.argtypes = [c_int32] * 7 + [POINTER(c_size_t)]
         l.b200_attention_decode_kv4.argtypes = [c_void_p] * 7 + [c_size_t] + [c_int32] * 11 + [c_void_p]
         l.b200_copy_pages.argtypes = [c_void_p] + [c_int32] * 5 + [c_void_p] * 3 + [c_int32, c_void_p, ctypes.c_int64,
                                                                                   c_void_p, c_void_p]
@@ -446,11 +447,13 @@ def new_kv4_pages(n_layers: int, n_pages: int, n_kv_heads: int, page_size: int, 
 
 
 def _kv4_layer(what: str, codes: torch.Tensor, params: torch.Tensor):
-    if codes.dim() != 5 or codes.shape[0] != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous():
+    shape = codes.shape
+    if len(shape) != 5 or shape[0] != 2 or codes.dtype is not torch.uint8 or not codes.is_contiguous():
         raise B200Error(2, f"{what}: codes must be a contiguous uint8 [2, n_pages, n_kv_heads, page_size, hs/2]")
-    if params.dtype != torch.bfloat16 or params.shape != codes.shape[:4] + (2,) or not params.is_contiguous():
-        raise B200Error(2, f"{what}: params must be a contiguous bf16 {tuple(codes.shape[:4]) + (2,)}")
-    _, n_pages, n_kv_heads, page_size, half = codes.shape
+    _, n_pages, n_kv_heads, page_size, half = shape
+    want = (2, n_pages, n_kv_heads, page_size, 2)
+    if params.dtype is not torch.bfloat16 or params.shape != want or not params.is_contiguous():
+        raise B200Error(2, f"{what}: params must be a contiguous bf16 {want}")
     return n_pages, n_kv_heads, page_size, 2 * half
 
 
@@ -508,9 +511,9 @@ def kv4_read(codes: torch.Tensor, params: torch.Tensor, page_table: torch.Tensor
 
 
 @functools.lru_cache(maxsize=256)
-def _kv4_scratch_bytes(batch: int, n_heads: int, n_kv_heads: int, hs: int) -> int:
+def _kv4_scratch_bytes(*sizes: int) -> int:
     n = c_size_t(0)
-    check(lib().b200_attention_decode_kv4_scratch_bytes(batch, n_heads, n_kv_heads, hs, byref(n)))
+    check(lib().b200_attention_decode_kv4_scratch_bytes_for(*sizes, byref(n)))
     return n.value
 
 
@@ -536,12 +539,17 @@ def attention_decode_kv4(q: torch.Tensor, codes: torch.Tensor, params: torch.Ten
     if out is None:
         out = torch.empty(batch, n_heads * hs, dtype=q.dtype, device=dev)
     ldo = _rows(what, "out", out, n_heads * hs, batch, q.dtype)
+    max_pages, dt = page_table.shape[1], _dt(q.dtype)
     if scratch is None:
-        scratch = torch.empty(_kv4_scratch_bytes(batch, n_heads, n_kv_heads, hs), dtype=torch.uint8, device=dev)
+        size, at = _kv4_scratch_bytes(batch, n_heads, n_kv_heads, hs, page_size, max_pages, dt), None
+        if size:
+            scratch = torch.empty(size, dtype=torch.uint8, device=dev)
+            at = scratch.data_ptr()
+    else:
+        size, at = scratch.numel() * scratch.element_size(), scratch.data_ptr()
     _call(dev, lib().b200_attention_decode_kv4, q.data_ptr(), codes.data_ptr(), params.data_ptr(),
-          page_table.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), scratch.data_ptr(),
-          scratch.numel() * scratch.element_size(), batch, n_heads, n_kv_heads, hs, ldq, ldo, n_pages, page_size,
-          page_table.shape[1], _dt(q.dtype), impl)
+          page_table.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), at, size, batch, n_heads, n_kv_heads, hs, ldq,
+          ldo, n_pages, page_size, max_pages, dt, impl)
     return out
 
 

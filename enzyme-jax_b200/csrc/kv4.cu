@@ -300,18 +300,17 @@ __global__ void __launch_bounds__(SW * 32) kv4_decode_simt_kernel(Kv4DecodeArgs 
   const bool lane_on = li * 8 < HS;
   pdl_launch_dependents();
   pdl_wait();  // everything below comes from the kernels before
-  unit_prefix<SW * 32>(a, pre, lens, warp_sums);
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i <= a.batch; i += blockDim.x) a.prefix[i] = pre[i];
+  const UnitRange range = unit_range<SW * 32>(a, pre, lens, warp_sums);
   const Kv4Pool& p = a.pool;
   const int nseg = p.n_kv_heads * a.subs;
-  const long long units = (long long)pre[a.batch] * nseg;
-  const int ctas = (int)(units < (long long)gridDim.x ? units : (long long)gridDim.x);
-  if ((int)blockIdx.x >= ctas) return;
-  const long long r0 = range_start(units, ctas, blockIdx.x), r1 = range_start(units, ctas, blockIdx.x + 1);
+  const long long r0 = range.first, r1 = range.last;
+  if (r0 == r1) {
+    if (a.whole) zero_segment<T>(a);
+    return;
+  }
   const uint32_t* codes = reinterpret_cast<const uint32_t*>(p.codes);
   const size_t half = kv4_half(p);
-  int b = 0;
+  int b = range.seq;
   for (long long x = r0; x < r1;) {
     while ((long long)pre[b + 1] * nseg <= x) ++b;
     const int nb = pre[b + 1] - pre[b];
@@ -528,7 +527,39 @@ int32_t check_pool_ptrs(const char* what, const Kv4Pool& p) {
 // long sequence fills the GPU too).
 int decode_simt_grid() { return 7 * sm_count(); }
 
-size_t partial_floats(int ctas, int cols, int head_size) { return (size_t)2 * ctas * cols * (head_size + 2); }
+long long table_units(int page_size, int max_pages) { return ((long long)max_pages * page_size + kUnit - 1) / kUnit; }
+
+// (by what the kernels are made for: a tensor-core shape that another alignment sends to the CUDA cores counts as one)
+int whole_units(int dtype, int head_size, int page_size) {
+  return dtype == B200_BF16 && (head_size == 64 || head_size == 128) && page_size % 16 == 0 ? kWholeUnitsMma : kWholeUnitsSimt;
+}
+
+// How a step is shared out: CTAs of either kernel, segments whole or not, scratch.
+struct DecodePlan {
+  int mma_cols, mma_subs, mma_grid, simt_grid;
+  bool whole;
+  size_t prefix_bytes, bytes;
+};
+DecodePlan decode_plan(int batch, int n_heads, int n_kv_heads, int head_size, long long cap_units, int whole_units) {
+  DecodePlan p;
+  const int group = n_heads / n_kv_heads;
+  const long long slice = std::min(batch, kMaxSlice);
+  p.mma_cols = std::min(8, group);
+  p.mma_subs = (group + p.mma_cols - 1) / p.mma_cols;
+  const long long mma_segs = slice * n_kv_heads * p.mma_subs, simt_segs = slice * n_heads;
+  const long long mma_max = kv4_decode_mma_grid(head_size, p.mma_cols), simt_max = decode_simt_grid();
+  p.whole = cap_units <= whole_units && mma_segs <= mma_max && simt_segs <= simt_max;
+  p.mma_grid = (int)std::max(1LL, std::min(mma_max, mma_segs * cap_units));
+  p.simt_grid = (int)std::max(1LL, std::min(simt_max, simt_segs * cap_units));
+  const size_t slots = std::max((size_t)p.simt_grid, (size_t)p.mma_grid * p.mma_cols);
+  p.prefix_bytes = align_up((size_t)(slice + 1) * 4, 256);
+  p.bytes = p.prefix_bytes + 2 * slots * (head_size + 2) * sizeof(float);
+  if (p.whole) {
+    p.mma_grid = (int)mma_segs;
+    p.simt_grid = (int)simt_segs;
+  }
+  return p;
+}
 
 }  // namespace
 
@@ -610,9 +641,18 @@ int32_t b200_attention_decode_kv4_scratch_bytes(int32_t batch, int32_t n_heads, 
   if (!bytes) return fail(B200_ERR_INVALID_ARG, "bytes is null");
   if (batch < 0 || n_heads <= 0 || n_kv_heads <= 0 || head_size <= 0 || n_heads % n_kv_heads)
     return fail(B200_ERR_BAD_SHAPE, "kv4 decode: batch=%d heads=%d kv_heads=%d head_size=%d", batch, n_heads, n_kv_heads, head_size);
-  const int cols = std::min(8, n_heads / n_kv_heads);
-  const size_t floats = std::max(partial_floats(decode_simt_grid(), 1, head_size), partial_floats(kv4_decode_mma_grid(head_size, cols), cols, head_size));
-  *bytes = align_up(((size_t)std::min(batch, kMaxSlice) + 1) * 4, 256) + floats * 4;
+  *bytes = decode_plan(batch, n_heads, n_kv_heads, head_size, 0x7fffffffLL, 0).bytes;
+  return B200_OK;
+}
+
+int32_t b200_attention_decode_kv4_scratch_bytes_for(int32_t batch, int32_t n_heads, int32_t n_kv_heads, int32_t head_size,
+                                                    int32_t page_size, int32_t max_pages, int32_t dtype, size_t* bytes) {
+  if (!bytes) return fail(B200_ERR_INVALID_ARG, "bytes is null");
+  if (batch < 0 || n_heads <= 0 || n_kv_heads <= 0 || head_size <= 0 || n_heads % n_kv_heads || page_size <= 0 || max_pages < 0)
+    return fail(B200_ERR_BAD_SHAPE, "kv4 decode: batch=%d heads=%d kv_heads=%d head_size=%d, %d pages of %d rows", batch, n_heads,
+                n_kv_heads, head_size, max_pages, page_size);
+  const DecodePlan plan = decode_plan(batch, n_heads, n_kv_heads, head_size, table_units(page_size, max_pages), whole_units(dtype, head_size, page_size));
+  *bytes = plan.whole ? 0 : plan.bytes;
   return B200_OK;
 }
 
@@ -634,37 +674,36 @@ int32_t b200_attention_decode_kv4(const void* q, const void* codes, const void* 
   if (dtype != B200_F32 && dtype != B200_BF16) return fail(B200_ERR_BAD_DTYPE, "kv4 decode: unsupported dtype %d", dtype);
   if (impl < 0 || impl > 2) return fail(B200_ERR_INVALID_ARG, "impl %d is not 0, 1 or 2", impl);
   if (batch == 0) return B200_OK;
-  if (!q || !o || !ctx_lens || !scratch) return fail(B200_ERR_INVALID_ARG, "kv4 decode: null operand");
+  const long long cap_units = table_units(page_size, max_pages);
+  if (cap_units * std::min(batch, kMaxSlice) > 0x7fffffffLL)
+    return fail(B200_ERR_BAD_SHAPE, "kv4 decode: %d page tables of %d pages of %d rows are too long together", batch, max_pages, page_size);
+  const DecodePlan plan = decode_plan(batch, n_heads, n_kv_heads, head_size, cap_units, whole_units(dtype, head_size, page_size));
+  if (!q || !o || !ctx_lens || (!scratch && !plan.whole)) return fail(B200_ERR_INVALID_ARG, "kv4 decode: null operand");
   B200_TRY(check_pool_ptrs("kv4 decode", a.pool));
   if (!aligned16(scratch)) return fail(B200_ERR_MISALIGNED, "kv4 decode: scratch must be 16-byte aligned");
-  size_t need = 0;
-  B200_TRY(b200_attention_decode_kv4_scratch_bytes(batch, n_heads, n_kv_heads, head_size, &need));
-  if (scratch_bytes < need) return fail(B200_ERR_WORKSPACE, "kv4 decode: scratch needs %zu bytes, %zu given", need, scratch_bytes);
+  if (scratch && scratch_bytes < plan.bytes)
+    return fail(B200_ERR_WORKSPACE, "kv4 decode: scratch needs %zu bytes, %zu given", plan.bytes, scratch_bytes);
   a.status = device_status_word();
   if (!a.status) return fail(B200_ERR_CUDA, "no device status word");
   a.n_heads = n_heads; a.ldq = ldq; a.ldo = ldo; a.dtype = dtype;
   a.scale = 1.f / sqrtf((float)head_size);
   a.prefix = (int32_t*)scratch;
-  a.partials = (float*)((char*)scratch + align_up(((size_t)std::min(batch, kMaxSlice) + 1) * 4, 256));
+  a.partials = (float*)((char*)scratch + plan.prefix_bytes);
+  a.whole = plan.whole;
   const bool mma = impl != 2 && kv4_decode_mma_supports(a);
   if (impl == 1 && !mma)
     return fail(B200_ERR_UNSUPPORTED, "kv4 decode on tensor cores needs bf16, head size 64 or 128 and pages of a multiple of 16 rows");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int group = n_heads / n_kv_heads;
-  a.cols = mma ? std::min(8, group) : 1;
-  a.subs = (group + a.cols - 1) / a.cols;
+  a.cols = mma ? plan.mma_cols : 1;
+  a.subs = mma ? plan.mma_subs : n_heads / n_kv_heads;
+  const int grid = mma ? plan.mma_grid : plan.simt_grid;  // (of a full slice: CTAs without work return)
   const size_t es = dtype == B200_BF16 ? 2 : 4;
-  const long long cap_units = ((long long)max_pages * page_size + kUnit - 1) / kUnit;
-  if (cap_units * std::min(batch, kMaxSlice) > 0x7fffffffLL)
-    return fail(B200_ERR_BAD_SHAPE, "kv4 decode: %d page tables of %d pages of %d rows are too long together", batch, max_pages, page_size);
-  const long long units_per_seq = cap_units * n_kv_heads * a.subs;
   for (int b0 = 0; b0 < batch; b0 += kMaxSlice) {
     a.batch = std::min(kMaxSlice, batch - b0);
     a.q = (const char*)q + (size_t)b0 * ldq * es;
     a.o = (char*)o + (size_t)b0 * ldo * es;
     a.ctx = ctx_lens + b0;
     a.pool.table = page_table + (size_t)b0 * max_pages;
-    const int grid = (int)std::max(1LL, std::min<long long>(mma ? kv4_decode_mma_grid(head_size, a.cols) : decode_simt_grid(), units_per_seq * a.batch));
     B200_TRY(by_type("kv4 decode", dtype, head_size, [&](auto t, auto hs) -> int32_t {
       using T = decltype(t);
       constexpr int HS = decltype(hs)::value;
@@ -674,6 +713,7 @@ int32_t b200_attention_decode_kv4(const void* q, const void* codes, const void* 
         B200_CUDA_OK(launch_pdl(kv4_decode_simt_kernel<T, HS>, dim3(grid), dim3(SW * 32), (2 * a.batch + 1) * sizeof(int32_t), s, a));
         B200_LAUNCH_OK("kv4_decode_simt_kernel");
       }
+      if (plan.whole) return B200_OK;
       B200_CUDA_OK(launch_pdl(kv4_join_kernel<T, HS>, dim3(a.batch * n_kv_heads * a.subs * a.cols), dim3(JW * 32), 0, s, a, grid));
       B200_LAUNCH_OK("kv4_join_kernel");
       return B200_OK;

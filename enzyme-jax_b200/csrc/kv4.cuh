@@ -33,6 +33,7 @@ struct Kv4DecodeArgs {
   int32_t* prefix = nullptr;       // [batch + 1]
   uint32_t* status = nullptr;
   int batch = 0, n_heads = 0, ldq = 0, ldo = 0, dtype = B200_BF16;
+  bool whole = false;              // one CTA per segment, no partials
   int subs = 1;                    // head subsets per key head: segments of a sequence are (key head, subset)
   int cols = 1;                    // query heads per subset (the last one may hold fewer)
   float scale = 1.f;
@@ -51,8 +52,15 @@ __device__ __forceinline__ int kv4_len(const Kv4DecodeArgs& a, int b) {
   const int n = *(a.ctx + b);
   return n <= 0 ? 0 : (n < cap ? n : (int)cap);
 }
+__device__ __forceinline__ int units_of(int len) { return (int)(((unsigned)len + kUnit - 1) / kUnit); }
 __device__ __forceinline__ long long range_start(long long units, int ctas, int c) { return units * c / ctas; }
 __device__ __forceinline__ int range_owner(long long units, int ctas, long long u) { return (int)(((u + 1) * ctas - 1) / units); }
+
+// Short tables, few segments: CTA i takes the whole of segment i (`whole`), which needs neither scratch nor a second kernel.
+// Up to this many units per segment, as long as every segment has a resident CTA.  Device time at 32/8 heads of 128, whole
+// against split and joined: 500 rows 8.2 / 8.8 us (1 sequence), 10.9 / 15.7 (16); 1000 rows 11.6 / 9.1 (1), 16.2 / 18.4 (16);
+// on the CUDA cores (6 fp32 heads of 48): 250 rows 8.3 / 8.4, 500 rows 13.9 / 8.4.  The call on the host takes 12 / 16 us.
+constexpr int kWholeUnitsMma = 4, kWholeUnitsSimt = 2;
 
 // Exclusive prefix of the sequences' unit counts into `pre` [batch + 1] and their lengths into `lens` [batch] (shared
 // memory), by all threads of the block.
@@ -63,7 +71,7 @@ __device__ __forceinline__ void unit_prefix(const Kv4DecodeArgs& a, int32_t* pre
   for (int b0 = 0; b0 < a.batch; b0 += THREADS) {
     const int b = b0 + threadIdx.x;
     const int len = b < a.batch ? kv4_len(a, b) : 0;
-    const int mine = (int)(((unsigned)len + kUnit - 1) / kUnit);
+    const int mine = units_of(len);
     if (b < a.batch) lens[b] = len;
     int inc = mine;
 #pragma unroll
@@ -85,6 +93,40 @@ __device__ __forceinline__ void unit_prefix(const Kv4DecodeArgs& a, int32_t* pre
   }
   if (threadIdx.x == 0) pre[a.batch] = base;
   __syncthreads();
+}
+
+// The CTA's range of units and the sequence it begins in; `ctas`: CTAs with work.
+struct UnitRange { long long first, last; int seq; };
+template <int THREADS>
+__device__ __forceinline__ UnitRange unit_range(const Kv4DecodeArgs& a, int32_t* pre, int32_t* lens, int32_t* warp_sums) {
+  const int nseg = a.pool.n_kv_heads * a.subs;
+  if (a.whole) {
+    const int b = (int)blockIdx.x / nseg, seg = (int)blockIdx.x % nseg, len = kv4_len(a, b), nb = units_of(len);
+    if (threadIdx.x == 0) {
+      pre[b] = 0;
+      pre[b + 1] = nb;
+      lens[b] = len;
+    }
+    __syncthreads();
+    return {(long long)seg * nb, (long long)(seg + 1) * nb, b};
+  }
+  unit_prefix<THREADS>(a, pre, lens, warp_sums);
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i <= a.batch; i += blockDim.x) a.prefix[i] = pre[i];
+  const long long units = (long long)pre[a.batch] * nseg;
+  const int ctas = (int)(units < (long long)gridDim.x ? units : (long long)gridDim.x);
+  if ((int)blockIdx.x >= ctas) return {0, 0, 0};
+  return {range_start(units, ctas, blockIdx.x), range_start(units, ctas, blockIdx.x + 1), 0};
+}
+
+// `whole` and a sequence without rows: zeros.
+template <typename T> __device__ __forceinline__ void zero_segment(const Kv4DecodeArgs& a) {
+  const int nseg = a.pool.n_kv_heads * a.subs, hs = a.pool.head_size;
+  const int b = (int)blockIdx.x / nseg, seg = (int)blockIdx.x % nseg;
+  const int group = a.n_heads / a.pool.n_kv_heads, first = (seg % a.subs) * a.cols;
+  const int n = min(a.cols, group - first) * hs;
+  T* o = (T*)a.o + (size_t)b * a.ldo + (size_t)((seg / a.subs) * group + first) * hs;
+  for (int e = threadIdx.x; e < n; e += blockDim.x) o[e] = from_f32<T>(0.f);
 }
 
 bool kv4_decode_mma_supports(const Kv4DecodeArgs& a);

@@ -126,17 +126,16 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
     ptx::tma_prefetch_desc(&tm_codes);
   }
   pdl_wait();  // everything below comes from the kernels before
-  unit_prefix<M_THREADS>(a, pre, lens, warp_sums);
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i <= a.batch; i += blockDim.x) a.prefix[i] = pre[i];
+  const UnitRange range = unit_range<M_THREADS>(a, pre, lens, warp_sums);
   const Kv4Pool& p = a.pool;
   const int nseg = p.n_kv_heads * a.subs;
-  const long long units = (long long)pre[a.batch] * nseg;
-  const int ctas = (int)(units < (long long)gridDim.x ? units : (long long)gridDim.x);
-  if ((int)blockIdx.x >= ctas || s_abort) return;
-  const long long r0 = range_start(units, ctas, blockIdx.x), r1 = range_start(units, ctas, blockIdx.x + 1);
+  const long long r0 = range.first, r1 = range.last;
+  if (r0 == r1 || s_abort) {
+    if (a.whole) zero_segment<bf16>(a);
+    return;
+  }
   const size_t half = kv4_half(p);
-  int b = 0;
+  int b = range.seq;
   int st = 0;  // stage and phase of the next unit
   uint32_t phase = 0u;
   auto next_stage = [&]() {

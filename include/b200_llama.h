@@ -424,10 +424,14 @@ B200_API int32_t b200_kv4_read(void* k, void* v, const void* codes, const void* 
 /* Decode attention over the 4-bit cache: one query row per sequence against its first ctx_lens[b] cached rows (int32
  * [batch] on the device, cut to max_pages * page_size; a sequence without rows gets zeros), grouped heads as above.
  * q, o [batch, ldq / ldo] of `dtype`.  scratch: b200_attention_decode_kv4_scratch_bytes() bytes, 16-byte aligned, used by
- * this call alone while it runs.  Pages outside the pool are skipped and reported as above.  impl: 0 = pick, 1 = tensor
+ * this call alone while it runs; b200_attention_decode_kv4_scratch_bytes_for() says how much of that a call with these page
+ * tables needs, and 0 where the tables are so short that scratch may be NULL.  Pages outside the pool are skipped and reported as above.  impl: 0 = pick, 1 = tensor
  * cores (bf16, head size 64 or 128, page_size a multiple of 16), 2 = CUDA cores. */
 B200_API int32_t b200_attention_decode_kv4_scratch_bytes(int32_t batch, int32_t n_heads, int32_t n_kv_heads,
                                                          int32_t head_size, size_t* bytes);
+B200_API int32_t b200_attention_decode_kv4_scratch_bytes_for(int32_t batch, int32_t n_heads, int32_t n_kv_heads,
+                                                             int32_t head_size, int32_t page_size, int32_t max_pages,
+                                                             int32_t dtype, size_t* bytes);
 B200_API int32_t b200_attention_decode_kv4(const void* q, const void* codes, const void* params,
                                            const int32_t* page_table, const int32_t* ctx_lens, void* o, void* scratch,
                                            size_t scratch_bytes, int32_t batch, int32_t n_heads, int32_t n_kv_heads,

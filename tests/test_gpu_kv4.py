@@ -1,4 +1,5 @@
 """The 4-bit key/value cache: quantisation to the bit, read back, decode attention, page copies, and a run of them."""
+import ctypes
 import math
 
 import pytest
@@ -215,6 +216,32 @@ def test_decode(lens, heads, hk, hs, page, dtype, impl):
     assert bool((err <= bound).all()), float((err / bound).max())
     for _ in range(2):
         assert torch.equal(o, B.attention_decode_kv4(q, codes, params, table, ctx, heads, impl=impl))
+
+
+@pytest.mark.parametrize("heads,hk,hs,dtype", [(8, 2, 128, torch.bfloat16), (20, 1, 64, torch.bfloat16), (6, 3, 48, torch.float32)])
+def test_decode_short_and_long_tables(heads, hk, hs, dtype):
+    # short tables need no scratch and one kernel; the same rows under longer tables are shared out and joined
+    lens = [200, 0, 256, 129, 1]
+    codes, params, table = cache(lens, hk, 64, hs, seed=8)
+    q = torch.randn(len(lens), heads * hs, generator=torch.Generator(device=DEV).manual_seed(5), device=DEV).to(dtype)
+    ctx = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    n = ctypes.c_size_t(7)
+    sizes = (len(lens), heads, hk, hs, 64)
+    fn = B.lib().b200_attention_decode_kv4_scratch_bytes_for
+    assert fn(*sizes, table.shape[1], B._dt(dtype), ctypes.byref(n)) == 0 and n.value == 0
+    long_table = torch.zeros(len(lens), 20, dtype=torch.int32, device=DEV)
+    long_table[:, :table.shape[1]] = table
+    assert fn(*sizes, 20, B._dt(dtype), ctypes.byref(n)) == 0 and n.value > 0
+    want, bound = decode_reference(q, codes, params, table, lens, heads)
+    for t in (table, long_table):
+        o = B.attention_decode_kv4(q, codes, params, t, ctx, heads, out=torch.full_like(q, float("nan")))
+        assert B.device_status() == 0
+        assert bool(((o.double() - want).abs() <= bound).all())
+    scratch = torch.empty(n.value, dtype=torch.uint8, device=DEV)
+    assert torch.equal(o, B.attention_decode_kv4(q, codes, params, long_table, ctx, heads, scratch=scratch))
+    with pytest.raises(B.B200Error) as e:
+        B.attention_decode_kv4(q, codes, params, long_table, ctx, heads, scratch=scratch[:-16])
+    assert e.value.status == 5
 
 
 @pytest.mark.parametrize("impl", [0, 2])
