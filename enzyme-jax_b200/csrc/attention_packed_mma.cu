@@ -126,6 +126,17 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
     ptx::tmem_relinquish();
   }
   pdl_wait();  // q, k, v and cu_seqlens come from the kernels before
+  if (threadIdx.x == 0 && !*abort_flag) {  // the query tiles do not wait for the look-up of the sequences
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int idx = 2 * pair + i;
+      if (idx >= n_tiles) break;
+      ptx::mbar_arrive_expect_tx(&q_full[i], C::kTile);
+#pragma unroll
+      for (int s = 0; s < C::kSubs; ++s)
+        ptx::tma_load_2d(smem + i * C::kTile + s * SUBB, &tmQ, (hk * group + idx % group) * HS + 64 * s, idx / group * TR, &q_full[i]);
+    }
+  }
   if (warp == 2) {
     // rows and keys of the two tiles
     const int cu_first = max(0, *(a.cu)), end = min(a.rows, *(a.cu + a.n_seqs));
@@ -164,19 +175,11 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
   const bool aborted = *abort_flag != 0u;
   const int n_blocks = max(geo[0].last, geo[1].last) + 1;
 
-  if (aborted || n_blocks == 0) {
+  if (aborted) {
     // fall through to the common exit
   } else if (warp == 0) {
     if (lane == 0) {
       const int kb = k_base;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (geo[i].last < geo[i].first) continue;
-        ptx::mbar_arrive_expect_tx(&q_full[i], C::kTile);
-#pragma unroll
-        for (int s = 0; s < C::kSubs; ++s)
-          ptx::tma_load_2d(smem + i * C::kTile + s * SUBB, &tmQ, geo[i].head * HS + 64 * s, geo[i].t0, &q_full[i]);
-      }
       bool ok = true;
       for (int x = 0; x < 2 * n_blocks && ok; ++x) {  // K_0, V_0, K_1, V_1, ...
         const int st = x % NS;
@@ -188,8 +191,12 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
           ptx::tma_load_2d(smem + C::kKV + st * C::kTile + s * SUBB, (x & 1) ? &tmV : &tmK, hk * HS + 64 * s,
                            kb + (x >> 1) * TR, &kv_full[st]);
       }
+      for (int i = 0; i < 2 && ok; ++i)  // no copy outlives the CTA, a query tile without live rows neither
+        if (2 * pair + i < n_tiles) ok = ptx::mbar_wait(&q_full[i], 0, abort_flag, status, ST_PACKED_TIMEOUT);
     }
     __syncwarp();
+  } else if (n_blocks == 0) {
+    // nothing to compute
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t idesc_s = ptx::idesc_bf16_f32(TR, TR);
