@@ -150,11 +150,13 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
       g[i].t0 = rb * TR;
       to[i] = min(g[i].t0 + TR, end) - 1;
       from[i] = cu_first;
-      if (idx < n_tiles) {
+      if (idx >= n_tiles) {
+        to[i] = -1;
+      } else if (i && g[1].t0 == g[0].t0) {  // two heads of one row block
+        from[1] = from[0];
+      } else {
         const int s = seq_of_row_warp(a.cu, a.n_seqs, g[i].t0);
         if (s >= 0 && s < a.n_seqs) from[i] = max(0, min(g[i].t0, *(a.cu + s)));
-      } else {
-        to[i] = -1;
       }
       if (to[i] < g[i].t0) to[i] = -1;
       if (to[i] >= from[i]) base = min(base, from[i]);
