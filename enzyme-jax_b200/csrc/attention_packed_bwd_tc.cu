@@ -3,7 +3,9 @@
 // the gradients are dV = P^T dO, dK = dS^T Q / sqrt(hs), dQ = dS K / sqrt(hs).  Two passes of one kernel, both free of atomics:
 //   MODE_DQ   a CTA owns 128 queries of a query head and streams the keys and values they see
 //   MODE_DKV  a CTA owns 128 keys of a key head and streams, for every query head of the group, the queries and their
-//             cotangents that see them (so the gradient of a shared head is one sum in a fixed order)
+//             cotangents that see them (so the gradient of a shared head is one sum in a fixed order).  The first keys of a
+//             long sequence make the longest CTA by far; two CTAs of a cluster then take half of the group's heads each and
+//             add up through distributed shared memory, one of them dV, the other dK
 // Both have the same shape: two fixed tiles F0, F1 and streamed tiles X0, X1,
 //   S = F0 X0^T,  dP = F1 X1^T  (TMEM, rows = the CTA's own rows)  ->  P, dS as bf16 over S, dP in TMEM
 //   DQ  (F0 = Q, F1 = dO, X0 = K, X1 = V):  acc0 += P X0 (see below),  acc1 += dS X0 -> dQ
@@ -102,6 +104,16 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[64]) {
   ptx::tmem_ld32_at<32>(taddr + 32u, v);
 }
 
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// 16 bytes into the shared memory of CTA `rank` of the cluster, at the place `addr` has in this one
+__device__ __forceinline__ void st_remote(uint32_t addr, uint32_t rank, const float* v) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
+}
+
 // 16 numbers of one row: a thread writes a row by itself, so whole 32-byte sectors at a time where the rows allow it
 __device__ __forceinline__ void store16(bf16* p, const float (&w)[16], bool wide) {
   uint32_t r[8];
@@ -125,7 +137,7 @@ struct OwnGeo {
   int n_it;     // blocks in all
 };
 
-template <int HS, int MODE>
+template <int HS, int MODE, int SPLIT>
 __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
     packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmF0, const __grid_constant__ CUtensorMap tmF1,
                          const __grid_constant__ CUtensorMap tmX0, const __grid_constant__ CUtensorMap tmX1,
@@ -153,7 +165,11 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = f.n_heads / f.n_kv_heads;
-  const int head = blockIdx.x;  // DKV: key head, DQ: query head
+  const int rank = MODE == MODE_DKV ? (int)blockIdx.x % SPLIT : 0;     // DKV: of the CTAs that share a key tile
+  const int head = MODE == MODE_DKV ? (int)blockIdx.x / SPLIT : blockIdx.x;  // DKV: key head, DQ: query head
+  auto meet_peer = [&]() {  // every thread of both CTAs, three times, whatever happened before
+    if (SPLIT == 2) cluster_sync();
+  };
   const int hk = MODE == MODE_DKV ? head : head / group;
   // the longest loops first: early keys are seen by the most queries, late queries see the most keys
   const int own = MODE == MODE_DKV ? (int)blockIdx.y : (int)gridDim.y - 1 - (int)blockIdx.y;
@@ -223,7 +239,7 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
       to = last_row + 1;
     }
     g.per_head = last_row >= g.r0 && to > g.x0 ? (to - g.x0 + BN - 1) / BN : 0;
-    g.n_it = g.per_head * (MODE == MODE_DKV ? group : 1);
+    g.n_it = g.per_head * (MODE == MODE_DKV ? group / SPLIT : 1);
     if (lane == 0) *geo = g;
   }
   ptx::tc_fence_before_sync();
@@ -234,18 +250,18 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
   const OwnGeo g = *geo;
   const int n_it = g.n_it;
 
-  if (aborted) {
-    // common exit below
-  } else if (n_it == 0) {
-    if (threadIdx.x == 0) {  // no copy outlives the CTA
+  if (aborted || n_it == 0) {
+    if (!aborted && threadIdx.x == 0) {  // no copy outlives the CTA
       ptx::mbar_wait(fix_full, 0, abort_flag, status, ST_PACKEDB_TIMEOUT);
       if (MODE == MODE_DQ) ptx::mbar_wait(o_full, 0, abort_flag, status, ST_PACKEDB_TIMEOUT);
     }
+    __syncwarp();
+    for (int i = 0; i < 3; ++i) meet_peer();
   } else if (warp == 0) {
     bool ok = true;
     for (int x = 0; x < 2 * n_it && ok; ++x) {
       const int st = x % NX, it = x >> 1;
-      const int qh = MODE == MODE_DKV ? hk * group + it / g.per_head : head;
+      const int qh = MODE == MODE_DKV ? hk * group + rank * (group / SPLIT) + it / g.per_head : head;
       const int row = g.x0 + (it % g.per_head) * BN;
       ok = ptx::mbar_wait_warp(&x_empty[st], ((uint32_t)(x / NX) & 1u) ^ 1u, abort_flag, status, ST_PACKEDB_TIMEOUT);
       if (MODE == MODE_DQ && x < NX && st >= NX - C::kOTiles)
@@ -272,6 +288,7 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
       }
       __syncwarp();
     }
+    for (int i = 0; i < 3; ++i) meet_peer();
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t id_kk = ptx::idesc_bf16_f32(BR, BN);               // both operands K-major
@@ -336,6 +353,7 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
       if (ok) ptx::mma_commit(acc_done);
     }
     __syncwarp();
+    for (int i = 0; i < 3; ++i) meet_peer();
   } else {
     const int qd = warp & 3;
     const int hf = (warp - 2) >> 2;   // columns NC hf .. NC hf + NC - 1 of a block
@@ -491,9 +509,25 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
       if (lane == 0) ptx::mbar_arrive(ds_full);
     }
     if (ok) ok = ptx::mbar_wait_warp(acc_done, 0, abort_flag, status, ST_PACKEDB_TIMEOUT);
-    if (ok) {
+    // Two CTAs: the first one adds up and writes dV, the second dK.  The streamed tiles' memory is free by now.
+    const uint32_t swap = ptx::smem_u32(smem + C::kX) + (uint32_t)row * 16;
+    constexpr bool shared = SPLIT == 2;
+    meet_peer();
+    if (shared && ok && hf != rank) {
       ptx::tc_fence_after_sync();
-      bool finite = true;
+#pragma unroll 1
+      for (int c = 0; c < HS; c += 32) {
+        float v[32];
+        ptx::tmem_ld32(lane_base + (uint32_t)((hf == 0 ? C::cAcc0 : C::cAcc1) + c), v);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) st_remote(swap + (uint32_t)((c + e) / 4 * BR * 16), (uint32_t)(rank ^ 1), v + e);
+      }
+    }
+    meet_peer();
+    bool finite = true;
+    if (ok && !(shared && hf != rank)) {
+      ptx::tc_fence_after_sync();
       if (MODE == MODE_DKV) {
         // half 0 writes dV, half 1 dK
         bf16* dst = hf == 0 ? (bf16*)a.dv + (size_t)r * a.lddv : (bf16*)a.dk + (size_t)r * a.lddk;
@@ -505,6 +539,13 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
           float v[32];
           ptx::tmem_ld32(src + (uint32_t)c, v);
           ptx::tmem_ld_wait();
+          if (shared) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 w = *reinterpret_cast<const float4*>(smem + C::kX + (c + e) / 4 * BR * 16 + row * 16);
+              v[e] += w.x; v[e + 1] += w.y; v[e + 2] += w.z; v[e + 3] += w.w;
+            }
+          }
           if (live) {
 #pragma unroll
             for (int e = 0; e < 32; e += 16) {
@@ -549,6 +590,9 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
           }
         }
       }
+    }
+    meet_peer();
+    if (ok) {
       // Zero weight times an infinity or NaN of a row that is masked here would not be zero: rows that did not come out
       // finite are computed again over the pairs they are part of alone.  Both halves meet first, so that neither
       // writes a row again while the other still writes it for the first time.
@@ -604,12 +648,14 @@ int32_t launch_hs(const PackedBwdArgs& a, cudaStream_t stream) {
   B200_TRY(make_map_2d(&xdo, a.d_o, f.rows, f.n_heads * HS, a.lddo, C::kBlock));
   CUtensorMap fo;
   B200_TRY(make_map_2d(&fo, f.o, f.rows, f.n_heads * HS, f.ldo, BR));
-  auto dq = packed_bwd_tc_kernel<HS, MODE_DQ>;
-  auto dkv = packed_bwd_tc_kernel<HS, MODE_DKV>;
+  auto dq = packed_bwd_tc_kernel<HS, MODE_DQ, 1>;
+  auto dkv = packed_bwd_tc_kernel<HS, MODE_DKV, 1>;
+  auto dkv2 = packed_bwd_tc_kernel<HS, MODE_DKV, 2>;
   static PerDeviceOnce attr_once;
   B200_TRY(attr_once.run([&](int&) -> int32_t {
     B200_CUDA_OK(cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     B200_CUDA_OK(cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    B200_CUDA_OK(cudaFuncSetAttribute(dkv2, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     return B200_OK;
   }));
   uint32_t* status = device_status_word();
@@ -619,8 +665,20 @@ int32_t launch_hs(const PackedBwdArgs& a, cudaStream_t stream) {
   B200_CUDA_OK(launch_pdl(dq, dim3(f.n_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, fq, fdo, xk, xv, fo, a,
                           scale, status));
   B200_LAUNCH_OK("packed_bwd_tc_kernel<dq>");
-  B200_CUDA_OK(launch_pdl(dkv, dim3(f.n_kv_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, fk, fv, xq, xdo, fo, a,
-                          scale, status));
+  // Two CTAs per key tile where there are few tiles, or not many and the sequences are long enough to differ in length.
+  // Backward with one / two (us, heads of 128): 12 ragged documents of 32/8 heads (304 tiles) 333 / 317, 2048 tokens of 8/2
+  // heads (32) 196 / 136; 8 x 1024 of 32/8 (512) 407 / 421, 64 x 128 of 32/8 (512) 216 / 246.  Heads of 64: 365 / 245 and
+  // 214 / 141, 8 x 1024 of 12/6 (384) 159 / 151; 64 x 128 of 32/8 (512) 122 / 139.
+  const long long key_tiles = (long long)f.n_kv_heads * blocks;
+  const bool few = 2 * key_tiles <= sm_count();
+  const bool uneven = key_tiles <= 3LL * sm_count() && f.rows >= 256LL * f.n_seqs;
+  const bool two = (f.n_heads / f.n_kv_heads) % 2 == 0 && (few || uneven);
+  if (two)
+    B200_CUDA_OK(launch_pdl_cluster(dkv2, dim3(f.n_kv_heads * 2, blocks), dim3(PB_THREADS), 2, C::kSmem, stream, fk, fv, xq, xdo, fo,
+                                    a, scale, status));
+  else
+    B200_CUDA_OK(launch_pdl(dkv, dim3(f.n_kv_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, fk, fv, xq, xdo, fo, a, scale,
+                            status));
   B200_LAUNCH_OK("packed_bwd_tc_kernel<dkv>");
   return B200_OK;
 }

@@ -204,6 +204,26 @@ def test_gradient_against_differences():
         assert abs(got - diff) <= float((bounds[i] * d.abs()).sum()) + 1e-6 * (1 + abs(diff))
 
 
+@pytest.mark.parametrize("lens,heads,kv_heads,hs", [
+    ([300, 0, 1100, 7], 8, 4, 64), ([300, 0, 1100, 7], 8, 2, 128),         # two CTAs share a key tile
+    ([700, 300], 6, 1, 128), ([129], 4, 2, 64), ([1, 1, 2], 2, 1, 128),
+    ([400, 100] * 20, 16, 8, 64), ([30] * 100, 32, 16, 64), ([600], 9, 3, 128)])  # they do not
+def test_backward_of_grouped_heads(lens, heads, kv_heads, hs):
+    q, k, v, d_o = make(lens, heads, kv_heads, hs, torch.bfloat16, seed=21, gap=3, tail=5)
+    cu = cu_of(lens, 3)
+    o, lse = B.attention_packed(q, k, v, cu, heads, kv_heads)
+    marks = [torch.full(x.shape, 7.0, dtype=x.dtype, device=DEV) for x in (q, k, v)]
+    got = B.attention_packed_backward(q, k, v, o, lse, d_o, cu, heads, kv_heads, dq=marks[0], dk=marks[1], dv=marks[2])
+    assert B.device_status() == 0
+    want, bounds = R.backward(q, k, v, d_o, lens, heads, kv_heads, 3)
+    for name, x, r, b in zip(("dq", "dk", "dv"), got, want, bounds):
+        err = (x.double() - r).abs()[3:-5]
+        assert bool((err <= b[3:-5]).all()), (name, float((err / b[3:-5]).max()))
+        assert bool((x[:3] == 7).all() and (x[-5:] == 7).all())
+    again = B.attention_packed_backward(q, k, v, o, lse, d_o, cu, heads, kv_heads)
+    assert all(torch.equal(x[3:-5], y[3:-5]) for x, y in zip(got, again))
+
+
 @pytest.mark.parametrize("impl", [0, 2])
 @pytest.mark.parametrize("lens", [[1] * 300, [1, 130, 1, 1, 63, 1, 200, 2, 1, 1]])
 @pytest.mark.parametrize("hs,dtype", [(64, torch.bfloat16), (128, torch.bfloat16), (48, torch.float32), (32, torch.bfloat16)])
