@@ -355,6 +355,13 @@ def _rows(what: str, name: str, t: torch.Tensor, cols: int, rows: Optional[int] 
     return ld
 
 
+def _rows_or_new(what: str, name: str, t: Optional[torch.Tensor], cols: int, rows: int, dtype: torch.dtype, dev):
+    """The caller's tensor, checked, or a new one, with its row pitch."""
+    if t is None:
+        return torch.empty(rows, cols, dtype=dtype, device=dev), cols
+    return t, _rows(what, name, t, cols, rows, dtype)
+
+
 def _index(what: str, name: str, t: torch.Tensor, dim: int = 1) -> None:
     if t.dtype is not torch.int32 or t.dim() != dim or not t.is_contiguous():
         raise B200Error(3, f"{what}: {name} must be a contiguous int32 tensor of {dim} dimension(s)")
@@ -385,9 +392,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     _index(what, "cu_seqlens", cu_seqlens)
     if cu_seqlens.numel() < 1:
         raise B200Error(2, f"{what}: cu_seqlens holds n_seqs + 1 entries, at least one")
-    if out is None:
-        out = torch.empty(rows, n_heads * hs, dtype=dt, device=dev)
-    ldo = _rows(what, "out", out, n_heads * hs, rows, dt)
+    out, ldo = _rows_or_new(what, "out", out, n_heads * hs, rows, dt, dev)
     if lse is None:
         lse = torch.empty(n_heads, rows, dtype=torch.float32, device=dev)
     elif lse.dtype != torch.float32 or tuple(lse.shape) != (n_heads, rows) or not lse.is_contiguous():
@@ -421,12 +426,9 @@ def attention_packed_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     _index(what, "cu_seqlens", cu_seqlens)
     if cu_seqlens.numel() < 1:
         raise B200Error(2, f"{what}: cu_seqlens holds n_seqs + 1 entries, at least one")
-    dq = torch.empty(rows, wq, dtype=dt, device=dev) if dq is None else dq
-    dk = torch.empty(rows, wk, dtype=dt, device=dev) if dk is None else dk
-    dv = torch.empty(rows, wk, dtype=dt, device=dev) if dv is None else dv
-    lddq = _rows(what, "dq", dq, wq, rows, dt)
-    lddk = _rows(what, "dk", dk, wk, rows, dt)
-    lddv = _rows(what, "dv", dv, wk, rows, dt)
+    dq, lddq = _rows_or_new(what, "dq", dq, wq, rows, dt, dev)
+    dk, lddk = _rows_or_new(what, "dk", dk, wk, rows, dt, dev)
+    dv, lddv = _rows_or_new(what, "dv", dv, wk, rows, dt, dev)
     delta = torch.empty(n_heads * rows, dtype=torch.float32, device=dev)
     _call(dev, lib().b200_attention_packed_backward, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
           lse.data_ptr(), d_o.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(),
@@ -500,10 +502,8 @@ def kv4_read(codes: torch.Tensor, params: torch.Tensor, page_table: torch.Tensor
     n_seqs = _kv4_rows(what, page_table, cu_seqlens, ctx_before)
     if rows < 0:
         raise B200Error(2, f"{what}: {rows} rows")
-    k = torch.empty(rows, n_kv_heads * hs, dtype=dtype, device=dev) if k is None else k
-    v = torch.empty(rows, n_kv_heads * hs, dtype=dtype, device=dev) if v is None else v
-    ldk = _rows(what, "k", k, n_kv_heads * hs, rows, dtype)
-    ldv = _rows(what, "v", v, n_kv_heads * hs, rows, dtype)
+    k, ldk = _rows_or_new(what, "k", k, n_kv_heads * hs, rows, dtype, dev)
+    v, ldv = _rows_or_new(what, "v", v, n_kv_heads * hs, rows, dtype, dev)
     _call(dev, lib().b200_kv4_read, k.data_ptr(), v.data_ptr(), codes.data_ptr(), params.data_ptr(),
           page_table.data_ptr(), cu_seqlens.data_ptr(), _ptr(ctx_before), n_seqs, rows, n_kv_heads, hs, ldk, ldv,
           n_pages, page_size, page_table.shape[1], _dt(dtype))
@@ -536,9 +536,7 @@ def attention_decode_kv4(q: torch.Tensor, codes: torch.Tensor, params: torch.Ten
     if page_table.shape[0] != batch or ctx_lens.numel() != batch:
         raise B200Error(2, f"{what}: page_table {tuple(page_table.shape)} and ctx_lens {tuple(ctx_lens.shape)} for a "
                            f"batch of {batch}")
-    if out is None:
-        out = torch.empty(batch, n_heads * hs, dtype=q.dtype, device=dev)
-    ldo = _rows(what, "out", out, n_heads * hs, batch, q.dtype)
+    out, ldo = _rows_or_new(what, "out", out, n_heads * hs, batch, q.dtype, dev)
     max_pages, dt = page_table.shape[1], _dt(q.dtype)
     if scratch is None:
         size, at = _kv4_scratch_bytes(batch, n_heads, n_kv_heads, hs, page_size, max_pages, dt), None
