@@ -8,8 +8,12 @@
 // one bad value must not come back as a plausible one.
 // A warp takes a packed row (or, when rows are few, a part of its heads): it finds the row's sequence and page once, then
 // hs/8 lanes share a (head, half), 8 elements and one 32-bit word of codes each.  A quotient is a product with the
-// reciprocal, rounded, and then checked against its exact remainder, which costs half of a division.
-// Bound: bytes of the inputs plus hs/2 + 4 per row and half at HBM speed; about 75 instructions per (head, half).
+// reciprocal, rounded, and then checked against its exact remainder, which costs half of a division; elements go two at a
+// time through the packed fp32 instructions, minimum and maximum through one packed 16-bit reduction.
+// Bound: bytes of the inputs plus hs/2 + 4 per row and half at HBM speed.  What bounds it now is instruction issue (2.7 of 4
+// per cycle before the packed forms) and the look-ups in front of the first store: 15,398 ragged prompt rows of 8 heads of 128,
+// appended and read back, take 54 us, 119 us with plain divisions and a look-up per row and head.  More items in flight per
+// warp, or fewer with more warps, changed nothing.
 #include "kv4.cuh"
 #include "attention_packed.cuh"
 
@@ -112,10 +116,31 @@ __device__ __noinline__ uint2 quantise_rare(float4 x, float4 y, float mn, float 
   return make_uint2(w, __byte_perm(__float_as_uint(scale), __float_as_uint(mn), 0x7632));
 }
 
-// Eight elements as they stand in memory.
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// Eight elements as they stand in memory.  range<L>: their smallest and largest number over the L lanes of a group (lanes
+// that are not `on` count for nothing), NaN if there is one.
 template <typename T> struct Raw8;
 template <> struct Raw8<bf16> {
   uint4 r;
+  // both in one word, the largest negated: one shuffle and one minimum per step
+  template <int L> __device__ __forceinline__ float2 range(bool on) const {
+    const uint32_t lo = min2_nan(min2_nan(r.x, r.y), min2_nan(r.z, r.w)), hi = max2_nan(max2_nan(r.x, r.y), max2_nan(r.z, r.w));
+    uint32_t m = min2_nan(__byte_perm(lo, hi, 0x5410) ^ 0x80000000u, __byte_perm(lo, hi, 0x7632) ^ 0x80000000u);
+    if (!on) m = 0x7f807f80u;
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) m = min2_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return make_float2(__uint_as_float(m << 16), __uint_as_float((m & 0xffff0000u) ^ 0x80000000u));
+  }
   __device__ __forceinline__ void load(const bf16* p) { r = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void set(int e, bf16 v) {
     uint32_t& w = (&r.x)[e >> 1];
@@ -133,6 +158,11 @@ template <> struct Raw8<bf16> {
 };
 template <> struct Raw8<float> {
   float4 a, b;
+  template <int L> __device__ __forceinline__ float2 range(bool on) const {
+    float lo = min3_nan(min3_nan(a.x, a.y, a.z), min3_nan(a.w, b.x, b.y), min_nan(b.z, b.w));
+    float hi = max3_nan(max3_nan(a.x, a.y, a.z), max3_nan(a.w, b.x, b.y), max_nan(b.z, b.w));
+    return make_float2(group_min<L>(on ? lo : INFINITY), group_max<L>(on ? hi : -INFINITY));
+  }
   __device__ __forceinline__ void load(const float* p) {
     a = *reinterpret_cast<const float4*>(p);
     b = *reinterpret_cast<const float4*>(p + 4);
@@ -178,38 +208,39 @@ __global__ void __launch_bounds__(AT, 4) kv4_append_kernel(Kv4RowsArgs a, const 
   int page, in_page;
   if (!place_of(a, t, &page, &in_page)) return;
   const size_t row0 = (size_t)page * nk * a.pool.page_size + in_page, half = kv4_half(a.pool);
+  uint32_t* codes_k = reinterpret_cast<uint32_t*>(a.pool.codes) + row0 * (HS / 8) + li;
+  uint32_t* codes_v = codes_k + half * (HS / 8);
+  uint32_t* prm_k = a.pool.params + row0;
   for (int i0 = first; i0 < last; i0 += U * GPW) {
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int item = i0 + j * GPW + sub;
       if (i0 + j * GPW >= last) break;  // the same for the warp
-      float x[8], lo = INFINITY, hi = -INFINITY;
+      float x[8];
       raw[j].get(x);
-      if (item < last && lane_on) {
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          lo = min3_nan(lo, x[e], x[e + 1]);
-          hi = max3_nan(hi, x[e], x[e + 1]);
-        }
-      }
-      lo = group_min<LPR>(lo);
-      hi = group_max<LPR>(hi);
-      const float mn = sizeof(T) == 2 ? lo : bf16_down(lo);  // a 16-bit minimum is one already
-      const float spread = hi - mn;
+      const float2 range = raw[j].template range<LPR>(item < last && lane_on);
+      const float mn = sizeof(T) == 2 ? range.x : bf16_down(range.x);  // a 16-bit minimum is one already
+      const float spread = range.y - mn;
       uint32_t word, prm;
       if (spread > 0x1p-90f && spread < 0x1p90f) {
         const float scale = bf16_up_nonneg(divide(spread, 15.f, 1.f / 15.f));
         float inv;
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
         inv = fmaf(fmaf(-scale, inv, 1.f), inv, inv);  // correctly rounded: no 8-bit number has a reciprocal near a midpoint
-        float c[8];
+        // `divide` for elements e and e + 4 at a time; adding 1.5 * 2^23 rounds to integers, ties to even
+        const float2 mn2 = make_float2(-mn, -mn), inv2 = make_float2(inv, inv), ns2 = make_float2(-scale, -scale);
+        const float2 up = make_float2(12582912.f, 12582912.f), down = make_float2(-12582912.f, -12582912.f);
+        float2 c[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)  // adding 1.5 * 2^23 rounds to integers, ties to even
-          c[e] = (divide(x[e] - mn, scale, inv) + 12582912.f) - 12582912.f;
+        for (int e = 0; e < 4; ++e) {
+          const float2 d = __fadd2_rn(make_float2(x[e], x[e + 4]), mn2);
+          const float2 q = __fmul2_rn(d, inv2);
+          c[e] = __fadd2_rn(__fadd2_rn(__ffma2_rn(__ffma2_rn(q, ns2, d), inv2, q), up), down);
+        }
         // four codes are a number below 2^16: packed by the multiply-add pipe, the integer pipe being the busier one
-        const float w0 = fmaf(fmaf(c[3], 16.f, c[2]), 256.f, fmaf(c[1], 16.f, c[0]));
-        const float w1 = fmaf(fmaf(c[7], 16.f, c[6]), 256.f, fmaf(c[5], 16.f, c[4]));
-        word = __byte_perm(__float_as_uint(w0 + 8388608.f), __float_as_uint(w1 + 8388608.f), 0x5410);
+        const float2 f16 = make_float2(16.f, 16.f), f256 = make_float2(256.f, 256.f), base = make_float2(8388608.f, 8388608.f);
+        const float2 w4 = __fadd2_rn(__ffma2_rn(__ffma2_rn(c[3], f16, c[2]), f256, __ffma2_rn(c[1], f16, c[0])), base);
+        word = __byte_perm(__float_as_uint(w4.x), __float_as_uint(w4.y), 0x5410);
         prm = __byte_perm(__float_as_uint(scale), __float_as_uint(mn), 0x7632);
       } else {
         const uint2 r = quantise_rare(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), mn, spread);
@@ -217,9 +248,10 @@ __global__ void __launch_bounds__(AT, 4) kv4_append_kernel(Kv4RowsArgs a, const 
         prm = r.y;
       }
       if (item < last) {
-        const size_t row = row0 + (size_t)(item >= nk ? item - nk : item) * a.pool.page_size + (item >= nk ? half : 0);
-        if (lane_on) reinterpret_cast<uint32_t*>(a.pool.codes)[row * (HS / 8) + li] = word;
-        if (li == 0) a.pool.params[row] = prm;
+        const bool is_v = item >= nk;
+        const size_t at = (size_t)((unsigned)(is_v ? item - nk : item) * (unsigned)a.pool.page_size);  // inside a page: 32 bits
+        if (lane_on) (is_v ? codes_v : codes_k)[at * (HS / 8)] = word;
+        if (li == 0) (is_v ? prm_k + half : prm_k)[at] = prm;
       }
     }
     load(i0 + U * GPW);
@@ -241,6 +273,11 @@ __global__ void __launch_bounds__(AT) kv4_read_kernel(Kv4RowsArgs a, T* __restri
   const int first = part * per_part, last = min(2 * nk, first + per_part);
   const size_t row0 = (size_t)page * nk * a.pool.page_size + in_page, half = kv4_half(a.pool);
   if (li * 8 >= HS) return;
+  const uint32_t* codes_k = reinterpret_cast<const uint32_t*>(a.pool.codes) + row0 * (HS / 8) + li;
+  const uint32_t* codes_v = codes_k + half * (HS / 8);
+  const uint32_t* prm_k = a.pool.params + row0;
+  T* kt = k + (size_t)t * ldk + li * 8;
+  T* vt = v + (size_t)t * ldv + li * 8;
   for (int i0 = first; i0 < last; i0 += U * GPW) {
     uint32_t word[U], prm[U];
 #pragma unroll
@@ -248,9 +285,9 @@ __global__ void __launch_bounds__(AT) kv4_read_kernel(Kv4RowsArgs a, T* __restri
       const int item = i0 + j * GPW + sub;
       const bool is_v = item >= nk;
       if (item < last) {
-        const size_t row = row0 + (size_t)(is_v ? item - nk : item) * a.pool.page_size + (is_v ? half : 0);
-        word[j] = reinterpret_cast<const uint32_t*>(a.pool.codes)[row * (HS / 8) + li];
-        prm[j] = a.pool.params[row];
+        const size_t at = (size_t)((unsigned)(is_v ? item - nk : item) * (unsigned)a.pool.page_size);
+        word[j] = (is_v ? codes_v : codes_k)[at * (HS / 8)];
+        prm[j] = (is_v ? prm_k + half : prm_k)[at];
       }
     }
 #pragma unroll
@@ -259,11 +296,18 @@ __global__ void __launch_bounds__(AT) kv4_read_kernel(Kv4RowsArgs a, T* __restri
       if (item >= last) break;
       const bool is_v = item >= nk;
       const float scale = __uint_as_float(prm[j] << 16), mn = __uint_as_float(prm[j] & 0xffff0000u);
+      const uint32_t even = word[j] & 0x0f0f0f0fu, odd = (word[j] >> 4) & 0x0f0f0f0fu;
+      const float2 base = make_float2(-8388608.f, -8388608.f), scale2 = make_float2(scale, scale), mn2 = make_float2(mn, mn);
       float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)  // 2^23 + code, less 2^23: exact
-        x[e] = fmaf(__uint_as_float(((word[j] >> (4 * e)) & 15u) | 0x4b000000u) - 8388608.f, scale, mn);
-      T* dst = (is_v ? v + (size_t)t * ldv : k + (size_t)t * ldk) + (is_v ? item - nk : item) * HS + li * 8;
+      for (int e = 0; e < 4; ++e) {  // 2^23 + code, less 2^23: exact
+        const float2 n = make_float2(__uint_as_float(__byte_perm(even, 0x4b000000u, 0x7440 + e)),
+                                     __uint_as_float(__byte_perm(odd, 0x4b000000u, 0x7440 + e)));
+        const float2 y = __ffma2_rn(__fadd2_rn(n, base), scale2, mn2);
+        x[2 * e] = y.x;
+        x[2 * e + 1] = y.y;
+      }
+      T* dst = is_v ? vt + (item - nk) * HS : kt + item * HS;
       if (vec) {
         store8(dst, x);
       } else {
@@ -511,6 +555,8 @@ template <typename F> int32_t by_type(const char* what, int dtype, int hs, F&& f
 int32_t check_pool(const char* what, const Kv4Pool& p) {
   if (p.n_pages < 0 || p.n_kv_heads <= 0 || p.page_size <= 0 || p.max_pages < 0 || p.head_size <= 0)
     return fail(B200_ERR_BAD_SHAPE, "%s: sizes must be positive", what);
+  if ((long long)p.n_kv_heads * p.page_size > 0x7fffffffLL)
+    return fail(B200_ERR_BAD_SHAPE, "%s: %d rows of %d heads are too many for one page", what, p.page_size, p.n_kv_heads);
   switch (p.head_size) {
     case 16: case 32: case 48: case 64: case 128: return B200_OK;
   }
