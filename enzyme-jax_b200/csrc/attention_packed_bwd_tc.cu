@@ -28,8 +28,12 @@
 // stands before the first dS; L2 prefetches of the next CTA's tiles changed nothing).
 //
 // Bound: 8 products of 128 x 128 x hs per (query block, key block), of which 5 are the formula's; 512 cycles each at head
-// size 128, 1024 cycles of exponentials.  Rounding to bf16 happens to P, dS and the results; sums are fp32.  All waits
-// are bounded.
+// size 128, 1024 cycles of exponentials.  A block's chain is 3550 cycles there (wait for S 640 to 1170, exponentials 1450, wait
+// for dP 190 to 320, dS 670 to 860), and 2600 to 2900 for two CTAs' blocks of 64 rows at head size 64; set-up to the first S
+// takes 3.3 to 4 us of a CTA and its epilogue 2 to 3, which short sequences pay per 128 rows.  12 ragged documents of 32/8 heads
+// (4789 rows): 314 us, 350 TFLOP/s over the formula's 5 products; 8 x 1024 tokens of 12 heads of 64: 129 us, 250.  Tried and
+// not kept: results through shared memory (129 -> 133 us), eight arrivals per meeting instead of 256 (no change).
+// Rounding to bf16 happens to P, dS and the results; sums are fp32.  All waits are bounded.
 #include <cuda.h>
 
 #include "attention_packed.cuh"
