@@ -475,8 +475,9 @@ def _kv4_rows(what: str, page_table: torch.Tensor, cu_seqlens: torch.Tensor, ctx
 def kv4_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, page_table: torch.Tensor,
                cu_seqlens: torch.Tensor, ctx_before: Optional[torch.Tensor] = None) -> None:
     """Quantises the packed rows k, v [rows, n_kv_heads*hs] into one layer of a 4-bit cache.  Row t of sequence s becomes
-    its cached row ``ctx_before[s] + t - cu_seqlens[s]`` (``ctx_before`` None: the sequences start empty).  Rows without
-    a place (behind the page table, or a page id outside the pool) are skipped and make :func:`device_status` raise."""
+    its cached row ``ctx_before[s] + t - cu_seqlens[s]`` (``ctx_before`` None: the sequences start empty).  No two rows of
+    a call may have the same place: sequences that share pages append behind them.  Rows without a place (behind the page
+    table, or a page id outside the pool) are skipped and make :func:`device_status` raise."""
     what = "kv4_append"
     dev = _device_of(what, "k v codes params page_table cu_seqlens ctx_before",
                      k, v, codes, params, page_table, cu_seqlens, ctx_before)

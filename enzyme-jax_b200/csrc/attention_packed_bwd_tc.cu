@@ -216,14 +216,19 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
     ptx::mbar_arrive_expect_tx(fix_full, 2 * C::kTile);
 #pragma unroll
     for (int s = 0; s < C::kSubs; ++s) {
-      ptx::tma_load_2d(smem + s * BSUB, &tmF0, head * HS + 64 * s, own * BR, fix_full);
-      ptx::tma_load_2d(smem + C::kTile + s * BSUB, &tmF1, head * HS + 64 * s, own * BR, fix_full);
+#pragma unroll
+      for (int y = 0; y < BR; y += BN) {  // 128 bytes of a row each
+        ptx::tma_load_2d(smem + s * BSUB + y * 128, &tmF0, head * HS + 64 * s, own * BR + y, fix_full);
+        ptx::tma_load_2d(smem + C::kTile + s * BSUB + y * 128, &tmF1, head * HS + 64 * s, own * BR + y, fix_full);
+      }
     }
     if (MODE == MODE_DQ) {
       ptx::mbar_arrive_expect_tx(o_full, C::kTile);
 #pragma unroll
       for (int s = 0; s < C::kSubs; ++s)
-        ptx::tma_load_2d(smem + C::kO + s * BSUB, &tmO, head * HS + 64 * s, own * BR, o_full);
+#pragma unroll
+        for (int y = 0; y < BR; y += BN)
+          ptx::tma_load_2d(smem + C::kO + s * BSUB + y * 128, &tmO, head * HS + 64 * s, own * BR + y, o_full);
     }
   }
   if (warp == 2) {
@@ -640,18 +645,13 @@ template <int HS>
 int32_t launch_hs(const PackedBwdArgs& a, cudaStream_t stream) {
   using C = BCfg<HS>;
   const PackedArgs& f = a.f;
-  // as the fixed tile of one pass (128 rows) and as the streamed tile of the other
-  CUtensorMap fq, fk, fv, fdo, xq, xk, xv, xdo;
-  B200_TRY(make_map_2d(&fq, f.q, f.rows, f.n_heads * HS, f.ldq, BR));
-  B200_TRY(make_map_2d(&fk, f.k, f.rows, f.n_kv_heads * HS, f.ldk, BR));
-  B200_TRY(make_map_2d(&fv, f.v, f.rows, f.n_kv_heads * HS, f.ldv, BR));
-  B200_TRY(make_map_2d(&fdo, a.d_o, f.rows, f.n_heads * HS, a.lddo, BR));
-  B200_TRY(make_map_2d(&xq, f.q, f.rows, f.n_heads * HS, f.ldq, C::kBlock));
-  B200_TRY(make_map_2d(&xk, f.k, f.rows, f.n_kv_heads * HS, f.ldk, C::kBlock));
-  B200_TRY(make_map_2d(&xv, f.v, f.rows, f.n_kv_heads * HS, f.ldv, C::kBlock));
-  B200_TRY(make_map_2d(&xdo, a.d_o, f.rows, f.n_heads * HS, a.lddo, C::kBlock));
-  CUtensorMap fo;
-  B200_TRY(make_map_2d(&fo, f.o, f.rows, f.n_heads * HS, f.ldo, BR));
+  // in boxes of a streamed block; a fixed tile is one or two of them
+  CUtensorMap mq, mk, mv, mdo, mo;
+  B200_TRY(make_map_2d(&mq, f.q, f.rows, f.n_heads * HS, f.ldq, C::kBlock));
+  B200_TRY(make_map_2d(&mk, f.k, f.rows, f.n_kv_heads * HS, f.ldk, C::kBlock));
+  B200_TRY(make_map_2d(&mv, f.v, f.rows, f.n_kv_heads * HS, f.ldv, C::kBlock));
+  B200_TRY(make_map_2d(&mdo, a.d_o, f.rows, f.n_heads * HS, a.lddo, C::kBlock));
+  B200_TRY(make_map_2d(&mo, f.o, f.rows, f.n_heads * HS, f.ldo, C::kBlock));
   auto dq = packed_bwd_tc_kernel<HS, MODE_DQ, 1>;
   auto dkv = packed_bwd_tc_kernel<HS, MODE_DKV, 1>;
   auto dkv2 = packed_bwd_tc_kernel<HS, MODE_DKV, 2>;
@@ -666,7 +666,7 @@ int32_t launch_hs(const PackedBwdArgs& a, cudaStream_t stream) {
   if (!status) return fail(B200_ERR_CUDA, "no device status word");
   const float scale = 1.f / sqrtf((float)HS);
   const unsigned blocks = (unsigned)cdiv(f.rows, BR);
-  B200_CUDA_OK(launch_pdl(dq, dim3(f.n_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, fq, fdo, xk, xv, fo, a,
+  B200_CUDA_OK(launch_pdl(dq, dim3(f.n_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, mq, mdo, mk, mv, mo, a,
                           scale, status));
   B200_LAUNCH_OK("packed_bwd_tc_kernel<dq>");
   // Two CTAs per key tile where there are few tiles, or not many and the sequences are long enough to differ in length.
@@ -678,10 +678,10 @@ int32_t launch_hs(const PackedBwdArgs& a, cudaStream_t stream) {
   const bool uneven = key_tiles <= 3LL * sm_count() && f.rows >= 256LL * f.n_seqs;
   const bool two = (f.n_heads / f.n_kv_heads) % 2 == 0 && (few || uneven);
   if (two)
-    B200_CUDA_OK(launch_pdl_cluster(dkv2, dim3(f.n_kv_heads * 2, blocks), dim3(PB_THREADS), 2, C::kSmem, stream, fk, fv, xq, xdo, fo,
+    B200_CUDA_OK(launch_pdl_cluster(dkv2, dim3(f.n_kv_heads * 2, blocks), dim3(PB_THREADS), 2, C::kSmem, stream, mk, mv, mq, mdo, mo,
                                     a, scale, status));
   else
-    B200_CUDA_OK(launch_pdl(dkv, dim3(f.n_kv_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, fk, fv, xq, xdo, fo, a, scale,
+    B200_CUDA_OK(launch_pdl(dkv, dim3(f.n_kv_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, mk, mv, mq, mdo, mo, a, scale,
                             status));
   B200_LAUNCH_OK("packed_bwd_tc_kernel<dkv>");
   return B200_OK;

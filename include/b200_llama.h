@@ -409,8 +409,8 @@ B200_API int32_t b200_attention_packed_backward(const void* q, const void* k, co
  *
  * b200_kv4_append quantises packed rows k, v [rows, ldk / ldv] into the pages: row t of sequence s (cu_seqlens as above)
  * becomes its row ctx_before[s] + t - cu_seqlens[s] (ctx_before NULL: 0).  A decode step is n_seqs = rows with
- * cu_seqlens = 0, 1, 2, ...  b200_kv4_read is the way back, to k, v of `dtype`.  page_table int32 [n_seqs, max_pages].
- * Positions behind the page table and page ids outside the pool are skipped; b200_device_status then answers
+ * cu_seqlens = 0, 1, 2, ...  No two rows of a call may have the same place.  b200_kv4_read is the way back, to k, v of
+ * `dtype`.  page_table int32 [n_seqs, max_pages].  Positions behind the page table and page ids outside the pool are skipped; b200_device_status then answers
  * B200_ERR_INVALID_ARG. */
 B200_API int32_t b200_kv4_append(const void* k, const void* v, void* codes, void* params, const int32_t* page_table,
                                  const int32_t* cu_seqlens, const int32_t* ctx_before, int32_t n_seqs, int32_t rows,
