@@ -1,4 +1,5 @@
-// Packed causal attention forward on the 5th-generation tensor cores (bf16, head size 64 or 128), flash-style.
+// Packed causal attention forward on the 5th-generation tensor cores (bf16, head size 64 or 128), in one pass over the keys
+// with a running maximum and sum.
 //
 // A CTA owns TWO tiles of 128 query rows that read the same key head: the tiles of one key head are listed row block by
 // row block with the heads of its group inside, and a CTA takes two neighbours of that list -- two heads of the group over

@@ -130,13 +130,14 @@ __global__ void __launch_bounds__(128) packed_fwd_simt_kernel(PackedArgs a, floa
     if (from <= to && from < RB && to >= 0) {
       const float nm = fmaxf(mx, bm);
       const float corr = mx == nm ? 1.f : exp_by_build(mx - nm);
+      const float ref = nm == -INFINITY ? 0.f : nm;  // scores of minus infinity alone: no weight yet
       l *= corr;
 #pragma unroll
       for (int i = 0; i < DPT; ++i) acc[i] *= corr;
       if (from <= 0 && to >= RB - 1) {
 #pragma unroll
         for (int uu = 0; uu < RB; ++uu) {
-          const float p = exp_by_build(s[uu] - nm);
+          const float p = exp_by_build(s[uu] - ref);
           l += p;
           axpy_quarter(acc, p, vq + uu * Q::kRow);
         }
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(128) packed_fwd_simt_kernel(PackedArgs a, floa
 #pragma unroll
         for (int uu = 0; uu < RB; ++uu) {
           if (uu >= from && uu <= to) {
-            const float p = exp_by_build(s[uu] - nm);
+            const float p = exp_by_build(s[uu] - ref);
             l += p;
             axpy_quarter(acc, p, vq + uu * Q::kRow);
           }

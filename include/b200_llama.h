@@ -410,8 +410,8 @@ B200_API int32_t b200_attention_packed_backward(const void* q, const void* k, co
  * b200_kv4_append quantises packed rows k, v [rows, ldk / ldv] into the pages: row t of sequence s (cu_seqlens as above)
  * becomes its row ctx_before[s] + t - cu_seqlens[s] (ctx_before NULL: 0).  A decode step is n_seqs = rows with
  * cu_seqlens = 0, 1, 2, ...  No two rows of a call may have the same place.  b200_kv4_read is the way back, to k, v of
- * `dtype`.  page_table int32 [n_seqs, max_pages].  Positions behind the page table and page ids outside the pool are skipped; b200_device_status then answers
- * B200_ERR_INVALID_ARG. */
+ * `dtype`.  page_table int32 [n_seqs, max_pages].  Positions behind the page table and page ids outside the pool are
+ * skipped; b200_device_status then answers B200_ERR_INVALID_ARG. */
 B200_API int32_t b200_kv4_append(const void* k, const void* v, void* codes, void* params, const int32_t* page_table,
                                  const int32_t* cu_seqlens, const int32_t* ctx_before, int32_t n_seqs, int32_t rows,
                                  int32_t n_kv_heads, int32_t head_size, int32_t ldk, int32_t ldv, int32_t n_pages,
@@ -425,8 +425,9 @@ B200_API int32_t b200_kv4_read(void* k, void* v, const void* codes, const void* 
  * [batch] on the device, cut to max_pages * page_size; a sequence without rows gets zeros), grouped heads as above.
  * q, o [batch, ldq / ldo] of `dtype`.  scratch: b200_attention_decode_kv4_scratch_bytes() bytes, 16-byte aligned, used by
  * this call alone while it runs; b200_attention_decode_kv4_scratch_bytes_for() says how much of that a call with these page
- * tables needs, and 0 where the tables are so short that scratch may be NULL.  Pages outside the pool are skipped and reported as above.  impl: 0 = pick, 1 = tensor
- * cores (bf16, head size 64 or 128, page_size a multiple of 16), 2 = CUDA cores. */
+ * tables needs, and 0 where the tables are so short that scratch may be NULL.  Pages outside the pool are skipped and
+ * reported as above.  impl: 0 = pick, 1 = tensor cores (bf16, head size 64 or 128, page_size a multiple of 16), 2 = CUDA
+ * cores. */
 B200_API int32_t b200_attention_decode_kv4_scratch_bytes(int32_t batch, int32_t n_heads, int32_t n_kv_heads,
                                                          int32_t head_size, size_t* bytes);
 B200_API int32_t b200_attention_decode_kv4_scratch_bytes_for(int32_t batch, int32_t n_heads, int32_t n_kv_heads,

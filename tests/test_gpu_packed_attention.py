@@ -149,6 +149,24 @@ def test_masked_infinities(hs, dtype, impl, bad):
     assert clean_o.shape == o.shape and clean_lse.shape == lse.shape
 
 
+@pytest.mark.parametrize("impl", [0, 2])
+@pytest.mark.parametrize("hs,dtype", [(64, torch.bfloat16), (128, torch.bfloat16), (48, torch.float32), (32, torch.bfloat16)])
+def test_scores_of_minus_infinity(hs, dtype, impl):
+    """Keys whose scores are minus infinity have no weight, however many of them a row meets first."""
+    heads, kv, dead, n = 4, 2, 200, 320
+    q, k, v, _ = make([n], heads, kv, hs, dtype, seed=9)
+    q, k, v = q.abs() + 0.1, k.clone(), v.clone()
+    k[:dead] = 0.0
+    k.view(n, kv, hs)[:dead, :, 3] = -math.inf
+    o, lse = B.attention_packed(q, k, v, cu_of([n]), heads, kv, impl=impl)
+    rest = [t[dead:].contiguous() for t in (q, k, v)]
+    ro, rl, bo, bl = R.forward(*rest, [n - dead], heads, kv)
+    assert bool(((o[dead:].double() - ro).abs() <= bo).all())
+    assert bool(((lse[:, dead:].double() - rl).abs() <= bl).all())
+    assert bool(o[:dead].isnan().all()) and bool((lse[:, :dead] == -math.inf).all())
+    assert B.device_status() == 0
+
+
 def test_strides_and_alignment():
     """Views with odd pitches and offsets take the CUDA-core kernel and give the same values."""
     lens, heads, kv, hs = [50, 90], 2, 1, 64
