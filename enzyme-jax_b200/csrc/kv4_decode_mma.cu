@@ -59,6 +59,12 @@ __device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, 
                : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the first product of a sum
+__device__ __forceinline__ void mma_u8s8_new(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
 __device__ __forceinline__ void mma_u8u8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
@@ -337,16 +343,17 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
               if (!whole && !(on[s] && u + 16 * s + 2 * r + kr < c1)) kp[r] = vp[s][r] = 0u;  // may be anything
             }
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) dh[n][j] = dl[n][j] = 0;
-#pragma unroll
             for (int i = 0; i < KW; ++i) {
               const uint32_t ea = even(kw[0][i]), eb = even(kw[1][i]), oa = odd(kw[0][i]), ob = odd(kw[1][i]);
 #pragma unroll
               for (int n = 0; n < NS; ++n) {
-                mma_u8s8(dh[n], ea, eb, oa, ob, qh[n][i][0], qh[n][i][1]);
-                mma_u8s8(dl[n], ea, eb, oa, ob, ql[n][i][0], ql[n][i][1]);
+                if (i == 0) {
+                  mma_u8s8_new(dh[n], ea, eb, oa, ob, qh[n][i][0], qh[n][i][1]);
+                  mma_u8s8_new(dl[n], ea, eb, oa, ob, ql[n][i][0], ql[n][i][1]);
+                } else {
+                  mma_u8s8(dh[n], ea, eb, oa, ob, qh[n][i][0], qh[n][i][1]);
+                  mma_u8s8(dl[n], ea, eb, oa, ob, ql[n][i][0], ql[n][i][1]);
+                }
               }
             }
 #pragma unroll
@@ -354,9 +361,11 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
               const float ks = __uint_as_float(kp[r] << 16), km = __uint_as_float(kp[r] & 0xffff0000u);
 #pragma unroll
               for (int n = 0; n < NS; ++n) {
-                const float d0 = (float)(256 * dh[n][2 * r] + dl[n][2 * r]), d1 = (float)(256 * dh[n][2 * r + 1] + dl[n][2 * r + 1]);
-                xs[n][s][2 * r] = fmaf(ks, d0 * f0[n], km * q0[n]);
-                xs[n][s][2 * r + 1] = fmaf(ks, d1 * f1[n], km * q1[n]);
+                const float2 d = make_float2((float)(256 * dh[n][2 * r] + dl[n][2 * r]), (float)(256 * dh[n][2 * r + 1] + dl[n][2 * r + 1]));
+                const float2 x = __ffma2_rn(make_float2(ks, ks), __fmul2_rn(d, make_float2(f0[n], f1[n])),
+                                            __fmul2_rn(make_float2(km, km), make_float2(q0[n], q1[n])));
+                xs[n][s][2 * r] = x.x;
+                xs[n][s][2 * r + 1] = x.y;
               }
               smax = fmaxf(smax, fabsf(__uint_as_float(vp[s][r] << 16)));
             }
@@ -409,12 +418,15 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
               const float vs = __uint_as_float(vp[s][r] << 16) * sc65, vm = __uint_as_float(vp[s][r] & 0xffff0000u);
 #pragma unroll
               for (int n = 0; n < NS; ++n) {
-                const float p0 = ex2(xs[n][s][2 * r] - m0[n]), p1 = ex2(xs[n][s][2 * r + 1] - m1[n]);
-                l0[n] += p0; l1[n] += p1;
-                c0s[n] = fmaf(p0, vm, c0s[n]); c1s[n] = fmaf(p1, vm, c1s[n]);
+                const float2 x = __fadd2_rn(make_float2(xs[n][s][2 * r], xs[n][s][2 * r + 1]), make_float2(-m0[n], -m1[n]));
+                const float2 p = make_float2(ex2(x.x), ex2(x.y));
+                const float2 l = __fadd2_rn(make_float2(l0[n], l1[n]), p);
+                const float2 c = __ffma2_rn(p, make_float2(vm, vm), make_float2(c0s[n], c1s[n]));
+                l0[n] = l.x; l1[n] = l.y;
+                c0s[n] = c.x; c1s[n] = c.y;
                 // rounded to integers in the low 16 bits of 2^23 + w, column 2t in the low half, column 2t + 1 in the high one
-                const uint32_t i0 = __float_as_uint(fmaf(p0, vs, 8388608.f)), i1 = __float_as_uint(fmaf(p1, vs, 8388608.f));
-                tr[n][r] = transpose8x8(__byte_perm(i0, i1, 0x5410u));
+                const float2 w = __ffma2_rn(p, make_float2(vs, vs), make_float2(8388608.f, 8388608.f));
+                tr[n][r] = transpose8x8(__byte_perm(__float_as_uint(w.x), __float_as_uint(w.y), 0x5410u));
               }
             }
             // now the weights of column g for keys 4t .. 4t + 3: the byte this column takes
