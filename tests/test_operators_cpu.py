@@ -40,6 +40,18 @@ def test_kv4_refusals():
     assert lib.b200_attention_decode_kv4_scratch_bytes(4, 4, 2, 64, None) == 1
 
 
+def test_kv4_refusals_by_size():
+    lib = B.lib()
+    n = ctypes.c_size_t(0)
+    size = lambda batch=4, h=4, hk=2, hs=64, page=16, width=2, dt=1, out=ctypes.byref(n): (
+        lib.b200_attention_decode_kv4_scratch_bytes_for(batch, h, hk, hs, page, width, dt, out))
+    assert size(h=3) == 2 and size(batch=-1) == 2 and size(page=0) == 2 and size(width=-1) == 2 and size(out=None) == 1
+    dec = lambda page=16, width=2, b=1: lib.b200_attention_decode_kv4(
+        P, P, P, P, P, P, P, 1 << 30, b, 4, 2, 64, 256, 256, 4, page, width, 1, 0, None)
+    assert dec(page=1 << 30) == 2                       # more rows than a page may have
+    assert dec(page=1 << 20, width=1 << 14, b=1 << 12) == 2   # page tables that are too long together
+
+
 def test_copy_pages_refusals():
     f = B.lib().b200_copy_pages
     call = lambda pool=P, planes=2, pages=4, heads=2, page=16, row=128, src=P, n=1, table=None, entries=0, pmap=None: f(
