@@ -9,10 +9,13 @@
 //   q.k = s sum q n + m sum q              o = sum_j (s_j p_j) n_j + sum_j p_j m_j
 // The 16 rows of an A operand are 16 keys (q.k) or 16 head dimensions (p.v); its 8 columns are four query heads twice,
 // because the other operand is a 16-bit integer in two bytes: query elements in steps of 1/32512 of their head's largest
-// (two products), weights s p -- kept in fp32 until then -- in steps of 2^-16 of a reference that is at most 8 times the
-// largest (columns 0..3 take the high bytes, 4..7 the low bytes of the same heads).  Sums of products are exact; they are
-// brought into fp32 when a reference changes and at the end.  Five to eight heads are two such sets over the same codes,
-// larger groups are cut into subsets of eight.
+// (two products), weights s p -- kept in fp32 until then -- in steps of 1/65535 of a power of two that is at most twice the
+// largest of a tile of 32 keys and a head (columns 0..3 take the high bytes, 4..7 the low bytes of the same heads).  So a
+// weight is rounded against its own tile, by 2^-16 of the largest there: a key that carries most of a head's weight, or a
+// value row of a far larger scale, costs the long tail of the others nothing.  (One step for all tiles, from the largest
+// weight so far, read every row far below it as its minimum.)  Sums of a tile's products are exact integers below 2^23; the
+// product starts them at the bits of the float 2^23, so that one packed subtraction makes numbers of them, which are
+// added up in fp32.  Five to eight heads are two such sets over the same codes, larger groups are cut into subsets of eight.
 // The order of the elements inside a contraction is free: a lane takes 16 contiguous bytes of a key row with the query
 // laid out to match; the values come through ldmatrix's byte transpose, which hands a lane two elements of four keys, and
 // the rows of the key operand are ordered so that one 8x8 transpose gives the lane the weights of those four.  The odd
@@ -65,10 +68,17 @@ __device__ __forceinline__ void mma_u8s8_new(int (&d)[4], uint32_t a0, uint32_t 
                : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
-__device__ __forceinline__ void mma_u8u8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// a whole sum on top of the bits of the float 2^23: below 2^23 the result, read as a float, is 2^23 + sum
+__device__ __forceinline__ void mma_u8u8_on_2p23(uint32_t (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                                 uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0x4b000000u));
+}
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -289,36 +299,16 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
         f1[n] = __shfl_sync(0xffffffffu, fs, 8 * (t & 1) + 4);
       }
 
-      int acc[NS][MT][4];
-      float m0[NS], m1[NS];                    // references of columns 2t, 2t + 1 (uniform over g): weights are <= 1
+      float2 acc[NS][MT][2];                   // elements 2 (8i + g) and the next one (held as 16 n), columns 2t, 2t + 1
+      float m0[NS], m1[NS];                    // references of columns 2t, 2t + 1 (uniform over g): p = e^(s - m) <= 1
       float l0[NS], l1[NS], c0s[NS], c1s[NS];  // this lane's share of sum p and of sum p m
-      float sc = __uint_as_float(237u << 23);  // power of two that keeps the value scales at most 1 (uniform)
-      bool kept = false;                       // s_o holds sums (uniform)
-      int tiles = 0;                           // a sum of 255 * 240 a key stays below 2^31 for 2^15 keys
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
         m0[n] = m1[n] = kLow;
         l0[n] = l1[n] = c0s[n] = c1s[n] = 0.f;
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[n][i][j] = 0;
+        for (int i = 0; i < MT; ++i) acc[n][i][0] = acc[n][i][1] = make_float2(0.f, 0.f);
       }
-      // Adds the integer sums of one set to its fp32 sums in shared memory (columns 8n .. 8n + 7), which are then scaled by
-      // e0, e1, and clears them.
-      auto keep = [&](int n, float e0, float e1) {
-        const float step = (t < 2 ? 256.f : 1.f) / 65535.f / sc;
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {  // elements 2 (8i + g) and the next one (held as 16 n), columns 2t, 2t + 1
-            float& at = s_o[warp][8 * n + 2 * t + (c & 1)][2 * (8 * i + g) + (c >> 1)];
-            const float was = kept ? at : 0.f;
-            at = fmaf((float)acc[n][i][c], (c >> 1) ? step * 0.0625f : step, was) * ((c & 1) ? e1 : e0);
-            acc[n][i][c] = 0;
-          }
-        }
-      };
 
       int u = (int)(x - s0) * kUnit + 32 * warp;  // first key of this warp's tile
       for (int left = (int)(x1 - x); left > 0; --left, u += kUnit, next_stage()) {
@@ -329,7 +319,7 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
           const uint32_t valid = s_valid[st];
           const bool on[2] = {((valid >> bit0) & 1u) != 0u, ((valid >> bit1) & 1u) != 0u};
           const bool whole = u + 32 <= c1 && on[0] && on[1];
-          float xs[NS][2][4], b0[NS], b1[NS], smax = 0.f;
+          float xs[NS][2][4], b0[NS], b1[NS];
           uint32_t vp[2][2];
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
@@ -367,7 +357,6 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
                 xs[n][s][2 * r] = x.x;
                 xs[n][s][2 * r + 1] = x.y;
               }
-              smax = fmaxf(smax, fabsf(__uint_as_float(vp[s][r] << 16)));
             }
           }
           if (!whole) {
@@ -380,7 +369,7 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
                   for (int n = 0; n < NS; ++n) xs[n][s][2 * r] = xs[n][s][2 * r + 1] = -INFINITY;
                 }
           }
-          bool raise = (++tiles & 1023) == 0 || smax * sc > 1.f;
+          bool raise = false;
 #pragma unroll
           for (int n = 0; n < NS; ++n) {
             b0[n] = fmaxf(fmaxf(xs[n][0][0], xs[n][0][2]), fmaxf(xs[n][1][0], xs[n][1][2]));
@@ -388,10 +377,7 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
             raise = raise || b0[n] > m0[n] || b1[n] > m1[n];
           }
           if (__any_sync(0xffffffffu, raise)) {
-            // Set the references 2 above the largest score, so that weights begin at 1/4 and may grow to 1, and the scales'
-            // factor so that they lie between 1/2 and 1.
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, o));
+            // The new reference is 2^8 above the largest, which fp32 does not mind and which few later keys exceed.
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
 #pragma unroll
@@ -399,39 +385,58 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
                 b0[n] = fmaxf(b0[n], __shfl_xor_sync(0xffffffffu, b0[n], o));
                 b1[n] = fmaxf(b1[n], __shfl_xor_sync(0xffffffffu, b1[n], o));
               }
-              const float n0 = b0[n] > m0[n] ? b0[n] + 2.f : m0[n], n1 = b1[n] > m1[n] ? b1[n] + 2.f : m1[n];
+              const float n0 = b0[n] > m0[n] ? b0[n] + 8.f : m0[n], n1 = b1[n] > m1[n] ? b1[n] + 8.f : m1[n];
               const float e0 = n0 == m0[n] ? 1.f : ex2(m0[n] - n0), e1 = n1 == m1[n] ? 1.f : ex2(m1[n] - n1);
               m0[n] = n0; m1[n] = n1;
               l0[n] *= e0; l1[n] *= e1; c0s[n] *= e0; c1s[n] *= e1;
-              keep(n, e0, e1);
+#pragma unroll
+              for (int i = 0; i < MT; ++i) {
+                acc[n][i][0] = __fmul2_rn(acc[n][i][0], make_float2(e0, e1));
+                acc[n][i][1] = __fmul2_rn(acc[n][i][1], make_float2(e0, e1));
+              }
             }
-            kept = true;
-            if (smax * sc > 1.f) sc = __uint_as_float((uint32_t)max(1, min(237, 253 - (int)(__float_as_uint(smax) >> 23))) << 23);
           }
-          const float sc65 = sc * 65535.f;
+          float2 w[NS][2][2], step[NS];  // weights s p of columns 2t, 2t + 1
           uint32_t wb[NS][2];
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            uint32_t tr[NS][2];
+          for (int n = 0; n < NS; ++n) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const float vs = __uint_as_float(vp[s][r] << 16) * sc65, vm = __uint_as_float(vp[s][r] & 0xffff0000u);
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
-              for (int n = 0; n < NS; ++n) {
+              for (int r = 0; r < 2; ++r) {
+                const float vs = __uint_as_float(vp[s][r] << 16), vm = __uint_as_float(vp[s][r] & 0xffff0000u);
                 const float2 x = __fadd2_rn(make_float2(xs[n][s][2 * r], xs[n][s][2 * r + 1]), make_float2(-m0[n], -m1[n]));
                 const float2 p = make_float2(ex2(x.x), ex2(x.y));
                 const float2 l = __fadd2_rn(make_float2(l0[n], l1[n]), p);
                 const float2 c = __ffma2_rn(p, make_float2(vm, vm), make_float2(c0s[n], c1s[n]));
                 l0[n] = l.x; l1[n] = l.y;
                 c0s[n] = c.x; c1s[n] = c.y;
-                // rounded to integers in the low 16 bits of 2^23 + w, column 2t in the low half, column 2t + 1 in the high one
-                const float2 w = __ffma2_rn(p, make_float2(vs, vs), make_float2(8388608.f, 8388608.f));
-                tr[n][r] = transpose8x8(__byte_perm(__float_as_uint(w.x), __float_as_uint(w.y), 0x5410u));
+                w[n][s][r] = __fmul2_rn(p, make_float2(vs, vs));
               }
-            }
-            // now the weights of column g for keys 4t .. 4t + 3: the byte this column takes
+            // exponents of the tile's largest weights: the upper halves of the two numbers in one word
+            const float t0 = fmaxf(fmaxf(w[n][0][0].x, w[n][0][1].x), fmaxf(w[n][1][0].x, w[n][1][1].x));
+            const float t1 = fmaxf(fmaxf(w[n][0][0].y, w[n][0][1].y), fmaxf(w[n][1][0].y, w[n][1][1].y));
+            uint32_t top = __byte_perm(__float_as_uint(t0), __float_as_uint(t1), 0x7632u);
 #pragma unroll
-            for (int n = 0; n < NS; ++n) wb[n][s] = __byte_perm(tr[n][0], tr[n][1], part_sel);
+            for (int o = 4; o < 32; o <<= 1) top = max2(top, __shfl_xor_sync(0xffffffffu, top, o));
+            // weights below 2^(e + 1) count 65535 2^-(e + 1) each; the exponent field is kept where both factors are
+            // normal numbers (a tile whose weights are all below 2^-111 loses bits)
+            const uint32_t f0 = max(top << 16 & 0x7f800000u, 16u << 23), f1 = max(top & 0x7f800000u, 16u << 23);
+            const uint32_t up_at = 0x477fff00u + (126u << 23), step_at = 0x37800080u - (126u << 23);  // 65535, 1/65535
+            const float2 up = make_float2(__uint_as_float(up_at - f0), __uint_as_float(up_at - f1));
+            step[n] = make_float2(__uint_as_float(step_at + f0), __uint_as_float(step_at + f1));
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              uint32_t tr[2];
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                // rounded to integers in the low 16 bits of 2^23 + w, column 2t in the low half, column 2t + 1 in the high one
+                const float2 z = __ffma2_rn(w[n][s][r], up, make_float2(8388608.f, 8388608.f));
+                tr[r] = transpose8x8(__byte_perm(__float_as_uint(z.x), __float_as_uint(z.y), 0x5410u));
+              }
+              // now the weights of column g for keys 4t .. 4t + 3: the byte this column takes
+              wb[n][s] = __byte_perm(tr[0], tr[1], part_sel);
+            }
           }
 #pragma unroll
           for (int i = 0; i < HS / 32; ++i) {  // 16 bytes of every row
@@ -441,7 +446,15 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
             for (int j = 0; j < 2; ++j) {
               const uint32_t a0 = even(y[j]), a1 = y[j] & 0xf0f0f0f0u, a2 = even(y[j + 2]), a3 = y[j + 2] & 0xf0f0f0f0u;
 #pragma unroll
-              for (int n = 0; n < NS; ++n) mma_u8u8(acc[n][2 * i + j], a0, a1, a2, a3, wb[n][0], wb[n][1]);
+              for (int n = 0; n < NS; ++n) {
+                uint32_t d[4];
+                mma_u8u8_on_2p23(d, a0, a1, a2, a3, wb[n][0], wb[n][1]);
+                const float2 base = make_float2(-8388608.f, -8388608.f);
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                  acc[n][2 * i + j][c] = __ffma2_rn(
+                      __fadd2_rn(make_float2(__uint_as_float(d[2 * c]), __uint_as_float(d[2 * c + 1])), base), step[n], acc[n][2 * i + j][c]);
+              }
             }
           }
         }
@@ -459,7 +472,15 @@ __global__ void __launch_bounds__(M_THREADS, kCtas(HS, NS))
           c0s[n] += __shfl_xor_sync(0xffffffffu, c0s[n], o);
           c1s[n] += __shfl_xor_sync(0xffffffffu, c1s[n], o);
         }
-        keep(n, 1.f, 1.f);
+        // high bytes count 256 times; the odd elements were held as 16 n
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float f = (t < 2 ? 256.f : 1.f) * (c ? 0.0625f : 1.f);
+            s_o[warp][8 * n + 2 * t][2 * (8 * i + g) + c] = acc[n][i][c].x * f;
+            s_o[warp][8 * n + 2 * t + 1][2 * (8 * i + g) + c] = acc[n][i][c].y * f;
+          }
         if (t < 2 && g == 0) {
           s_m[warp][4 * n + 2 * t] = m0[n]; s_m[warp][4 * n + 2 * t + 1] = m1[n];
           s_l[warp][4 * n + 2 * t] = l0[n]; s_l[warp][4 * n + 2 * t + 1] = l1[n];
