@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(SW * 32) kv4_decode_simt_kernel(Kv4DecodeArgs 
 #pragma unroll
       for (int g = 0; g < SG; ++g) {
         if (live[g]) {  // a row behind the end may hold anything
-          const float pr = exp_by_build(s[g] - nm);
+          const float pr = nm == -INFINITY ? 0.f : exp_by_build(s[g] - nm);  // (scores of minus infinity alone: no weight yet)
           l += pr;
           const float w = pr * __uint_as_float(vp[g] << 16);
           cmin = fmaf(pr, __uint_as_float(vp[g] & 0xffff0000u), cmin);

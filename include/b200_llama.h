@@ -422,7 +422,8 @@ B200_API int32_t b200_kv4_read(void* k, void* v, const void* codes, const void* 
                                int32_t page_size, int32_t max_pages, int32_t dtype, b200_stream_t stream);
 
 /* Decode attention over the 4-bit cache: one query row per sequence against its first ctx_lens[b] cached rows (int32
- * [batch] on the device, cut to max_pages * page_size; a sequence without rows gets zeros), grouped heads as above.
+ * [batch] on the device, cut to max_pages * page_size), grouped heads as above.  A score of minus infinity (fp32 overflow)
+ * has no weight; a sequence without rows, or without a score above minus infinity, gets zeros.
  * q, o [batch, ldq / ldo] of `dtype`.  scratch: b200_attention_decode_kv4_scratch_bytes() bytes, 16-byte aligned, used by
  * this call alone while it runs; b200_attention_decode_kv4_scratch_bytes_for() says how much of that a call with these page
  * tables needs, and 0 where the tables are so short that scratch may be NULL.  Pages outside the pool are skipped and

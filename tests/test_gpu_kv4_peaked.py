@@ -192,3 +192,22 @@ def test_rows_that_read_back_as_nan(hs, half, impl):
         want, bound = reference(q[b], [x[b, :lens[b]] for x in k], [x[b, :lens[b]] for x in v], heads, impl == 0)
         ok = ((o[b].double() - want).abs() <= bound).view(hk, -1)
         assert bool(ok[1].all()) and (b == 1 or bool(ok[0].all()))
+
+
+@pytest.mark.parametrize("heads,hk,hs,dtype,impl", [(4, 2, 64, torch.bfloat16, 0), (4, 2, 128, torch.bfloat16, 0),
+                                                    (4, 2, 64, torch.bfloat16, 2), (6, 3, 48, torch.float32, 0)])
+@pytest.mark.parametrize("dead", [32, 192, 384])   # whole tiles
+def test_scores_of_minus_infinity(heads, hk, hs, dtype, impl, dead):
+    """Keys of the type's lowest value, whose scores overflow to minus infinity, have no weight, however many come first."""
+    g = torch.Generator(device=DEV).manual_seed(9)
+    n, page = 400, 16
+    k, v = rows(g, 2, n, hk, hs, 0.02, 0.2, 0.0), rows(g, 2, n, hk, hs, 0.05, 0.35, 1.0)
+    q = (torch.rand(2, heads * hs, generator=g, device=DEV) + 0.5).to(dtype)
+    k[1][:, :dead], k[2][:, :dead] = 0.0, bf16(torch.tensor(torch.finfo(torch.bfloat16).min, device=DEV))
+    table, _ = pages_of(2, n, page, seed=9)
+    codes, params = pool_of(k, v, table, page)
+    o = B.attention_decode_kv4(q, codes, params, table, torch.tensor([n, dead], dtype=torch.int32, device=DEV), heads, impl=impl)
+    assert B.device_status() == 0
+    want, bound = reference(q[0], [x[0, dead:] for x in k], [x[0, dead:] for x in v], heads, impl == 0 and dtype == torch.bfloat16)
+    assert bool(((o[0].double() - want).abs() <= bound).all())
+    assert bool((o[1] == 0).all())
