@@ -669,7 +669,7 @@ class PageAllocator:
 
     def refs(self, page: int) -> int:
         """Number of holders of a page (0: free)."""
-        return self._refs.get(page, 0)
+        return self._refs.get(int(page), 0)
 
     def alloc(self, n: int):
         if n > len(self._free):
@@ -678,6 +678,11 @@ class PageAllocator:
         for p in pages:
             self._refs[p] = 1
         return pages
+
+    @staticmethod
+    def _numbers(pages):
+        """Page numbers as plain ints: elements of a tensor or an array count as the numbers they hold."""
+        return [int(p) for p in pages]
 
     def _held(self, pages) -> None:
         counts: Dict[int, int] = {}
@@ -689,7 +694,7 @@ class PageAllocator:
 
     def free(self, pages) -> None:
         """Gives pages back, once per entry; all of them or, when one is not held, none."""
-        pages = list(pages)
+        pages = self._numbers(pages)
         self._held(pages)
         gone = []
         for p in pages:
@@ -701,7 +706,7 @@ class PageAllocator:
 
     def share(self, pages) -> None:
         """Adds one holder to each of the pages."""
-        pages = list(pages)
+        pages = self._numbers(pages)
         for p in pages:
             if p not in self._refs:
                 raise B200Error(1, f"page {p} is not an allocated page of this pool")
@@ -712,7 +717,7 @@ class PageAllocator:
         """Pages of a second sequence that begins with the first ``length`` rows of the sequence on ``pages``: full pages
         are shared, a partly filled last one gets a page of its own.  Returns ``(new_pages, copies)``; ``copies`` is a
         list of at most one ``(src, dst, rows)`` for :func:`copy_pages`."""
-        pages = list(pages)
+        pages = self._numbers(pages)
         if length < 0 or page_size <= 0 or length > len(pages) * page_size:
             raise B200Error(2, f"{length} rows do not fit {len(pages)} pages of {page_size}")
         full, rest = divmod(length, page_size)

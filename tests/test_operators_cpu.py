@@ -116,6 +116,24 @@ def test_allocator_compacts():
     assert a.refs(page_map[z[1]]) == 1
 
 
+def test_allocator_takes_page_numbers_of_any_integer_kind():
+    a = B.PageAllocator(6)
+    x = torch.tensor(a.alloc(4), dtype=torch.int32)
+    assert a.refs(x[1]) == 1
+    a.free(x[2:])                                   # a row of a page table, its elements 0-d tensors
+    assert a.free_pages == 4
+    a.share(x[:1])
+    child, copies = a.fork(x[:2], 20, 16)
+    assert child[0] == int(x[0]) and a.refs(int(x[0])) == 3 and copies[0][0] == int(x[1])
+    assert all(type(p) is int for p in child)
+    a.free(x[:2].numpy())
+    a.free([x[0]])
+    a.free(child)
+    assert a.free_pages == 6 and sorted(a.alloc(6)) == list(range(6))
+    with pytest.raises(B.B200Error):
+        a.free(torch.tensor([6]))
+
+
 def test_reference_gradient_against_differences():
     g = torch.Generator().manual_seed(0)
     lens, heads, kv, hs = [5, 1, 7], 4, 2, 8
