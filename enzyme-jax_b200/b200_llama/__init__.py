@@ -589,10 +589,14 @@ def _copy_pages(what, pool, src, dst, rows, page_table, page_map) -> None:
     if page_map is not None and page_map.numel() != n_pages:
         raise B200Error(2, f"{what}: page_map has {page_map.numel()} entries for {n_pages} pages")
     dev = _device_of(what, "pool src dst rows page_table page_map", pool, src, dst, rows, page_table, page_map)
-    if pool.numel() == 0:
-        return
+    n = src.numel()
+    if pool.numel() == 0:  # nothing to copy, but the table may have to follow the pages
+        if page_table is None:
+            return
+        planes = n_heads = page_size = row = 1
+        n = 0
     _call(dev, lib().b200_copy_pages, pool.data_ptr(), planes, n_pages, n_heads, page_size, row * pool.element_size(),
-          src.data_ptr(), dst.data_ptr(), _ptr(rows), src.numel(), _ptr(page_table),
+          src.data_ptr(), dst.data_ptr(), _ptr(rows), n, _ptr(page_table),
           0 if page_table is None else page_table.numel(), _ptr(page_map))
 
 
@@ -633,8 +637,9 @@ def compact_pages(pools, src, dst, page_table: torch.Tensor, page_map) -> None:
         _check_copies(what, pools[0].shape[-4] if pools[0].dim() >= 4 else 0, src, dst)
     src, dst = _page_list(what, "src", src, dev), _page_list(what, "dst", dst, dev)
     page_map = _page_list(what, "page_map", page_map, dev)
-    for i, pool in enumerate(pools):  # the table follows in the last pool's launch
-        last = i == len(pools) - 1
+    moved = [p for p in pools if p.numel()] or pools[-1:]
+    for i, pool in enumerate(moved):  # the table follows in the last pool's launch
+        last = i == len(moved) - 1
         _copy_pages(what, pool, src, dst, None, page_table if last else None, page_map if last else None)
 
 

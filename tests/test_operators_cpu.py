@@ -134,6 +134,27 @@ def test_allocator_takes_page_numbers_of_any_integer_kind():
         a.free(torch.tensor([6]))
 
 
+@pytest.fixture
+def launches(monkeypatch):
+    """The arguments of every call that would go to the library, with tensors of the host in the place of the device's."""
+    made = []
+    monkeypatch.setattr(B, "_device_of", lambda what, names, *tensors: torch.device("cpu"))
+    monkeypatch.setattr(B, "_page_list", lambda what, name, x, dev: torch.as_tensor(x, dtype=torch.int32))
+    monkeypatch.setattr(B, "_call", lambda dev, fn, *args: made.append(args))
+    return made
+
+
+def test_compact_rewrites_the_table_whatever_the_pools_hold(launches):
+    full, empty = torch.zeros(2, 6, 2, 4, 8), torch.zeros(0, 6, 2, 4, 8)
+    table = torch.tensor([[5, 4]], dtype=torch.int32)
+    for pools, copies in (([full, empty], [2]), ([empty, full], [2]), ([full, full], [2, 2]), ([empty], [0])):
+        launches.clear()
+        B.compact_pages(pools, [5, 4], [0, 1], table, [0, 1, 2, 3, 1, 0])
+        assert [a[9] for a in launches] == copies             # copies of each launch
+        assert [a[11] for a in launches] == [0] * (len(copies) - 1) + [2]   # and table entries: once, with the last
+        assert all(min(a[1:6]) > 0 for a in launches)
+
+
 def test_reference_gradient_against_differences():
     g = torch.Generator().manual_seed(0)
     lens, heads, kv, hs = [5, 1, 7], 4, 2, 8
