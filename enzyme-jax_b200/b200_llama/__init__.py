@@ -577,25 +577,30 @@ def _page_list(what: str, name: str, x, dev) -> torch.Tensor:
     return torch.tensor([int(i) for i in x], dtype=torch.int32, device=dev)
 
 
-def _copy_pages(what, pool, src, dst, rows, page_table, page_map) -> None:
+def _check_pool(what, pool, src, dst, rows, page_table, page_map) -> None:
+    """Everything that can be refused about one pool of a call, before any of its pools is touched."""
     if pool.dim() < 4 or not pool.is_contiguous():
         raise B200Error(2, f"{what}: the pool must be contiguous [..., n_pages, n_heads, page_size, row]")
-    n_pages, n_heads, page_size, row = pool.shape[-4:]
-    planes = 1
-    for d in pool.shape[:-4]:
-        planes *= d
+    n_pages = pool.shape[-4]
     if src.numel() != dst.numel() or (rows is not None and rows.numel() != src.numel()):
         raise B200Error(2, f"{what}: src, dst and rows must have one entry per copy")
     if page_map is not None and page_map.numel() != n_pages:
         raise B200Error(2, f"{what}: page_map has {page_map.numel()} entries for {n_pages} pages")
-    dev = _device_of(what, "pool src dst rows page_table page_map", pool, src, dst, rows, page_table, page_map)
+    _device_of(what, "pool src dst rows page_table page_map", pool, src, dst, rows, page_table, page_map)
+
+
+def _copy_pages(what, pool, src, dst, rows, page_table, page_map) -> None:
+    n_pages, n_heads, page_size, row = pool.shape[-4:]
+    planes = 1
+    for d in pool.shape[:-4]:
+        planes *= d
     n = src.numel()
     if pool.numel() == 0:  # nothing to copy, but the table may have to follow the pages
         if page_table is None:
             return
         planes = n_heads = page_size = row = 1
         n = 0
-    _call(dev, lib().b200_copy_pages, pool.data_ptr(), planes, n_pages, n_heads, page_size, row * pool.element_size(),
+    _call(pool.device, lib().b200_copy_pages, pool.data_ptr(), planes, n_pages, n_heads, page_size, row * pool.element_size(),
           src.data_ptr(), dst.data_ptr(), _ptr(rows), n, _ptr(page_table),
           0 if page_table is None else page_table.numel(), _ptr(page_map))
 
@@ -614,8 +619,9 @@ def copy_pages(pool: torch.Tensor, src, dst, rows=None) -> None:
     elif any(lists):
         raise B200Error(1, f"{what}: give src and dst both as lists or both as CUDA tensors")
     rows = None if rows is None else _page_list(what, "rows", rows, pool.device)
-    _copy_pages(what, pool, _page_list(what, "src", src, pool.device), _page_list(what, "dst", dst, pool.device), rows,
-                None, None)
+    src, dst = _page_list(what, "src", src, pool.device), _page_list(what, "dst", dst, pool.device)
+    _check_pool(what, pool, src, dst, rows, None, None)
+    _copy_pages(what, pool, src, dst, rows, None, None)
 
 
 def compact_pages(pools, src, dst, page_table: torch.Tensor, page_map) -> None:
@@ -637,6 +643,8 @@ def compact_pages(pools, src, dst, page_table: torch.Tensor, page_map) -> None:
         _check_copies(what, pools[0].shape[-4] if pools[0].dim() >= 4 else 0, src, dst)
     src, dst = _page_list(what, "src", src, dev), _page_list(what, "dst", dst, dev)
     page_map = _page_list(what, "page_map", page_map, dev)
+    for pool in pools:
+        _check_pool(what, pool, src, dst, None, page_table, page_map)
     moved = [p for p in pools if p.numel()] or pools[-1:]
     for i, pool in enumerate(moved):  # the table follows in the last pool's launch
         last = i == len(moved) - 1

@@ -155,6 +155,16 @@ def test_compact_rewrites_the_table_whatever_the_pools_hold(launches):
         assert all(min(a[1:6]) > 0 for a in launches)
 
 
+def test_a_refused_compaction_moves_nothing(launches):
+    good, other = torch.zeros(2, 6, 2, 4, 8), torch.zeros(2, 6, 2, 4, 16)[..., ::2]
+    table = torch.tensor([[5, 4]], dtype=torch.int32)
+    with pytest.raises(B.B200Error):
+        B.compact_pages([good, other], [5], [0], table, [0, 1, 2, 3, 4, 0])      # the second pool is not contiguous
+    with pytest.raises(B.B200Error):
+        B.compact_pages([good, good], [5], [0], table, [0, 1, 2, 3, 4])          # the map names five pages of six
+    assert not launches
+
+
 def test_reference_gradient_against_differences():
     g = torch.Generator().manual_seed(0)
     lens, heads, kv, hs = [5, 1, 7], 4, 2, 8
