@@ -564,7 +564,9 @@ int32_t check_pool(const char* what, const Kv4Pool& p) {
   return fail(B200_ERR_BAD_SHAPE, "%s: head size %d is not one of 16/32/48/64/128", what, p.head_size);
 }
 int32_t check_pool_ptrs(const char* what, const Kv4Pool& p) {
-  if (!p.codes || !p.params || !p.table) return fail(B200_ERR_INVALID_ARG, "%s: null operand", what);
+  // (memory of no bytes may have no address: a pool without pages, page tables without columns)
+  if ((p.n_pages > 0 && (!p.codes || !p.params)) || (p.max_pages > 0 && !p.table))
+    return fail(B200_ERR_INVALID_ARG, "%s: null operand", what);
   if ((reinterpret_cast<uintptr_t>(p.codes) | reinterpret_cast<uintptr_t>(p.params)) & 3u)
     return fail(B200_ERR_MISALIGNED, "%s: codes and params must be 4-byte aligned", what);
   return B200_OK;

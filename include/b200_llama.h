@@ -410,7 +410,8 @@ B200_API int32_t b200_attention_packed_backward(const void* q, const void* k, co
  * b200_kv4_append quantises packed rows k, v [rows, ldk / ldv] into the pages: row t of sequence s (cu_seqlens as above)
  * becomes its row ctx_before[s] + t - cu_seqlens[s] (ctx_before NULL: 0).  A decode step is n_seqs = rows with
  * cu_seqlens = 0, 1, 2, ...  No two rows of a call may have the same place.  b200_kv4_read is the way back, to k, v of
- * `dtype`.  page_table int32 [n_seqs, max_pages].  Positions behind the page table and page ids outside the pool are
+ * `dtype`.  page_table int32 [n_seqs, max_pages]; pools without pages
+ * and tables without columns are fine and may be NULL.  Positions behind the page table and page ids outside the pool are
  * skipped; b200_device_status then answers B200_ERR_INVALID_ARG. */
 B200_API int32_t b200_kv4_append(const void* k, const void* v, void* codes, void* params, const int32_t* page_table,
                                  const int32_t* cu_seqlens, const int32_t* ctx_before, int32_t n_seqs, int32_t rows,
@@ -426,7 +427,7 @@ B200_API int32_t b200_kv4_read(void* k, void* v, const void* codes, const void* 
  * has no weight; a sequence without rows, or without a score above minus infinity, gets zeros.
  * q, o [batch, ldq / ldo] of `dtype`.  scratch: b200_attention_decode_kv4_scratch_bytes() bytes, 16-byte aligned, used by
  * this call alone while it runs; b200_attention_decode_kv4_scratch_bytes_for() says how much of that a call with these page
- * tables needs, and 0 where the tables are so short that scratch may be NULL.  Pages outside the pool are skipped and
+ * tables needs, and 0 where the tables are so short that scratch may be NULL (if given, it still has its full size).  Pages outside the pool are skipped and
  * reported as above.  impl: 0 = pick, 1 = tensor cores (bf16, head size 64 or 128, page_size a multiple of 16), 2 = CUDA
  * cores. */
 B200_API int32_t b200_attention_decode_kv4_scratch_bytes(int32_t batch, int32_t n_heads, int32_t n_kv_heads,

@@ -17,3 +17,32 @@ def test_compact_with_a_pool_that_holds_nothing(order):
     assert B.device_status() == 0 and table.tolist() == [[0, 1, 2, -1]]
     if 0 in order:
         assert full[0, :, 0, 0, 0].tolist() == [5, 4, 2, 3, 4, 5]
+
+
+@pytest.mark.parametrize("batch,heads,hk,hs,dtype", [(3, 4, 2, 64, torch.bfloat16), (700, 32, 8, 128, torch.bfloat16),
+                                                     (2, 6, 6, 48, torch.float32)])
+@pytest.mark.parametrize("n_pages", [0, 2])
+def test_page_tables_without_columns(batch, heads, hk, hs, dtype, n_pages):
+    """A cache that holds nothing yet: every sequence has zero rows and gets zeros; appended rows have no place."""
+    codes, params = B.new_kv4_pages(1, n_pages, hk, 16, hs)
+    table = torch.zeros(batch, 0, dtype=torch.int32, device=DEV)
+    ctx = torch.zeros(batch, dtype=torch.int32, device=DEV)
+    q = torch.randn(batch, heads * hs, device=DEV).to(dtype)
+    o = B.attention_decode_kv4(q, codes[0], params[0], table, ctx, heads, out=torch.full_like(q, 7.0))
+    assert B.device_status() == 0 and bool((o == 0).all())
+    none = torch.zeros(batch + 1, dtype=torch.int32, device=DEV)
+    kv = torch.randn(2, hk * hs, device=DEV).to(dtype)
+    B.kv4_append(kv, kv, codes[0], params[0], table, none)
+    assert B.device_status() == 0
+    none[-1] = 2
+    B.kv4_append(kv, kv, codes[0], params[0], table, none)
+    with pytest.raises(B.B200Error) as e:
+        B.device_status()
+    assert e.value.status == 1 and bool((params == 0).all())
+    # a pool without pages under tables that name some: skipped and reported
+    if n_pages == 0:
+        table = torch.zeros(batch, 1, dtype=torch.int32, device=DEV)
+        o = B.attention_decode_kv4(q, codes[0], params[0], table, ctx + 3, heads, out=torch.full_like(q, 7.0))
+        with pytest.raises(B.B200Error) as e:
+            B.device_status()
+        assert e.value.status == 1 and bool((o == 0).all())
