@@ -512,9 +512,11 @@ def kv4_read(codes: torch.Tensor, params: torch.Tensor, page_table: torch.Tensor
 
 
 @functools.lru_cache(maxsize=256)
-def _kv4_scratch_bytes(*sizes: int) -> int:
+def _kv4_scratch_bytes(device: int, *sizes: int) -> int:
+    """Scratch of a step on one device: the shares of a step go by its number of SMs."""
     n = c_size_t(0)
-    check(lib().b200_attention_decode_kv4_scratch_bytes_for(*sizes, byref(n)))
+    with torch.cuda.device(device):
+        check(lib().b200_attention_decode_kv4_scratch_bytes_for(*sizes, byref(n)))
     return n.value
 
 
@@ -540,7 +542,8 @@ def attention_decode_kv4(q: torch.Tensor, codes: torch.Tensor, params: torch.Ten
     out, ldo = _rows_or_new(what, "out", out, n_heads * hs, batch, q.dtype, dev)
     max_pages, dt = page_table.shape[1], _dt(q.dtype)
     if scratch is None:
-        size, at = _kv4_scratch_bytes(batch, n_heads, n_kv_heads, hs, page_size, max_pages, dt), None
+        size = _kv4_scratch_bytes(dev.index, batch, n_heads, n_kv_heads, hs, page_size, max_pages, dt)
+        at = None
         if size:
             scratch = torch.empty(size, dtype=torch.uint8, device=dev)
             at = scratch.data_ptr()

@@ -165,6 +165,37 @@ def test_a_refused_compaction_moves_nothing(launches):
     assert not launches
 
 
+def test_decode_scratch_goes_by_the_device_of_the_tensors(monkeypatch):
+    """Devices may differ in their number of SMs, and the current one need not be the tensors'."""
+    current = [0]
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *exc):
+            current[0] = self.before
+
+    class Lib:
+        @staticmethod
+        def b200_attention_decode_kv4_scratch_bytes_for(*args):
+            args[-1]._obj.value = 1000 * (current[0] + 1)
+            return 0
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(B, "lib", lambda: Lib)
+    sizes = (2, 4, 2, 64, 16, 40, 1)
+    B._kv4_scratch_bytes.cache_clear()
+    try:
+        assert [B._kv4_scratch_bytes(d, *sizes) for d in (0, 1, 0, 1)] == [1000, 2000, 1000, 2000]
+    finally:
+        B._kv4_scratch_bytes.cache_clear()
+    assert current == [0]
+
+
 def test_reference_gradient_against_differences():
     g = torch.Generator().manual_seed(0)
     lens, heads, kv, hs = [5, 1, 7], 4, 2, 8
