@@ -336,6 +336,9 @@ def _call(dev: torch.device, fn, *args) -> None:
         check(status)
 
 
+_INT32_MAX = 0x7FFFFFFF
+
+
 def _rows(what: str, name: str, t: torch.Tensor, cols: int, rows: Optional[int] = None,
           dtype: Optional[torch.dtype] = None) -> int:
     """Row pitch of a [rows, cols] tensor with unit column stride."""
@@ -352,6 +355,8 @@ def _rows(what: str, name: str, t: torch.Tensor, cols: int, rows: Optional[int] 
         return max(cols, 1)
     if unit != 1 or ld < cols:
         raise B200Error(2, f"{what}: {name} needs unit column stride and rows that do not overlap")
+    if ld > _INT32_MAX or shape[0] > _INT32_MAX:  # (a foreign call takes the low 32 bits without a word)
+        raise B200Error(2, f"{what}: {name} has {shape[0]} rows of pitch {ld}, more than 32 bits hold")
     return ld
 
 
@@ -584,7 +589,9 @@ def _check_pool(what, pool, src, dst, rows, page_table, page_map) -> None:
     """Everything that can be refused about one pool of a call, before any of its pools is touched."""
     if pool.dim() < 4 or not pool.is_contiguous():
         raise B200Error(2, f"{what}: the pool must be contiguous [..., n_pages, n_heads, page_size, row]")
-    n_pages = pool.shape[-4]
+    n_pages, n_heads, page_size, row = pool.shape[-4:]
+    if max(n_pages, page_size * n_heads * row * pool.element_size()) > _INT32_MAX:
+        raise B200Error(2, f"{what}: {n_pages} pages of [{n_heads}, {page_size}, {row}] {pool.dtype}: a page exceeds 2 GiB")
     if src.numel() != dst.numel() or (rows is not None and rows.numel() != src.numel()):
         raise B200Error(2, f"{what}: src, dst and rows must have one entry per copy")
     if page_map is not None and page_map.numel() != n_pages:

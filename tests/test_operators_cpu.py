@@ -196,6 +196,19 @@ def test_decode_scratch_goes_by_the_device_of_the_tensors(monkeypatch):
     assert current == [0]
 
 
+def test_pitches_and_pages_past_32_bits_are_refused(launches):
+    """Sizes go to the library in 32 bits; what does not fit is refused, not cut to its low half."""
+    wide = torch.empty(2, (1 << 32) + 64, dtype=torch.bfloat16, device="meta")[:, :64]
+    with pytest.raises(B.B200Error) as e:
+        B._rows("x", "q", wide, 64)
+    assert e.value.status == 2
+    assert B._rows("x", "q", torch.empty(2, (1 << 31) - 1, dtype=torch.uint8, device="meta")[:, :64], 64) == (1 << 31) - 1
+    pool = torch.empty(1, 2, 1, 1, (1 << 32) + 64, dtype=torch.uint8, device="meta")
+    with pytest.raises(B.B200Error) as e:
+        B.copy_pages(pool, [0], [1])
+    assert e.value.status == 2 and not launches
+
+
 def test_reference_gradient_against_differences():
     g = torch.Generator().manual_seed(0)
     lens, heads, kv, hs = [5, 1, 7], 4, 2, 8
