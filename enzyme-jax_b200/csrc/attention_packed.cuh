@@ -114,7 +114,7 @@ __device__ __noinline__ void packed_fwd_row(const T* q, const T* k, const T* v, 
     const float s = row_dot<T, HS>(q, k + (size_t)u * ldk) * scale;
     const float nm = fmaxf(m, s);
     const float corr = m == nm ? 1.f : exp_by_build(m - nm);
-    const float p = nm == -INFINITY ? 0.f : exp_by_build(s - nm);  // (a score of minus infinity has no weight)
+    const float p = nm == -INFINITY && s == s ? 0.f : exp_by_build(s - nm);  // (a score of minus infinity has no weight, a NaN is one)
     l = l * corr + p;
 #pragma unroll
     for (int i = 0; i < N; ++i)

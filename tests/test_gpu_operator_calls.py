@@ -1,4 +1,6 @@
 """Calls of the packed, 4-bit and page operators at the edges of what their documentation allows."""
+import math
+
 import pytest
 import torch
 
@@ -46,3 +48,29 @@ def test_page_tables_without_columns(batch, heads, hk, hs, dtype, n_pages):
         with pytest.raises(B.B200Error) as e:
             B.device_status()
         assert e.value.status == 1 and bool((o == 0).all())
+
+
+@pytest.mark.parametrize("impl", [0, 2])
+@pytest.mark.parametrize("hs,dtype", [(64, torch.bfloat16), (128, torch.bfloat16), (48, torch.float32)])
+@pytest.mark.parametrize("what", ["q", "k"])
+def test_a_nan_in_the_first_key_or_a_query(what, hs, dtype, impl):
+    """A score that is NaN makes its row NaN, also where it is the first one the row meets; other sequences are untouched."""
+    g = torch.Generator(device=DEV).manual_seed(0)
+    lens, heads, kv = [30, 200, 170], 4, 2
+    q, k, v = (torch.randn(400, n * hs, generator=g, device=DEV).to(dtype) for n in (heads, kv, kv))
+    cu = torch.tensor([0, 30, 230, 400], dtype=torch.int32, device=DEV)
+    clean, clean_lse = B.attention_packed(q, k, v, cu, heads, kv, impl=impl)
+    if what == "k":
+        k[30, 3] = math.nan                       # key head 0: query heads 0 and 1 of the second sequence
+        rows, cols = slice(30, 230), slice(0, 2 * hs)
+    else:
+        q[130, 3] = math.nan                      # query head 0
+        rows, cols = slice(130, 131), slice(0, hs)
+    o, lse = B.attention_packed(q, k, v, cu, heads, kv, impl=impl)
+    assert B.device_status() == 0
+    bad = torch.zeros_like(o, dtype=torch.bool)
+    bad[rows, cols] = True
+    assert torch.equal(o.isnan(), bad) and torch.equal(o[~bad], clean[~bad])
+    bad_lse = torch.zeros_like(lse, dtype=torch.bool)
+    bad_lse[:cols.stop // hs, rows] = True
+    assert torch.equal(lse.isnan(), bad_lse) and torch.equal(lse[~bad_lse], clean_lse[~bad_lse])
