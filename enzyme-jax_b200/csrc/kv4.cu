@@ -415,6 +415,7 @@ __global__ void __launch_bounds__(SW * 32) kv4_decode_simt_kernel(Kv4DecodeArgs 
       }
       const float nm = fmaxf(m, bm);
       const float corr = m == nm ? 1.f : exp_by_build(m - nm);
+      const float ref = nm == -INFINITY ? 0.f : nm;  // scores of minus infinity alone: no weight yet (a NaN keeps its own)
       l *= corr;
       cmin *= corr;
 #pragma unroll
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__(SW * 32) kv4_decode_simt_kernel(Kv4DecodeArgs 
 #pragma unroll
       for (int g = 0; g < SG; ++g) {
         if (live[g]) {  // a row behind the end may hold anything
-          const float pr = nm == -INFINITY ? 0.f : exp_by_build(s[g] - nm);  // (scores of minus infinity alone: no weight yet)
+          const float pr = exp_by_build(s[g] - ref);
           l += pr;
           const float w = pr * __uint_as_float(vp[g] << 16);
           cmin = fmaf(pr, __uint_as_float(vp[g] & 0xffff0000u), cmin);

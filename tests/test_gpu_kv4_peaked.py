@@ -211,3 +211,22 @@ def test_scores_of_minus_infinity(heads, hk, hs, dtype, impl, dead):
     want, bound = reference(q[0], [x[0, dead:] for x in k], [x[0, dead:] for x in v], heads, impl == 0 and dtype == torch.bfloat16)
     assert bool(((o[0].double() - want).abs() <= bound).all())
     assert bool((o[1] == 0).all())
+
+
+@pytest.mark.parametrize("heads,hk,hs,dtype,impl", [(4, 2, 64, torch.bfloat16, 0), (4, 2, 128, torch.bfloat16, 2),
+                                                    (6, 3, 48, torch.float32, 0)])
+@pytest.mark.parametrize("half", [0, 1])
+def test_first_rows_that_read_back_as_nan(heads, hk, hs, dtype, half, impl):
+    """The rows a lane meets first are NaN, before it has any number to compare with."""
+    g = torch.Generator(device=DEV).manual_seed(11)
+    n, page = 300, 16
+    k, v = rows(g, 2, n, hk, hs, 0.02, 0.2, 0.0), rows(g, 2, n, hk, hs, 0.05, 0.35, 1.0)
+    q, _ = queries(g, 2, heads, hk, hs)
+    table, _ = pages_of(2, n, page, seed=9)
+    codes, params = pool_of(k, v, table, page)
+    for pg in table[0, :9].tolist():
+        params[half, pg, 0] = math.nan        # 144 rows of sequence 0, key head 0
+    o = B.attention_decode_kv4(q.to(dtype), codes, params, table, torch.tensor([n, n], dtype=torch.int32, device=DEV), heads, impl=impl)
+    assert B.device_status() == 0
+    bad = o.view(2, hk, -1).isnan()
+    assert bool(bad[0, 0].all()) and not bool(bad[0, 1:].any()) and not bool(bad[1].any())
