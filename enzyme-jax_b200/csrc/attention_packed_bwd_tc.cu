@@ -145,7 +145,7 @@ template <int HS, int MODE, int SPLIT>
 __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
     packed_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmF0, const __grid_constant__ CUtensorMap tmF1,
                          const __grid_constant__ CUtensorMap tmX0, const __grid_constant__ CUtensorMap tmX1,
-                         const __grid_constant__ CUtensorMap tmO, PackedBwdArgs a, float scale, uint32_t* status) {
+                         const __grid_constant__ CUtensorMap tmO, const __grid_constant__ PackedBwdArgs a, float scale, uint32_t* status) {
   using C = BCfg<HS>;
   constexpr int BN = C::kBlock, NC = BN / 2;  // streamed rows per block; of them per softmax thread
   const PackedArgs& f = a.f;
@@ -602,30 +602,14 @@ __global__ void __launch_bounds__(PB_THREADS, BCfg<HS>::kCtas)
     }
     meet_peer();
     if (ok) {
-      // Zero weight times an infinity or NaN of a row that is masked here would not be zero: rows that did not come out
-      // finite are computed again over the pairs they are part of alone.  Both halves meet first, so that neither
-      // writes a row again while the other still writes it for the first time.
+      // Both halves meet before either redoes a row, which the other may still write for the first time (dQ).
       meet();
-      unsigned redo = __ballot_sync(0xffffffffu, ok && live && !finite);
-      while (redo) {
-        const int b = __ffs(redo) - 1;
-        redo &= redo - 1;
-        const int rr = g.r0 + qd * 32 + b;
-        const int first = __shfl_sync(0xffffffffu, span.first, b), last = __shfl_sync(0xffffffffu, span.last, b);
-        const bf16* kr = (const bf16*)f.k + hk * HS;
-        const bf16* vr = (const bf16*)f.v + hk * HS;
-        if (MODE == MODE_DKV) {
-          const size_t st = (size_t)hk * group * f.rows;
-          packed_dkv_row<bf16, HS>((const bf16*)f.q + hk * group * HS, kr + (size_t)rr * f.ldk, vr + (size_t)rr * f.ldv,
-                                   (const bf16*)a.d_o + hk * group * HS, f.lse + st, a.delta + st,
-                                   (bf16*)a.dk + (size_t)rr * a.lddk + hk * HS, (bf16*)a.dv + (size_t)rr * a.lddv + hk * HS,
-                                   f.ldq, a.lddo, f.rows, group, rr, first, last, scale);
-        } else {
-          const float dl = __shfl_sync(0xffffffffu, delta, b);
-          packed_dq_row<bf16, HS>((const bf16*)f.q + (size_t)rr * f.ldq + head * HS, kr, vr,
-                                  (const bf16*)a.d_o + (size_t)rr * a.lddo + head * HS, f.lse[(size_t)head * f.rows + rr], dl,
-                                  (bf16*)a.dq + (size_t)rr * a.lddq + head * HS, f.ldk, f.ldv, first, rr, scale);
-        }
+      const unsigned bad = __ballot_sync(0xffffffffu, ok && live && !finite);
+      if (bad) {
+        const int r0 = g.r0 + qd * 32, x_end = min(f.rows, g.x0 + g.per_head * BN);
+        if (MODE == MODE_DQ) redo_dq<HS>(a, bad, r0, head, g.x0, x_end, scale);
+        else if (hf == 0) redo_dkv<HS, false>(a, bad, r0, hk, g.x0, x_end, scale);
+        else redo_dkv<HS, true>(a, bad, r0, hk, g.x0, x_end, scale);
       }
     }
   }

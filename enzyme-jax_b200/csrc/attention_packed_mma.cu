@@ -397,8 +397,8 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
         }
       }
       if (live && a.lse) a.lse[(size_t)g.head * a.rows + t] = ms * 0.6931471805599453f + logf(l);
-      // Zero weight times an infinity or NaN in a row that is masked here would not be zero: rows that did not come out
-      // finite are computed again over the rows they see alone.
+      // Zero weight times an infinity or NaN in a value row that is masked here is not zero: where there is one, rows that
+      // did not come out finite are computed again over the rows they see alone.
       unsigned redo = __ballot_sync(0xffffffffu, live && !finite);
       while (redo) {
         const int r = __ffs(redo) - 1;
@@ -406,9 +406,9 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
         const int tr = g.t0 + qd * 32 + r;
         const int first = __shfl_sync(0xffffffffu, span.first, r);
         __syncwarp();
-        packed_fwd_row<bf16, HS>((const bf16*)a.q + (size_t)tr * a.ldq + g.head * HS, (const bf16*)a.k + hk * HS,
-                                 (const bf16*)a.v + hk * HS, (bf16*)a.o + (size_t)tr * a.ldo + g.head * HS,
-                                 a.lse ? a.lse + (size_t)g.head * a.rows + tr : nullptr, a.ldk, a.ldv, first, tr, scale);
+        redo_fwd<HS>((const bf16*)a.q + (size_t)tr * a.ldq + g.head * HS, (const bf16*)a.k + hk * HS, (const bf16*)a.v + hk * HS,
+                     (bf16*)a.o + (size_t)tr * a.ldo + g.head * HS, a.lse ? a.lse + (size_t)g.head * a.rows + tr : nullptr, a.ldk,
+                     a.ldv, first, tr, scale, k_base + g.first * TR, min(a.rows, k_base + (g.last + 1) * TR));
       }
     }
   }

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import b200_llama as B
+import packed_reference as R
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -74,3 +75,96 @@ def test_a_nan_in_the_first_key_or_a_query(what, hs, dtype, impl):
     bad_lse = torch.zeros_like(lse, dtype=torch.bool)
     bad_lse[:cols.stop // hs, rows] = True
     assert torch.equal(lse.isnan(), bad_lse) and torch.equal(lse[~bad_lse], clean_lse[~bad_lse])
+
+
+@pytest.mark.parametrize("heads,kv,hs", [(4, 2, 64), (4, 1, 128), (3, 3, 128)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_whole_sequences_that_are_not_finite(heads, kv, hs, bad):
+    """Every other sequence of a batch holds nothing but infinities or NaN, in every operand; many of them share tiles.  The
+    others come out as if they were alone, forward and backward, and to the bit again."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    lens = [5, 30, 1, 60, 100, 3, 1, 1, 250, 7, 129, 64, 2, 40]
+    T, cu = sum(lens), torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), dtype=torch.int32, device=DEV)
+    q, k, v, d_o = (torch.randn(T, n * hs, generator=g, device=DEV).bfloat16() for n in (heads, kv, kv, heads))
+    ro, rl, bo, bl = R.forward(q, k, v, lens, heads, kv)
+    want, bounds = R.backward(q, k, v, d_o, lens, heads, kv)
+    fine = torch.ones(T, dtype=torch.bool, device=DEV)
+    for i in range(0, len(lens), 2):
+        fine[cu[i]:cu[i + 1]] = False
+    for x in (q, k, v, d_o):
+        x[~fine] = bad
+    first = None
+    for _ in range(2):
+        o, lse = B.attention_packed(q, k, v, cu, heads, kv)
+        grads = B.attention_packed_backward(q, k, v, o, lse, d_o, cu, heads, kv)
+        assert B.device_status() == 0
+        assert bool(((o.double() - ro).abs() <= bo)[fine].all()) and not bool(o[~fine].isfinite().any())
+        assert bool(((lse.double() - rl).abs() <= bl)[:, fine].all())
+        for x, r, b in zip(grads, want, bounds):
+            assert bool(((x.double() - r).abs() <= b)[fine].all())
+        if first is not None:
+            assert all(torch.equal(x[fine], y[fine]) for x, y in zip((o,) + grads, first))
+        first = (o,) + grads
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_one_row_that_is_not_finite_in_each_operand(bad):
+    """Rows after and before it, in its own tile and in others: what does not see it is as it was, what sees it is not finite."""
+    T, heads, kv, hs = 600, 4, 2, 128
+    g = torch.Generator(device=DEV).manual_seed(2)
+    cu = torch.tensor([0, T], dtype=torch.int32, device=DEV)
+    ops = [torch.randn(T, n * hs, generator=g, device=DEV).bfloat16() for n in (heads, kv, kv, heads)]
+    o, lse = B.attention_packed(*ops[:3], cu, heads, kv)
+    clean = B.attention_packed_backward(*ops[:3], o, lse, ops[3], cu, heads, kv)
+    want, bounds = R.backward(*ops, [T], heads, kv)
+    ro, _, bo, _ = R.forward(*ops[:3], [T], heads, kv)
+    at = 300
+    for i in range(4):
+        x = [t.clone() for t in ops]
+        x[i][at, 5] = bad                                        # key or query head 0
+        oo, ll = B.attention_packed(*x[:3], cu, heads, kv)
+        dq, dk, dv = B.attention_packed_backward(*x[:3], o, lse, x[3], cu, heads, kv)
+        assert B.device_status() == 0
+        if i in (1, 2):                                          # a key or value row: rows before it do not see it
+            assert bool(((oo.double() - ro).abs() <= bo)[:at].all())
+            seen = ops[0][at:, 5] > 0 if i == 1 and bad == math.inf else slice(None)   # q < 0: a score of minus infinity, no weight
+            assert not bool(oo[at:, 5][seen].isfinite().any())
+            assert bool(((dq.double() - want[0]).abs() <= bounds[0])[:at].all())
+        else:                                                    # a query or cotangent row: later keys are not seen by it
+            for y, r, b in zip((dk, dv), want[1:], bounds[1:]):
+                assert bool(((y.double() - r).abs() <= b)[at + 1:].all())
+            rest = torch.arange(T, device=DEV) != at
+            assert bool(((dq.double() - want[0]).abs() <= bounds[0])[rest].all()) and not bool(dq[at, :hs].isfinite().any())
+        other = slice(hs, kv * hs)                               # the second key head
+        assert torch.equal(dk[:, other], clean[1][:, other]) and torch.equal(dv[:, other], clean[2][:, other])
+
+
+@pytest.mark.parametrize("what", ["k", "v"])
+def test_a_nan_does_not_cost_a_pass_over_every_row(what):
+    """One NaN in an early row, which every later row sees: they are NaN by right, and nothing is computed again for them.
+    (A pass pair by pair takes 600 to 1400 times as long as the products.)"""
+    T, heads, kv, hs = 4096, 8, 2, 128
+    g = torch.Generator(device=DEV).manual_seed(0)
+    q, k, v, d_o = (torch.randn(T, n * hs, generator=g, device=DEV).bfloat16() for n in (heads, kv, kv, heads))
+    cu = torch.tensor([0, T], dtype=torch.int32, device=DEV)
+
+    def passes():
+        o, lse = B.attention_packed(q, k, v, cu, heads, kv)
+        return (lambda: B.attention_packed(q, k, v, cu, heads, kv),
+                lambda: B.attention_packed_backward(q, k, v, o, lse, d_o, cu, heads, kv))
+
+    def time(f):
+        best = math.inf
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            f()
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    before = [time(f) for f in passes()]
+    (k if what == "k" else v)[T // 4, 3] = math.nan
+    after = [time(f) for f in passes()]
+    assert all(a < 30 * b for a, b in zip(after, before)), (before, after)
