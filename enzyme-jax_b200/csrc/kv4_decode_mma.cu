@@ -98,7 +98,6 @@ __device__ __forceinline__ uint32_t even(uint32_t x) { return x & 0x0f0f0f0fu; }
 __device__ __forceinline__ uint32_t odd(uint32_t x) { return (x >> 4) & 0x0f0f0f0fu; }
 
 template <int W> struct Words;
-template <> struct Words<1> { using V = uint32_t; };
 template <> struct Words<2> { using V = uint2; };
 template <> struct Words<4> { using V = uint4; };
 template <int W> __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&r)[W]) {
