@@ -499,8 +499,9 @@ def kv4_read(codes: torch.Tensor, params: torch.Tensor, page_table: torch.Tensor
              ctx_before: Optional[torch.Tensor], rows: int, *, dtype: torch.dtype = torch.bfloat16,
              k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None):
     """Reads cached rows back as packed k, v [rows, n_kv_heads*hs]: the way back of :func:`kv4_append` with the same
-    ``cu_seqlens`` and ``ctx_before``, e.g. the keys of a shared prefix for :func:`attention_packed`.  Rows without a
-    place are not written."""
+    ``cu_seqlens`` and ``ctx_before``.  Rows without a place are not written.  (:func:`attention_packed` takes as many
+    queries as keys: it attends to rows read back only where every one of them has a query; a single query per sequence
+    is :func:`attention_decode_kv4`.)"""
     what = "kv4_read"
     dev = _device_of(what, "codes params page_table cu_seqlens ctx_before k v",
                      codes, params, page_table, cu_seqlens, ctx_before, k, v)
@@ -530,7 +531,9 @@ def attention_decode_kv4(q: torch.Tensor, codes: torch.Tensor, params: torch.Ten
                          scratch: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Decode attention of q [batch, n_heads*hs] over one layer of a 4-bit cache.  Sequence b attends to its first
     ``ctx_lens[b]`` (int32 [batch] on the device) cached rows; zero rows give a zero output.  Query head h reads key head
-    h / (n_heads / n_kv_heads)."""
+    h / (n_heads / n_kv_heads).  bf16 heads of 64 and 128 on pages of a multiple of 16 rows take the tensor cores, where
+    query elements are held to 2^-16 of their head's largest and weights to 2^-16 of the largest of 32 neighbouring keys;
+    ``impl=2`` keeps both in fp32."""
     what = "attention_decode_kv4"
     dev = _device_of(what, "q codes params page_table ctx_lens out scratch",
                      q, codes, params, page_table, ctx_lens, out, scratch)

@@ -653,7 +653,9 @@ int32_t launch_hs(const PackedBwdArgs& a, cudaStream_t stream) {
   B200_CUDA_OK(launch_pdl(dq, dim3(f.n_heads, blocks), dim3(PB_THREADS), C::kSmem, stream, mq, mdo, mk, mv, mo, a,
                           scale, status));
   B200_LAUNCH_OK("packed_bwd_tc_kernel<dq>");
-  // Two CTAs per key tile where there are few tiles, or not many and the sequences are long enough to differ in length.
+  // Two CTAs per key tile where there are few tiles, or not many and the sequences are long on average (256 rows), so that the
+  // first keys of one make a CTA that outlasts the others.  The lengths themselves are on the device: one long sequence among
+  // many short ones is taken for a short batch, and its first tiles then end the pass alone.
   // Backward with one / two (us, heads of 128): 12 ragged documents of 32/8 heads (304 tiles) 333 / 317, 2048 tokens of 8/2
   // heads (32) 196 / 136; 8 x 1024 of 32/8 (512) 407 / 421, 64 x 128 of 32/8 (512) 216 / 246.  Heads of 64: 365 / 245 and
   // 214 / 141, 8 x 1024 of 12/6 (384) 159 / 151; 64 x 128 of 32/8 (512) 122 / 139.

@@ -20,7 +20,7 @@
 // Bound: at head size 128 a tile and block are 2 x 512 cycles of tensor pipe and 1024 cycles of exponentials (16 per
 // cycle and SM); at 64 the exponentials alone.  All waits are bounded.
 // Measured at 32/8 heads of 128: 2 x 8192 tokens 1040 to 1160 us (950 to 1057 TFLOP/s over the pairs seen, 0.56 to 0.62 of a
-// large library product; the power limit moves it), 24 ragged prompts (15,398 rows) 281 to 306 us (556 to 607 TFLOP/s: 77 % of
+// large library product; the power limit moves it), 24 ragged prompts (15,398 rows) 284 to 309 us (551 to 600 TFLOP/s: 77 % of
 // the pairs computed are seen, and a CTA's first loads and last stores stand alone).  A tile's block takes 3640 cycles: 1800
 // softmax, 250 until the product thread wakes, 1213 for P V and the next S, 380 until the softmax threads see it.  Tried and
 // slower or the same: part of the exponentials as a polynomial on the FMA lanes, sixteen softmax warps with shared rows, P

@@ -57,9 +57,11 @@ __device__ __forceinline__ long long range_start(long long units, int ctas, int 
 __device__ __forceinline__ int range_owner(long long units, int ctas, long long u) { return (int)(((u + 1) * ctas - 1) / units); }
 
 // Short tables, few segments: CTA i takes the whole of segment i (`whole`), which needs neither scratch nor a second kernel.
-// Up to this many units per segment, as long as every segment has a resident CTA.  Device time at 32/8 heads of 128, whole
-// against split and joined: 500 rows 8.2 / 8.8 us (1 sequence), 10.9 / 15.7 (16); 1000 rows 11.6 / 9.1 (1), 16.2 / 18.4 (16);
-// on the CUDA cores (6 fp32 heads of 48): 250 rows 8.3 / 8.4, 500 rows 13.9 / 8.4.  The call on the host takes 12 / 16 us.
+// Up to this many units per segment, as long as every segment has a resident CTA.  The border is where a step of few segments,
+// most of whose SMs stay idle, stops gaining; it goes by the table's length alone, so steps of many segments, which gain at
+// longer tables too, are split there.  Device time at 32/8 heads of 128, whole against split and joined: 500 rows 6.8 / 7.7 us
+// (1 sequence), 8.8 / 13.8 (16); 1000 rows 9.9 / 8.1 (1), 13.1 / 16.0 (16); on the CUDA cores (6 fp32 heads of 48): 250 rows
+// 8.3 / 8.4, 500 rows 13.9 / 8.4.  The call on the host takes 12 / 15 us.
 constexpr int kWholeUnitsMma = 4, kWholeUnitsSimt = 2;
 
 // Exclusive prefix of the sequences' unit counts into `pre` [batch + 1] and their lengths into `lens` [batch] (shared

@@ -22,10 +22,12 @@
 // elements of a value byte stay in its high half (16 n) and the factor is taken out of their sums.
 // One warp brings units of 128 keys (codes and parameters of both halves, four TMA copies per page piece) into a ring of
 // shared-memory stages and runs ahead over segment borders; four warps take 32 keys of a unit each.
-// HBM-bound: hs + 8 bytes per (key, key head), each read once.  64 sequences of 4096 rows, 32 heads of 128: 197 us back to
-// back (5.8 TB/s, 0.90 of a copy), 230 us behind a kernel that left L2 full of written lines (0.77).  16 sequences of up to 32,768 rows, 32/8 heads: 62 us (2.8
-// TB/s): at one segment per CTA the time is set-up, the first loads and the joining kernel.  Tried: codes loaded into
-// registers with four CTAs per SM (290 us where this form took 265 then), four CTAs on two stages (275 against 249).
+// HBM-bound: hs + 8 bytes per (key, key head), each read once.  64 sequences of 4096 rows, 32 heads of 128: 201 us back to
+// back (5.7 TB/s, 0.88 of a copy; 194 with one step for all tiles), 231 us behind a kernel that left L2 full of written lines
+// (0.76).  16 sequences of up to 32,768 rows, 32/8 heads: 59 us (3.0 TB/s): at one segment per CTA the time is set-up, the
+// first loads and the joining kernel.  Tried: codes loaded into registers with four CTAs per SM (290 us where this form took
+// 265 then), four CTAs on two stages (275 against 249), scores without integer conversions (their sums begun at 1.5 2^23: no
+// change).
 #include <algorithm>
 
 #include "kv4.cuh"
